@@ -257,7 +257,7 @@ def _extend(s):
     mask = fine[:, None] & (col >= have[:, None]) & (col < last[:, None])
     place = available - 1 - ((cum - need)[:, None] + col - have[:, None])
     table[mask] = free[place[mask]]
-    used = torch.where(fine, cum, torch.zeros_like(cum)).max()
+    used = torch.where(fine & (need > 0), cum, torch.zeros_like(cum)).max()
     # rows of the packed batch
     row = torch.arange(total, device=dev)
     request = torch.searchsorted(row_end, row, right=True)
