@@ -47,6 +47,8 @@ EXPORTS = (
     "ade_b200_factored_static", "ade_b200_factored_static_status", "ade_b200_recon", "ade_b200_expand_codes",
     "ade_b200_recon_expanded", "ade_b200_expand_codes_f8", "ade_b200_recon_expanded_f8", "ade_b200_set_option",
     "ade_b200_rmsnorm", "ade_b200_add_rmsnorm", "ade_b200_rope", "ade_b200_silu_mul", "ade_b200_attn_decode",
+    "ade_b200_paged_extend", "ade_b200_paged_write", "ade_b200_paged_attn", "ade_b200_paged_attn_workspace_bytes",
+    "ade_b200_multi_delta", "ade_b200_multi_delta_workspace_bytes", "ade_b200_token_logprobs",
 )
 
 
@@ -61,6 +63,20 @@ class AdeDelta(ctypes.Structure):
         ("M", ctypes.c_int), ("N", ctypes.c_int), ("r", ctypes.c_int),
         ("n_blocks", ctypes.c_int), ("block_rows", ctypes.c_int * (MAX_BLOCKS + 1)), ("block_groups", ctypes.c_int * (MAX_BLOCKS + 1)),
     ]
+
+
+class AdeDeltaBank(ctypes.Structure):
+    """struct ade_delta_bank of include/ade_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("uq", "us", "uz", "vt", "vs", "vz", "start")] + [(n, ctypes.c_int) for n in ("M", "N", "groups", "deltas")]
+
+
+# paged_extend: why a request did not grow (ADE_PAGED_* of include/ade_b200.h)
+PAGED_STATUS = {
+    1: "ADE_PAGED_NO_PAGE: no free page is left for it",
+    2: "ADE_PAGED_TABLE_FULL: it would be longer than its row of the block table",
+    3: "ADE_PAGED_NO_ROW: its new tokens do not fit the rows of the batch",
+    4: "ADE_PAGED_BAD_LENGTH: its length is negative or beyond its row of the block table",
+}
 
 
 class AdeKernelError(RuntimeError):
@@ -122,6 +138,17 @@ def load() -> ctypes.CDLL:
     lib.ade_b200_attn_decode.argtypes = [vp] * 11 + [ci] * 5 + [ll] * 5 + [ctypes.c_float, vp]
     for name in ("ade_b200_rmsnorm", "ade_b200_add_rmsnorm", "ade_b200_rope", "ade_b200_silu_mul", "ade_b200_attn_decode"):
         getattr(lib, name).restype = ci
+    lib.ade_b200_paged_extend.argtypes = [vp] * 11 + [ci, ci, ll, ci, ci, ci, vp]
+    lib.ade_b200_paged_write.argtypes = [vp] * 7 + [ci] * 5 + [ll] * 5 + [vp]
+    lib.ade_b200_paged_attn.argtypes = [vp] * 10 + [sz] + [ci] * 3 + [ll] + [ci] * 5 + [ll] * 3 + [ctypes.c_float, vp]
+    lib.ade_b200_paged_attn_workspace_bytes.argtypes = [ci] * 4
+    lib.ade_b200_multi_delta.argtypes = [vp, vp, ctypes.POINTER(AdeDeltaBank), vp, vp, vp, sz, ci, vp]
+    lib.ade_b200_multi_delta_workspace_bytes.argtypes = [ci, ci]
+    lib.ade_b200_token_logprobs.argtypes = [vp, ci, vp, vp, vp, vp, vp, ci, ci, ll, ci, vp]
+    for name in ("ade_b200_paged_extend", "ade_b200_paged_write", "ade_b200_paged_attn", "ade_b200_multi_delta", "ade_b200_token_logprobs"):
+        getattr(lib, name).restype = ci
+    for name in ("ade_b200_paged_attn_workspace_bytes", "ade_b200_multi_delta_workspace_bytes"):
+        getattr(lib, name).restype = sz
     lib.ade_b200_set_option.argtypes = [ci, ctypes.c_longlong]
     lib.ade_b200_set_option.restype = ci
     for name in ("ade_b200_pack_codes", "ade_b200_pack_zeros", "ade_b200_factored", "ade_b200_recon", "ade_b200_expand_codes",

@@ -8,6 +8,7 @@
 #include "compress.cuh"
 #include "decode_ops.cuh"
 #include "factored.cuh"
+#include "host.h"
 #include "linear_tc.cuh"
 #include "recon.cuh"
 #include "recon_strip.cuh"
@@ -333,6 +334,15 @@ int static_scratch_base(char** out) {
 }
 
 }  // namespace
+
+bool ade_host::cuda_ok(cudaError_t e) { return ::cuda_ok(e); }
+
+int ade_host::sm_count(int* sms) {
+    const DeviceInfo* di = nullptr;
+    const int rc = device_info(&di);
+    if (rc == ADE_OK) *sms = di->sms;
+    return rc;
+}
 
 extern "C" {
 

@@ -1,0 +1,325 @@
+// Paged key-value cache: page allocation and slot maps, the write of new keys and values, attention of single rows.
+//
+// A cache layer is two arrays k_pages, v_pages [pages][kv_heads][page_size][head_dim] of bfloat16.  A request owns an
+// ordered list of pages, its row of block_table [B][width]; token i of the request lives in page block_table[b][i / page_size]
+// at offset i % page_size, and slot = page * page_size + offset names that place for all layers.  No counterpart in the reference,
+// which keeps one contiguous cache per batch inside transformers (src/evaluate.py:241 calls model.generate).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ade {
+
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// ------------------------------------------------------------------ page allocation, block tables, slot maps
+constexpr int PX_THREADS = 1024;
+constexpr int PX_MAX_REQUESTS = 4096;
+constexpr int PX_ITEMS = PX_MAX_REQUESTS / PX_THREADS;       // requests per thread of the scans
+
+struct ExtendParams {
+    const int* lengths;          // [B] tokens each request has
+    const int* fresh;            // [B] tokens to add; negative: the request ends and its pages go back
+    int* table;                  // [B][width], rows table_stride apart
+    int* free_pages;             // [pages] stack of free pages
+    const int* free_count;       // its height
+    int *lengths_out, *count_out, *status;
+    long long *slots, *positions;    // [total]
+    int* requests;                   // [total]
+    int B, width, pages, page_size, total;
+    long long table_stride;
+};
+
+enum { PX_OK = 0, PX_NO_PAGE = 1, PX_TABLE_FULL = 2, PX_NO_ROW = 3, PX_BAD_LENGTH = 4 };
+
+// inclusive prefix sums over the CTA of `v`, one value per thread; `ws`: 33 words
+__device__ __forceinline__ long long px_scan(long long v, long long* ws) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) ws[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        long long s = ws[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xFFFFFFFFu, s, o);
+            if (lane >= o) s += u;
+        }
+        ws[lane] = s;
+    }
+    __syncthreads();
+    const long long base = warp ? ws[warp - 1] : 0;
+    __syncthreads();
+    return base + v;
+}
+
+// smallest b with sums[b] > i, for ascending sums
+__device__ __forceinline__ int px_find(const int* sums, int n, int i) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > i) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// One CTA.  Three prefix sums over the requests (rows of the packed batch, pages handed back, pages needed) say which row, page
+// and stack entry belongs to whom; everything behind them is independent per row and per page.  The sums are kept in 64
+// bits until they are compared with `total` and the number of pages, and saturated to 31 bits behind that.
+__global__ void __launch_bounds__(PX_THREADS) paged_extend_kernel(const ExtendParams p) {
+    extern __shared__ int px_smem[];
+    int* row_end = px_smem;              // [B] inclusive sums of the rows
+    int* back_end = row_end + p.B;       // [B] ... of the pages handed back
+    int* need_end = back_end + p.B;      // [B] ... of the pages needed
+    __shared__ long long ws[33];
+    __shared__ int s_used;
+    const int tid = threadIdx.x, b0 = tid * PX_ITEMS;
+    const long long kSat = 0x7FFFFFFF;
+    if (tid == 0) s_used = 0;
+    int len[PX_ITEMS], grow[PX_ITEMS], have[PX_ITEMS], last[PX_ITEMS], st[PX_ITEMS];
+    bool rel[PX_ITEMS];
+    const int count = min(max(*p.free_count, 0), p.pages);
+    long long rows = 0, back = 0;
+#pragma unroll
+    for (int i = 0; i < PX_ITEMS; ++i) {
+        const int b = b0 + i;
+        len[i] = grow[i] = have[i] = last[i] = 0;
+        st[i] = PX_OK;
+        rel[i] = false;
+        if (b < p.B) {
+            len[i] = p.lengths[b];
+            const int f = p.fresh[b];
+            if (len[i] < 0 || len[i] > static_cast<long long>(p.width) * p.page_size) {
+                st[i] = PX_BAD_LENGTH;
+            } else {
+                have[i] = static_cast<int>((len[i] + static_cast<long long>(p.page_size) - 1) / p.page_size);
+                rel[i] = f < 0;
+                grow[i] = max(f, 0);
+                const long long end = (static_cast<long long>(len[i]) + grow[i] + p.page_size - 1) / p.page_size;
+                if (end > p.width) st[i] = PX_TABLE_FULL;
+                last[i] = static_cast<int>(end);
+            }
+        }
+        rows += grow[i];
+        back += rel[i] ? have[i] : 0;
+    }
+    long long row_at = px_scan(rows, ws) - rows, back_at = px_scan(back, ws) - back;
+    long long need = 0;
+#pragma unroll
+    for (int i = 0; i < PX_ITEMS; ++i) {
+        const int b = b0 + i;
+        row_at += grow[i];
+        back_at += rel[i] ? have[i] : 0;
+        if (b < p.B) {
+            if (row_at > p.total && !rel[i] && st[i] != PX_BAD_LENGTH) st[i] = PX_NO_ROW;
+            row_end[b] = static_cast<int>(min(row_at, kSat));
+            back_end[b] = static_cast<int>(min(back_at, kSat));
+            if (st[i] == PX_OK && !rel[i]) need += last[i] - have[i];
+        }
+    }
+    long long need_at = px_scan(need, ws) - need;
+    const int back_total = back_end[p.B - 1];
+    const int available = static_cast<int>(min(static_cast<long long>(count) + back_total, static_cast<long long>(p.pages)));
+    int used = 0;
+#pragma unroll
+    for (int i = 0; i < PX_ITEMS; ++i) {
+        const int b = b0 + i;
+        if (b < p.B) {
+            const bool asks = st[i] == PX_OK && !rel[i] && last[i] > have[i];
+            if (asks) {
+                need_at += last[i] - have[i];
+                if (need_at > available) st[i] = PX_NO_PAGE;
+                else used = static_cast<int>(need_at);
+            }
+            need_end[b] = static_cast<int>(min(need_at, kSat));
+            p.status[b] = st[i];
+        }
+    }
+    if (used) atomicMax(&s_used, used);
+    __syncthreads();                         // every thread has read lengths and free_count: they may be the outputs
+    used = s_used;
+#pragma unroll
+    for (int i = 0; i < PX_ITEMS; ++i)
+        if (b0 + i < p.B) p.lengths_out[b0 + i] = rel[i] ? 0 : st[i] == PX_OK ? len[i] + grow[i] : len[i];
+    if (tid == 0) *p.count_out = available - used;
+    __syncthreads();                         // status and lengths_out of every request are in place
+    // entry i of the stack once the pages handed back lie on it
+    auto stack = [&](int i) {
+        if (i < count) return p.free_pages[i];
+        const int b = px_find(back_end, p.B, i - count);
+        return p.table[b * p.table_stride + (i - count - (b ? back_end[b - 1] : 0))];
+    };
+    for (int i = tid; i < available - count; i += PX_THREADS) p.free_pages[count + i] = stack(count + i);
+    // pages taken: the i-th of all comes from the i-th place below the top.  A request's own entries lie behind those it has,
+    // so no entry that is read here (a released request's) is written.
+    for (int i = tid; i < used; i += PX_THREADS) {
+        const int b = px_find(need_end, p.B, i);
+        const int first = b ? need_end[b - 1] : 0;
+        const long long len_b = p.lengths_out[b] - p.fresh[b];
+        const int col = static_cast<int>((len_b + p.page_size - 1) / p.page_size) + i - first;
+        p.table[b * p.table_stride + col] = stack(available - 1 - i);
+    }
+    // rows of the packed batch
+    for (int r = tid; r < p.total; r += PX_THREADS) {
+        long long slot = -1, pos = 0;
+        int req = -1;
+        const int b = px_find(row_end, p.B, r);
+        if (b < p.B && p.status[b] == PX_OK) {
+            const int start = b ? row_end[b - 1] : 0;
+            const int len_b = p.lengths_out[b] - p.fresh[b];
+            const int at = len_b + r - start, col = at / p.page_size;
+            const int have_b = (len_b + p.page_size - 1) / p.page_size;
+            const int page = col < have_b ? p.table[b * p.table_stride + col] : stack(available - 1 - ((b ? need_end[b - 1] : 0) + col - have_b));
+            if (page >= 0 && page < p.pages) {
+                slot = static_cast<long long>(page) * p.page_size + at % p.page_size;
+                pos = at;
+                req = b;
+            }
+        }
+        p.slots[r] = slot;
+        p.positions[r] = pos;
+        p.requests[r] = req;
+    }
+}
+
+// ------------------------------------------------------------------ keys and values of new tokens into their pages
+struct WriteParams {
+    const __nv_bfloat16 *k, *v, *cs, *sn;      // k, v [T][heads][dim] by strides; cs, sn [T][dim] or nullptr: k is stored as it is
+    const long long* slots;
+    __nv_bfloat16 *kp, *vp;
+    long long slot_count, k_row, k_head, v_row, v_head, cs_row;
+    int T, heads, dim, page_size;
+};
+
+// A thread moves sixteen dimensions of one head: eight of the first half and the eight they are rotated with.  k cos + rotate_half(k) sin
+// is formed in float32 and rounded once, to the bfloat16 that the cache stores.
+template <bool VEC>
+__global__ void __launch_bounds__(256) paged_write_kernel(const WriteParams p) {
+    constexpr int E = VEC ? 8 : 1;
+    const int half = p.dim >> 1, pieces = half / E;
+    const long long total = static_cast<long long>(p.T) * p.heads * pieces;
+    for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+        const int d = static_cast<int>(e % pieces) * E;
+        const long long th = e / pieces;
+        const int h = static_cast<int>(th % p.heads);
+        const long long t = th / p.heads, slot = p.slots[t];
+        if (slot < 0 || slot >= p.slot_count) continue;
+        const long long page = slot / p.page_size;
+        const long long to = ((page * p.heads + h) * p.page_size + (slot - page * p.page_size)) * p.dim + d;
+        const __nv_bfloat16 *kr = p.k + t * p.k_row + h * p.k_head + d, *vr = p.v + t * p.v_row + h * p.v_head + d;
+        if constexpr (VEC) {
+            auto ld = [](const __nv_bfloat16* a) { return *reinterpret_cast<const uint4*>(a); };
+            auto st = [](__nv_bfloat16* a, const uint4& w) { *reinterpret_cast<uint4*>(a) = w; };
+            uint4 a = ld(kr), b = ld(kr + half);
+            const uint4 v0 = ld(vr), v1 = ld(vr + half);
+            if (p.cs) {
+                const __nv_bfloat16 *c = p.cs + t * p.cs_row + d, *s = p.sn + t * p.cs_row + d;
+                const uint4 c0 = ld(c), c1 = ld(c + half), s0 = ld(s), s1 = ld(s + half);
+                uint32_t *aw = reinterpret_cast<uint32_t*>(&a), *bw = reinterpret_cast<uint32_t*>(&b);
+                const uint32_t *c0w = reinterpret_cast<const uint32_t*>(&c0), *c1w = reinterpret_cast<const uint32_t*>(&c1),
+                               *s0w = reinterpret_cast<const uint32_t*>(&s0), *s1w = reinterpret_cast<const uint32_t*>(&s1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float al = bf_lo(aw[i]), ah = bf_hi(aw[i]), bl = bf_lo(bw[i]), bh = bf_hi(bw[i]);
+                    aw[i] = pack_bf2(al * bf_lo(c0w[i]) - bl * bf_lo(s0w[i]), ah * bf_hi(c0w[i]) - bh * bf_hi(s0w[i]));
+                    bw[i] = pack_bf2(bl * bf_lo(c1w[i]) + al * bf_lo(s1w[i]), bh * bf_hi(c1w[i]) + ah * bf_hi(s1w[i]));
+                }
+            }
+            st(p.kp + to, a);
+            st(p.kp + to + half, b);
+            st(p.vp + to, v0);
+            st(p.vp + to + half, v1);
+        } else {
+            float a = __bfloat162float(kr[0]), b = __bfloat162float(kr[half]);
+            if (p.cs) {
+                const __nv_bfloat16 *c = p.cs + t * p.cs_row + d, *s = p.sn + t * p.cs_row + d;
+                const float ra = a * __bfloat162float(c[0]) - b * __bfloat162float(s[0]);
+                b = b * __bfloat162float(c[half]) + a * __bfloat162float(s[half]);
+                a = ra;
+            }
+            p.kp[to] = __float2bfloat16_rn(a);
+            p.kp[to + half] = __float2bfloat16_rn(b);
+            p.vp[to] = vr[0];
+            p.vp[to + half] = vr[half];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ attention of single rows over the pages of their requests
+struct PagedAttnParams {
+    const __nv_bfloat16 *q, *cs, *sn;          // q [T][q_heads][dim] by strides; cs, sn [T][dim] or nullptr: q is used as it is
+    const int* table;
+    const int* requests;                       // [T] row of the block table, outside 0 .. B - 1: the row has no request
+    const long long* positions;                // [T] the row sees positions 0 .. positions[t] of its request
+    const __nv_bfloat16 *kp, *vp;
+    __nv_bfloat16* out;                        // [T][q_heads][dim]
+    long long table_stride, q_row, q_head, cs_row;
+    int T, B, width, pages, page_size, q_heads, kv_heads, dim;
+    float scale;
+};
+
+// One CTA per (row, query head), one position per warp at a time, a running softmax per warp, the warps joined at the end.
+__global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnParams p) {
+    __shared__ float s_m[4], s_l[4], s_acc[4][256];
+    const int t = blockIdx.x / p.q_heads, h = blockIdx.x % p.q_heads, kvh = h / (p.q_heads / p.kv_heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.dim >> 5, half = p.dim >> 1;
+    const int b = p.requests[t];
+    const long long last = p.positions[t];
+    long long n = b < 0 || b >= p.B || last < 0 ? 0 : last + 1;
+    n = min(n, static_cast<long long>(p.width) * p.page_size);
+    float q[8], acc[8];
+    for (int i = 0; i < per; ++i) {
+        const int d = lane + 32 * i;
+        const __nv_bfloat16* qr = p.q + t * p.q_row + h * p.q_head;
+        q[i] = __bfloat162float(qr[d]);
+        if (p.cs) {
+            const float o = d < half ? -__bfloat162float(qr[d + half]) : __bfloat162float(qr[d - half]);
+            q[i] = q[i] * __bfloat162float(p.cs[t * p.cs_row + d]) + o * __bfloat162float(p.sn[t * p.cs_row + d]);
+        }
+        acc[i] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    for (long long j = warp; j < n; j += 4) {
+        const int page = p.table[b * p.table_stride + j / p.page_size];
+        if (page < 0 || page >= p.pages) continue;
+        const long long at = ((static_cast<long long>(page) * p.kv_heads + kvh) * p.page_size + j % p.page_size) * p.dim;
+        float s = 0.f;
+        for (int i = 0; i < per; ++i) s += q[i] * __bfloat162float(p.kp[at + lane + 32 * i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        s *= p.scale;
+        const float mn = fmaxf(m, s), f = mn == -INFINITY ? 1.f : expf(m - mn), w = mn == -INFINITY ? 0.f : expf(s - mn);
+        l = l * f + w;
+        for (int i = 0; i < per; ++i) acc[i] = acc[i] * f + w * __bfloat162float(p.vp[at + lane + 32 * i]);
+        m = mn;
+    }
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+    }
+    for (int i = 0; i < per; ++i) s_acc[warp][lane + 32 * i] = acc[i];
+    __syncthreads();
+    const float mm = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    for (int d = threadIdx.x; d < p.dim; d += 128) {
+        float num = 0.f, den = 0.f;
+        for (int w = 0; w < 4; ++w) {
+            const float f = s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - mm);
+            num += f * s_acc[w][d];
+            den += f * s_l[w];
+        }
+        p.out[(static_cast<long long>(t) * p.q_heads + h) * p.dim + d] = __float2bfloat16_rn(den > 0.f ? num / den : 0.f);
+    }
+}
+
+}  // namespace ade

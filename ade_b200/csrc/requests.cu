@@ -1,0 +1,136 @@
+// C ABI of the operators of a serving step over a batch of independent requests (declared in include/ade_b200.h): paged key-value cache,
+// attention over it, deltas of many fine-tuned models, log probabilities.  Host side only validates arguments and launches.
+#include "../../include/ade_b200.h"
+
+#include "host.h"
+#include "logprobs.cuh"
+#include "multi_delta.cuh"
+#include "paged.cuh"
+
+using ade_host::aligned16;
+using ade_host::cuda_ok;
+
+namespace {
+
+int launched() { return cuda_ok(cudaGetLastError()) ? ADE_OK : ADE_ERR_CUDA; }
+
+bool dim_ok(int head_dim) { return head_dim >= 32 && head_dim <= 256 && head_dim % 32 == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
+                          int32_t* lengths_out, int32_t* free_count_out, int32_t* status, long long* slots, long long* positions, int32_t* requests,
+                          int B, int width, long long table_row_stride, int pages, int page_size, int total, void* stream) {
+    if (!lengths || !new_tokens || !block_table || !free_pages || !free_count || !lengths_out || !free_count_out || !status) return ADE_ERR_NULL;
+    if (total > 0 && (!slots || !positions || !requests)) return ADE_ERR_NULL;
+    if (B < 1 || B > ADE_B200_MAX_REQUESTS || width < 1 || table_row_stride < width || pages < 1 || page_size < 1 || total < 0) return ADE_ERR_SHAPE;
+    if (static_cast<long long>(width) * page_size > 0x7FFFFFFFll || total > (1 << 30)) return ADE_ERR_SHAPE;
+    int sms = 0;
+    const int rc = ade_host::sm_count(&sms);
+    if (rc) return rc;
+    ade::ExtendParams p = {lengths, new_tokens, block_table, free_pages, free_count, lengths_out, free_count_out, status, slots, positions, requests,
+                           B, width, pages, page_size, total, table_row_stride};
+    const size_t smem = 3 * static_cast<size_t>(B) * sizeof(int);
+    if (smem > 40 * 1024 && !cuda_ok(cudaFuncSetAttribute(ade::paged_extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))))
+        return ADE_ERR_CUDA;
+    ade::paged_extend_kernel<<<1, ade::PX_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched();
+}
+
+int ade_b200_paged_write(const void* k, const void* v, const void* cos_t, const void* sin_t, const long long* slots, void* k_pages, void* v_pages,
+                         int T, int kv_heads, int head_dim, int pages, int page_size, long long k_row_stride, long long k_head_stride,
+                         long long v_row_stride, long long v_head_stride, long long cs_row_stride, void* stream) {
+    if (!k || !v || !slots || !k_pages || !v_pages || !cos_t != !sin_t) return ADE_ERR_NULL;
+    if (T < 1 || kv_heads < 1 || !dim_ok(head_dim) || pages < 1 || page_size < 1) return ADE_ERR_SHAPE;
+    if (k_row_stride < 0 || k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0 || cs_row_stride < 0) return ADE_ERR_SHAPE;
+    if (!aligned16(k_pages) || !aligned16(v_pages)) return ADE_ERR_ALIGN;
+    int sms = 0;
+    const int rc = ade_host::sm_count(&sms);
+    if (rc) return rc;
+    using bf = __nv_bfloat16;
+    ade::WriteParams p = {static_cast<const bf*>(k), static_cast<const bf*>(v), static_cast<const bf*>(cos_t), static_cast<const bf*>(sin_t), slots,
+                          static_cast<bf*>(k_pages), static_cast<bf*>(v_pages), static_cast<long long>(pages) * page_size, k_row_stride, k_head_stride,
+                          v_row_stride, v_head_stride, cs_row_stride, T, kv_heads, head_dim, page_size};
+    const bool vec = aligned16(k) && aligned16(v) && (!cos_t || (aligned16(cos_t) && aligned16(sin_t))) &&
+                     ((k_row_stride | k_head_stride | v_row_stride | v_head_stride | (cos_t ? cs_row_stride : 0)) & 7) == 0;
+    const long long work = static_cast<long long>(T) * kv_heads * (head_dim / 2 / (vec ? 8 : 1)), want = (work + 255) / 256;
+    const int grid = static_cast<int>(want < 16ll * sms ? want : 16ll * sms);
+    (vec ? ade::paged_write_kernel<true> : ade::paged_write_kernel<false>)<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched();
+}
+
+size_t ade_b200_paged_attn_workspace_bytes(int T, int q_heads, int kv_heads, int head_dim) {
+    return T < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || !dim_ok(head_dim) ? 0 : 16;
+}
+
+int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, const int32_t* block_table, const int32_t* requests,
+                        const long long* positions, const void* k_pages, const void* v_pages, void* out, void* work, size_t work_bytes, int T, int B,
+                        int width, long long table_row_stride, int q_heads, int kv_heads, int head_dim, int pages, int page_size,
+                        long long q_row_stride, long long q_head_stride, long long cs_row_stride, float scale, void* stream) {
+    if (!q || !block_table || !requests || !positions || !k_pages || !v_pages || !out || !cos_t != !sin_t) return ADE_ERR_NULL;
+    if (T < 1 || B < 1 || width < 1 || table_row_stride < width || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || !dim_ok(head_dim) ||
+        pages < 1 || page_size < 1 || q_row_stride < 0 || q_head_stride < 0 || cs_row_stride < 0)
+        return ADE_ERR_SHAPE;
+    if (!work) return ADE_ERR_NULL;
+    if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(work)) return ADE_ERR_ALIGN;
+    if (work_bytes < ade_b200_paged_attn_workspace_bytes(T, q_heads, kv_heads, head_dim)) return ADE_ERR_SCRATCH;
+    if (static_cast<long long>(T) * q_heads > 0x7FFFFFFFll) return ADE_ERR_SHAPE;
+    int sms = 0;
+    const int rc = ade_host::sm_count(&sms);
+    if (rc) return rc;
+    using bf = __nv_bfloat16;
+    ade::PagedAttnParams p = {static_cast<const bf*>(q), static_cast<const bf*>(cos_t), static_cast<const bf*>(sin_t), block_table, requests, positions,
+                              static_cast<const bf*>(k_pages), static_cast<const bf*>(v_pages), static_cast<bf*>(out), table_row_stride, q_row_stride,
+                              q_head_stride, cs_row_stride, T, B, width, pages, page_size, q_heads, kv_heads, head_dim, scale};
+    ade::paged_attn_kernel<<<T * q_heads, 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched();
+}
+
+size_t ade_b200_multi_delta_workspace_bytes(int T, int N) {
+    return T < 1 || T > ADE_B200_MAX_TOKENS || N < 1 ? 0 : static_cast<size_t>(T) * ADE_B200_MAX_RANK * sizeof(float);
+}
+
+int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_bank_t* bank, const int32_t* ids, void* out, void* work, size_t work_bytes,
+                         int T, void* stream) {
+    if (!x || !y_dense || !bank || !ids || !out) return ADE_ERR_NULL;
+    const ade_delta_bank_t& d = *bank;
+    if (!d.uq || !d.us || !d.uz || !d.vt || !d.vs || !d.vz || !d.start) return ADE_ERR_NULL;
+    if (T < 1 || T > ADE_B200_MAX_TOKENS || d.M < 1 || d.N < 128 || d.N % 128 || d.groups < 1 || d.deltas < 1) return ADE_ERR_SHAPE;
+    if (!work) return ADE_ERR_NULL;
+    const void* all[] = {x, y_dense, out, work, d.uq, d.us, d.uz, d.vt, d.vs, d.vz};
+    for (const void* a : all)
+        if (!aligned16(a)) return ADE_ERR_ALIGN;
+    if (work_bytes < ade_b200_multi_delta_workspace_bytes(T, d.N)) return ADE_ERR_SCRATCH;
+    int sms = 0;
+    const int rc = ade_host::sm_count(&sms);
+    if (rc) return rc;
+    using bf = __nv_bfloat16;
+    ade::MultiDeltaParams p = {static_cast<const bf*>(x), static_cast<const bf*>(y_dense), static_cast<bf*>(out), d.uq, d.uz, d.vt, d.vz,
+                               reinterpret_cast<const bf*>(d.us), reinterpret_cast<const bf*>(d.vs), d.start, ids, static_cast<float*>(work),
+                               d.M, d.N, d.groups, d.deltas, T};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    ade::multi_delta_v_kernel<<<dim3(T, d.groups < ade::MD_MAX_GROUPS ? d.groups : ade::MD_MAX_GROUPS), 256, 0, st>>>(p);
+    ade::multi_delta_u_kernel<<<dim3(T, (d.M + 255) / 256), 256, 0, st>>>(p);
+    return launched();
+}
+
+int ade_b200_token_logprobs(const void* logits, int dtype, const long long* tokens, float* logprobs, float* entropy, float* top_logprobs,
+                            long long* top_tokens, int rows, int vocab, long long row_stride, int top, void* stream) {
+    if (!logits || !entropy || !tokens != !logprobs || (top > 0 && (!top_logprobs || !top_tokens))) return ADE_ERR_NULL;
+    if (rows < 1 || vocab < 1 || row_stride < 0 || top < 0 || top > ade::LP_MAX_TOP || top > vocab || dtype < ADE_DTYPE_F32 || dtype > ADE_DTYPE_F16) return ADE_ERR_SHAPE;
+    int sms = 0;
+    const int rc = ade_host::sm_count(&sms);
+    if (rc) return rc;
+    const ade::LogprobParams p = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, row_stride, rows, vocab, top};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case ADE_DTYPE_F32: ade::logprob_kernel<float><<<rows, ade::LP_THREADS, 0, st>>>(p); break;
+        case ADE_DTYPE_BF16: ade::logprob_kernel<__nv_bfloat16><<<rows, ade::LP_THREADS, 0, st>>>(p); break;
+        default: ade::logprob_kernel<__half><<<rows, ade::LP_THREADS, 0, st>>>(p);
+    }
+    return launched();
+}
+
+}  // extern "C"

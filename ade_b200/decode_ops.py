@@ -22,7 +22,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .kernels import _on_device
+from .kernels import _call, _on_device
 
 MAX_ROWS = 512          # token rows (batch * sequence) up to which the fused kernels are used unconditionally
 SILU_TYPES = ("SiLU", "SiLUActivation")
@@ -133,6 +133,23 @@ def attn_decode(q, k, v, cos, sin, mask, layer, scale: float) -> torch.Tensor:
             layer.keys.data_ptr(), layer.values.data_ptr(), layer.cumulative_length.data_ptr(), ticket.data_ptr(), out.data_ptr(), B, hq, hk, hd, L,
             row(q), row(k), row(v), 0 if cos.shape[0] == 1 else hd, 0 if mask is None else mask.stride(0), float(scale))
     return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0):
+    """What a row of logits says about tokens, in one launch (``ade_b200_token_logprobs``).
+
+    Parameters:
+        logits: (rows, vocabulary) float32, bfloat16 or float16 CUDA tensor, last dimension contiguous.
+        tokens: (rows,) int64: the tokens whose log probability is asked for.  A negative one marks a row without a token (its
+            log probability is 0); one beyond the vocabulary gives NaN.  None: not asked for.
+        top: how many of the likeliest tokens to return, 0 .. 32.
+
+    Returns:
+        (logprobs (rows,) or empty without tokens, entropy (rows,), top_logprobs (rows, top), top_tokens (rows, top) int64); floats in
+        float32, natural logarithms.  Equal logits come in the order of their tokens.  There is no backward pass: logits that
+        require a gradient are refused outside ``torch.no_grad()``.
+    """
+    return _call(_lib.ops().token_logprobs, logits, tokens, top)
 
 
 def _attn_decode_ok(mod, x, cos, mask, layer) -> bool:

@@ -327,6 +327,20 @@ def _kernel_error(e: RuntimeError) -> Exception:
     return _lib.AdeKernelError(msg) if msg.startswith("ade_b200_") else e
 
 
+def _call(op, *args):
+    """One call of a binding that checks its arguments itself.  What it refuses (and tensors that are on no CUDA device) is a
+    ValueError here, a status of the C ABI an AdeKernelError; anything else, out of memory among it, stays what it is."""
+    try:
+        return op(*args)
+    except NotImplementedError:
+        raise ValueError(f"{op.__name__}: the tensors must be on a CUDA device") from None
+    except RuntimeError as e:
+        if type(e) is not RuntimeError:
+            raise
+        msg = str(e).split("\n")[0]
+        raise (_lib.AdeKernelError if msg.startswith("ade_b200_") else ValueError)(msg) from None
+
+
 def _flat_blocks(p4: dict):
     """Block structure of a fused group's U^ as the flat (row, group, row, group, ...) list the binding takes."""
     fb = p4.get("_flat_blocks")
@@ -400,3 +414,46 @@ def recon_int4(p4, base, group_size=GROUP, dbg_acc=None, status=None, expanded=N
                                     u8, v8)
         except RuntimeError as e:
             raise _kernel_error(e) from None
+
+
+# ---------------------------------------------------------------------------- deltas of many fine-tuned models
+BANK_KEYS = ("uq", "us", "uz", "vt", "vs", "vz", "start")
+
+
+def bank_deltas(stored_forms) -> dict:
+    """Bank of the deltas that several fine-tuned models have on one module, for `multi_delta_forward`.
+
+    Parameters:
+        stored_forms: one ``pack_int4`` result per model, all of the same d_o and d_i on one CUDA device; ranks may differ.
+
+    Returns:
+        dict of the tensors of ``struct ade_delta_bank``: the models' rank groups one behind the other, each group's codes of U^
+        and of V^^T in one piece (``uq`` (groups, d_o, 64), ``vt`` (groups, 128, d_i / 2)), scales and zero-points beside them,
+        ``start`` (models + 1) int32 with the first group of each model, and the ints ``M``, ``N``.  The bank holds copies.
+    """
+    forms = list(stored_forms)
+    if not forms:
+        raise ValueError("bank_deltas: no deltas given")
+    M, N, dev = int(forms[0]["M"]), int(forms[0]["N"]), forms[0]["uq"].device
+    for f in forms:
+        if (int(f["M"]), int(f["N"])) != (M, N) or any(f[k].device != dev for k in STORED_KEYS):
+            raise ValueError("bank_deltas: the deltas must have the same d_o and d_i and be on one device")
+        if not GROUP <= int(f["r"]) <= 2048 or int(f["r"]) % GROUP:
+            raise ValueError(f"bank_deltas: rank {f['r']} must be a multiple of {GROUP} up to 2048")
+    ng = [int(f["r"]) // GROUP for f in forms]
+    columns = lambda key, *tail: torch.cat([f[key].reshape(M, n, *tail).transpose(0, 1) for f, n in zip(forms, ng)]).contiguous()
+    start = torch.tensor([sum(ng[:i]) for i in range(len(ng) + 1)], dtype=torch.int32)
+    return {"uq": columns("uq", GROUP // 2), "us": columns("us"), "uz": columns("uz"),
+            "vt": torch.cat([f["vt"].reshape(n, GROUP, N // 2) for f, n in zip(forms, ng)]), "vs": torch.cat([f["vs"] for f in forms]),
+            "vz": torch.cat([f["vz"] for f in forms]), "start": start.to(dev), "M": M, "N": N}
+
+
+def multi_delta_forward(x: torch.Tensor, y_dense: torch.Tensor, bank: dict, ids: torch.Tensor) -> torch.Tensor:
+    """y_dense + U^ (V^^T x) with a delta of its own for every token row (``ade_b200_multi_delta``).
+
+    x (T, d_i) and y_dense (T, d_o) are contiguous bfloat16 CUDA tensors, T <= 128; ids (T,) int32 names each row's model in
+    `bank` (``bank_deltas``) and may change between replays of a captured graph; a row whose id is outside the bank gets
+    y_dense alone.  Returns a fresh (T, d_o) bfloat16 tensor.  Each delta in use is read once for all of its rows.  No
+    counterpart in the reference, which serves one delta at a time (src/serving.py:133-194).
+    """
+    return _call(_lib.ops().multi_delta, x, y_dense, *[bank[k] for k in BANK_KEYS], bank["M"], bank["N"], ids)

@@ -301,6 +301,92 @@ int ade_b200_attn_decode(const void* q, const void* k, const void* v, const void
                          long long cs_batch_stride, long long mask_row_stride, float scale, void* stream);
 
 /*
+ * A serving step over a batch of independent requests: every request has its own length, its own pages of the key-value
+ * cache and its own fine-tuned model.  No counterpart in the reference, which serves one delta and one batch of equal lengths
+ * at a time (src/serving.py:133-194, src/evaluate.py:241).  Strides are in elements.
+ *
+ * Paged cache.  k_pages, v_pages bf16 [pages][kv_heads][page_size][head_dim], contiguous, one pair per layer; one block table
+ * int32 [B][width] (rows table_row_stride apart) for all layers: token i of request b lives in page block_table[b][i / page_size] at
+ * offset i % page_size, and slot = page * page_size + offset.  Free pages lie on a stack: free_pages[0 .. *free_count - 1] of
+ * `pages` entries.  Everything is device memory, so a captured graph follows the requests' lengths.
+ *
+ *   ade_b200_paged_extend  adds new_tokens[b] tokens to each request (0: none).  A negative number ends the request: its pages
+ *                  go back on the stack before any page is taken, and its length becomes 0.  Pages are taken from the top of
+ *                  the stack in the order of the requests and entered into block_table behind those a request has.  The rows of
+ *                  the new tokens are numbered through the requests in order: request b's follow those of 0 .. b - 1.  For each
+ *                  row of 0 .. total - 1: its slot, its position in the request, its request; rows behind the last one, and those
+ *                  of a request that could not grow, get slot -1, position 0, request -1.  status[b]: ADE_PAGED_OK, or why
+ *                  request b did not grow (its length then stays): ADE_PAGED_NO_PAGE (the stack does not reach to it),
+ *                  ADE_PAGED_TABLE_FULL (width * page_size), ADE_PAGED_NO_ROW (its rows do not end within `total`),
+ *                  ADE_PAGED_BAD_LENGTH (negative, or beyond its row of the table; nothing is handed back either).  lengths_out
+ *                  and free_count_out may be lengths and free_count.  B <= ADE_B200_MAX_REQUESTS, width * page_size < 2^31,
+ *                  total <= 2^30.
+ *   ade_b200_paged_write   k [T][kv_heads][head_dim] (rotated with cos / sin [T][head_dim] in float32 and rounded once; both NULL:
+ *                  as it is) and v into the slots of their rows; slots outside 0 .. pages * page_size - 1 are left out.  Of two rows
+ *                  with the same slot either may stay.  head_dim a multiple of 32 up to 256, here and below.
+ *   ade_b200_paged_attn    out[t][h] = softmax(scale q[t][h] K^T) V over positions 0 .. positions[t] of request requests[t], query head
+ *                  h on key-value head h / (q_heads / kv_heads); q rotated with cos / sin in float32, or both NULL.  Any number
+ *                  of rows may belong to one request.  Rows without a request (outside 0 .. B - 1) or with a negative position are zero;
+ *                  positions beyond width * page_size, and those in table entries outside 0 .. pages - 1, are not attended to; a
+ *                  row that attends to nothing is zero.  Scores, sums and the weighted sum in float32.  work: 16-byte aligned,
+ *                  ade_b200_paged_attn_workspace_bytes, contents of no meaning before and after the call.
+ *
+ *   ade_b200_multi_delta   out[t] = y_dense[t] + U_d^ (V_d^^T x[t]) with d = ids[t], each row of x [T][N], y_dense and out [T][M]
+ *                  (contiguous; out may be y_dense) with the delta of its own fine-tuned model; ids outside 0 .. deltas - 1: y_dense alone.
+ *                  T <= ADE_B200_MAX_TOKENS, N % 128 == 0.  ids and the bank's start are read on the device.
+ *
+ *   ade_b200_token_logprobs  from logits [rows][vocab] (rows row_stride apart; ADE_DTYPE_*): logprobs[r] = log softmax of token
+ *                  tokens[r] (negative: none, 0; vocab or more: NaN; tokens and logprobs both NULL: left out), entropy[r] of the
+ *                  distribution, and the `top` (up to 32) likeliest tokens with their log probabilities, equal logits by the lower
+ *                  index, NaN before all.  A row with a NaN or +inf, or of nothing but -inf, has NaN everywhere but in
+ *                  top_tokens.  Sums in float32.
+ */
+#define ADE_B200_MAX_REQUESTS 4096
+#define ADE_PAGED_OK 0
+#define ADE_PAGED_NO_PAGE 1
+#define ADE_PAGED_TABLE_FULL 2
+#define ADE_PAGED_NO_ROW 3
+#define ADE_PAGED_BAD_LENGTH 4
+#define ADE_DTYPE_F32 0
+#define ADE_DTYPE_BF16 1
+#define ADE_DTYPE_F16 2
+
+/*
+ * Deltas of many fine-tuned models of one module, rank group by rank group (128 ranks), all pointers 16-byte aligned:
+ * delta d owns groups start[d] .. start[d + 1] - 1 (at most ADE_B200_MAX_RANK / 128 of them are used).
+ *   uq uint8 [groups][M][64], us bf16 [groups][M], uz uint8 [groups][M]           U^, packed along the rank axis
+ *   vt uint8 [groups][128][N/2], vs bf16 [groups][N], vz uint8 [groups][N]        V^^T, packed along d_i
+ * in the nibble order of ade_delta_t; start int32 [deltas + 1].
+ */
+typedef struct ade_delta_bank {
+    const uint8_t* uq;
+    const uint16_t* us;
+    const uint8_t* uz;
+    const uint8_t* vt;
+    const uint16_t* vs;
+    const uint8_t* vz;
+    const int32_t* start;
+    int M, N, groups, deltas;
+} ade_delta_bank_t;
+
+int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
+                          int32_t* lengths_out, int32_t* free_count_out, int32_t* status, long long* slots, long long* positions, int32_t* requests,
+                          int B, int width, long long table_row_stride, int pages, int page_size, int total, void* stream);
+int ade_b200_paged_write(const void* k, const void* v, const void* cos_t, const void* sin_t, const long long* slots, void* k_pages, void* v_pages,
+                         int T, int kv_heads, int head_dim, int pages, int page_size, long long k_row_stride, long long k_head_stride,
+                         long long v_row_stride, long long v_head_stride, long long cs_row_stride, void* stream);
+size_t ade_b200_paged_attn_workspace_bytes(int T, int q_heads, int kv_heads, int head_dim);
+int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, const int32_t* block_table, const int32_t* requests,
+                        const long long* positions, const void* k_pages, const void* v_pages, void* out, void* work, size_t work_bytes, int T, int B,
+                        int width, long long table_row_stride, int q_heads, int kv_heads, int head_dim, int pages, int page_size,
+                        long long q_row_stride, long long q_head_stride, long long cs_row_stride, float scale, void* stream);
+size_t ade_b200_multi_delta_workspace_bytes(int T, int N);
+int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_bank_t* bank, const int32_t* ids, void* out, void* work, size_t work_bytes,
+                         int T, void* stream);
+int ade_b200_token_logprobs(const void* logits, int dtype, const long long* tokens, float* logprobs, float* entropy, float* top_logprobs,
+                            long long* top_tokens, int rows, int vocab, long long row_stride, int top, void* stream);
+
+/*
  * Process-wide options.  No counterpart in the reference.
  *   ADE_OPT_WAIT_LIMIT_CYCLES   clock cycles a wait inside a kernel (for h, for an operand stage, ...) may take
  *                               before the kernel gives up, records its status and runs to its end; 0 restores the
