@@ -1,4 +1,4 @@
-// Paged key-value cache: page allocation and slot maps, the write of new keys and values, attention of single rows.
+// Paged key-value cache: page allocation and slot maps, the write of new keys and values (paged_attn.cuh reads them).
 //
 // A cache layer is two arrays k_pages, v_pages [pages][kv_heads][page_size][head_dim] of bfloat16.  A request owns an
 // ordered list of pages, its row of block_table [B][width]; token i of the request lives in page block_table[b][i / page_size]
@@ -253,72 +253,6 @@ __global__ void __launch_bounds__(256) paged_write_kernel(const WriteParams p) {
             p.vp[to] = vr[0];
             p.vp[to + half] = vr[half];
         }
-    }
-}
-
-// ------------------------------------------------------------------ attention of single rows over the pages of their requests
-struct PagedAttnParams {
-    const __nv_bfloat16 *q, *cs, *sn;          // q [T][q_heads][dim] by strides; cs, sn [T][dim] or nullptr: q is used as it is
-    const int* table;
-    const int* requests;                       // [T] row of the block table, outside 0 .. B - 1: the row has no request
-    const long long* positions;                // [T] the row sees positions 0 .. positions[t] of its request
-    const __nv_bfloat16 *kp, *vp;
-    __nv_bfloat16* out;                        // [T][q_heads][dim]
-    long long table_stride, q_row, q_head, cs_row;
-    int T, B, width, pages, page_size, q_heads, kv_heads, dim;
-    float scale;
-};
-
-// One CTA per (row, query head), one position per warp at a time, a running softmax per warp, the warps joined at the end.
-__global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnParams p) {
-    __shared__ float s_m[4], s_l[4], s_acc[4][256];
-    const int t = blockIdx.x / p.q_heads, h = blockIdx.x % p.q_heads, kvh = h / (p.q_heads / p.kv_heads);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.dim >> 5, half = p.dim >> 1;
-    const int b = p.requests[t];
-    const long long last = p.positions[t];
-    long long n = b < 0 || b >= p.B || last < 0 ? 0 : last + 1;
-    n = min(n, static_cast<long long>(p.width) * p.page_size);
-    float q[8], acc[8];
-    for (int i = 0; i < per; ++i) {
-        const int d = lane + 32 * i;
-        const __nv_bfloat16* qr = p.q + t * p.q_row + h * p.q_head;
-        q[i] = __bfloat162float(qr[d]);
-        if (p.cs) {
-            const float o = d < half ? -__bfloat162float(qr[d + half]) : __bfloat162float(qr[d - half]);
-            q[i] = q[i] * __bfloat162float(p.cs[t * p.cs_row + d]) + o * __bfloat162float(p.sn[t * p.cs_row + d]);
-        }
-        acc[i] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (long long j = warp; j < n; j += 4) {
-        const int page = p.table[b * p.table_stride + j / p.page_size];
-        if (page < 0 || page >= p.pages) continue;
-        const long long at = ((static_cast<long long>(page) * p.kv_heads + kvh) * p.page_size + j % p.page_size) * p.dim;
-        float s = 0.f;
-        for (int i = 0; i < per; ++i) s += q[i] * __bfloat162float(p.kp[at + lane + 32 * i]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        s *= p.scale;
-        const float mn = fmaxf(m, s), f = mn == -INFINITY ? 1.f : expf(m - mn), w = mn == -INFINITY ? 0.f : expf(s - mn);
-        l = l * f + w;
-        for (int i = 0; i < per; ++i) acc[i] = acc[i] * f + w * __bfloat162float(p.vp[at + lane + 32 * i]);
-        m = mn;
-    }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
-    for (int i = 0; i < per; ++i) s_acc[warp][lane + 32 * i] = acc[i];
-    __syncthreads();
-    const float mm = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    for (int d = threadIdx.x; d < p.dim; d += 128) {
-        float num = 0.f, den = 0.f;
-        for (int w = 0; w < 4; ++w) {
-            const float f = s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - mm);
-            num += f * s_acc[w][d];
-            den += f * s_l[w];
-        }
-        p.out[(static_cast<long long>(t) * p.q_heads + h) * p.dim + d] = __float2bfloat16_rn(den > 0.f ? num / den : 0.f);
     }
 }
 

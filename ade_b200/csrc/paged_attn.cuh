@@ -1,0 +1,486 @@
+// Attention of single token rows over the pages of their requests, split over the cache's length and joined.
+//
+//   out[t][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q~ . k_j - m),   j = 0 .. positions[t],   m the largest score
+//
+// A (row, key-value head) pair reads its keys and values once for up to eight query heads.  Both products run on the warp matrix
+// instruction m16n8k16 with the heads as its 16 rows: rows 0-7 hold the bfloat16 rounding of an operand, rows 8-15 what that
+// rounding left over, so queries and probabilities enter with 16 bits of mantissa at no cost (one to eight heads leave those rows
+// free) and the two halves of a result are added in float32.  The running maximum and sum of the softmax stay in registers.
+//
+// The cache is cut into tiles of 16 positions; the tiles of all pairs, one pair behind the other, are shared out evenly over the
+// CTAs and there over the warps, whatever the lengths.  A warp streams its tiles through cp.async stages of its own and never waits
+// for another; what it has of a pair that others share goes to the workspace as (maximum, sum, weighted sum), and a second
+// launch joins those parts in the order of the tiles.  A CTA whose tiles all belong to one pair joins its warps' parts itself.
+#pragma once
+#include "paged.cuh"
+#include "ptx.cuh"
+
+namespace ade {
+
+constexpr int PA_MAX_CTAS = 160;           // one CTA per SM; bounds the workspace
+constexpr int PA_MAX_ROWS = 1024;          // rows of one launch (their prefix sums lie in shared memory)
+constexpr int PA_HEADS = 8;                // query heads that share one pass over the keys and values
+constexpr int PA_TILE = 16;                // positions of a tile
+
+struct PagedAttnParams {
+    const __nv_bfloat16 *q, *cs, *sn;          // q [T][q_heads][dim] by strides; cs, sn [T][dim] or nullptr: q is used as it is
+    const int* table;
+    const int* requests;                       // [T] row of the block table, outside 0 .. B - 1: the row has no request
+    const long long* positions;                // [T] the row sees positions 0 .. positions[t] of its request
+    const __nv_bfloat16 *kp, *vp;
+    __nv_bfloat16* out;                        // [T][q_heads][dim]
+    float* part;                               // [warps][2][PA_HEADS][dim] weighted sums
+    float2* stat;                              // [warps][2][PA_HEADS] (maximum in powers of two, sum)
+    int4* meta;                                // [warps] (row + 1 or 0, pair, last warp, flags) of a pair that begins there and goes on
+    long long table_stride, q_row, q_head, cs_row;
+    int T, B, width, pages, page_size, q_heads, kv_heads;
+    float scale2;                              // scale * log2(e)
+};
+
+template <int HD>
+struct PaShape {
+    static constexpr int kWarps = HD <= 128 ? 8 : 4;
+    static constexpr int kChunks = HD / 8;                               // 16-byte pieces of a row
+    static constexpr int kTileBytes = PA_TILE * HD * 2;
+    static constexpr int kStages = 192 * 1024 / (kWarps * 2 * kTileBytes) < 8 ? 192 * 1024 / (kWarps * 2 * kTileBytes) : 8;
+    static constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * 2 * kTileBytes;
+    // where piece c of row r lies in a tile: the eight rows that a matrix load reads at one piece are spread over the banks
+    __device__ static __forceinline__ uint32_t at(int r, int c) {
+        return static_cast<uint32_t>(r * kChunks + (kChunks % 8 == 0 ? c ^ (r & 7) : c ^ (r >> 1 & 3))) * 16u;
+    }
+};
+inline size_t pa_smem_bytes(size_t ring, int warps, int stages, int T) {
+    return ring + static_cast<size_t>(T + 1) * 8 + static_cast<size_t>(T) * 8 + static_cast<size_t>(warps) * stages * 4 + static_cast<size_t>(warps) * PA_HEADS * 8;
+}
+
+__device__ __forceinline__ void pa_ldm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void pa_ldm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+// 16 bytes global -> shared; nothing is read and zeros are written where `live` is false
+__device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void pa_cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// bfloat16 pair of (a, b), and the pair of what that rounding left over
+__device__ __forceinline__ uint32_t pa_split(float a, float b, uint32_t& rest) {
+    const uint32_t hi = pack_bf2(a, b);
+    rest = pack_bf2(a - bf_lo(hi), b - bf_hi(hi));
+    return hi;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel(const PagedAttnParams p) {
+    using S = PaShape<HD>;
+    constexpr int KS = HD / 16, NW = S::kWarps, NT = NW * 32;
+    extern __shared__ __align__(128) uint8_t pa_smem[];
+    long long* prefix = reinterpret_cast<long long*>(pa_smem + S::kRing);        // [T + 1] tiles of the rows before (one pair each)
+    int* rown = reinterpret_cast<int*>(prefix + p.T + 1);                          // [T] positions the row sees
+    int* rowreq = rown + p.T;                                                      // [T] its request
+    float2* mstat = reinterpret_cast<float2*>(rowreq + p.T);                       // [NW][PA_HEADS]
+    uint32_t* masks = reinterpret_cast<uint32_t*>(mstat + NW * PA_HEADS);          // [NW][stages] positions of a tile that count
+    __shared__ long long ws[NW];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
+    const int group = p.q_heads / p.kv_heads, sets = (group + PA_HEADS - 1) / PA_HEADS, H = p.kv_heads * sets;
+
+    // tiles of every row, summed
+    const int per = (p.T + NT - 1) / NT, ta = min(tid * per, p.T), tb = min(ta + per, p.T);
+    long long mine = 0;
+    for (int t = ta; t < tb; ++t) {
+        const int req = p.requests[t];
+        const long long pos = p.positions[t];
+        const int n = req < 0 || req >= p.B || pos < 0 ? 0 : static_cast<int>(min(pos + 1, static_cast<long long>(p.width) * p.page_size));
+        rown[t] = n;
+        rowreq[t] = req;
+        mine += (n + PA_TILE - 1) / PA_TILE;
+    }
+    long long run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xFFFFFFFFu, run, o);
+        if (lane >= o) run += u;
+    }
+    if (lane == 31) ws[warp] = run;
+    __syncthreads();
+    run -= mine;
+    for (int w = 0; w < warp; ++w) run += ws[w];
+    for (int t = ta; t < tb; ++t) {
+        prefix[t] = run;
+        run += (rown[t] + PA_TILE - 1) / PA_TILE;
+    }
+    if (tid == NT - 1) prefix[p.T] = run;
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // rows that see nothing are zero
+    for (int t = blockIdx.x; t < p.T; t += gridDim.x)
+        if (rown[t] == 0)
+            for (int i = tid; i < p.q_heads * HD / 8; i += NT)
+                reinterpret_cast<uint4*>(p.out + static_cast<long long>(t) * p.q_heads * HD)[i] = make_uint4(0u, 0u, 0u, 0u);
+
+    // this warp's tiles f .. f_end - 1 of all, and whether its whole CTA works on one pair
+    const long long total = prefix[p.T] * H;
+    const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total)), cta = blockIdx.x;
+    auto cta_begin = [&](int c) { return total * c / ctas; };
+    const int wid = cta * NW + warp;
+    if (cta >= ctas) {
+        if (lane == 0) p.meta[wid] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    const long long F0 = cta_begin(cta), F1 = cta_begin(cta + 1);
+    long long f = F0 + (F1 - F0) * warp / NW;
+    const long long f_end = F0 + (F1 - F0) * (warp + 1) / NW;
+    struct Cursor {
+        int t, pair, tile, nt;
+    };
+    auto locate = [&](long long g) {
+        int lo = 0, hi = p.T - 1;                                       // the row with prefix[t] * H <= g < prefix[t + 1] * H
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (prefix[mid] * H <= g) lo = mid;
+            else hi = mid - 1;
+        }
+        Cursor c;
+        c.t = lo;
+        c.nt = static_cast<int>(prefix[lo + 1] - prefix[lo]);
+        const long long rest = g - prefix[lo] * H;
+        c.pair = static_cast<int>(rest / c.nt);
+        c.tile = static_cast<int>(rest - static_cast<long long>(c.pair) * c.nt);
+        return c;
+    };
+    auto advance = [&](Cursor& c) {
+        if (++c.tile < c.nt) return;
+        c.tile = 0;
+        if (++c.pair < H) return;
+        c.pair = 0;
+        do {
+            ++c.t;
+        } while (c.t < p.T && prefix[c.t + 1] == prefix[c.t]);
+        c.nt = c.t < p.T ? static_cast<int>(prefix[c.t + 1] - prefix[c.t]) : 1;
+    };
+    auto pair_begin = [&](const Cursor& c) { return prefix[c.t] * H + static_cast<long long>(c.pair) * c.nt; };
+    const Cursor c0 = locate(F0);
+    const bool merged = F1 <= pair_begin(c0) + c0.nt;                     // the CTA's tiles are all of pair c0
+    int4 meta = make_int4(0, 0, 0, 0);
+    // (last warp, flags) of the pair of c, which goes on behind this CTA or this warp
+    auto chain = [&](const Cursor& c) {
+        const long long fe = pair_begin(c) + c.nt;
+        const int last = static_cast<int>((fe * ctas + total - 1) / total) - 1;
+        const long long L0 = cta_begin(last), L1 = cta_begin(last + 1);
+        const int lw = static_cast<int>(((fe - L0) * NW + (L1 - L0) - 1) / (L1 - L0)) - 1;
+        const bool last_merged = L0 >= pair_begin(c) && L1 <= fe;
+        return make_int4(c.t + 1, c.pair, last * NW + min(lw, NW - 1), (merged ? 1 : 0) | (last_merged ? 2 : 0));
+    };
+
+    const uint32_t ring = smem_u32(pa_smem) + static_cast<uint32_t>(warp) * (S::kStages * 2 * S::kTileBytes);
+    uint32_t* mk = masks + warp * S::kStages;
+    // ---- the copies, STAGES - 1 tiles ahead of the arithmetic, the look at the block table one more
+    Cursor ahead = f < f_end ? locate(f) : c0;
+    long long f_look = f;
+    int l_page = -1, l_off = 0, l_kvh = 0;
+    auto look = [&] {
+        l_page = -1;
+        if (f_look < f_end) {
+            const int pos = ahead.tile * PA_TILE + (lane & 15);
+            l_kvh = ahead.pair / sets;
+            if (pos < rown[ahead.t]) {
+                const int col = pos / p.page_size;
+                l_off = pos - col * p.page_size;
+                l_page = p.table[rowreq[ahead.t] * p.table_stride + col];
+            }
+            advance(ahead);
+        }
+        ++f_look;
+    };
+    auto issue = [&](int stage) {
+        const bool ok = l_page >= 0 && l_page < p.pages;
+        const uint32_t row = ok ? (static_cast<uint32_t>(l_page) * p.kv_heads + l_kvh) * p.page_size + l_off : 0u;
+        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
+        if (lane == 0) mk[stage] = mask;
+        const uint32_t dst = ring + static_cast<uint32_t>(stage) * (2 * S::kTileBytes);
+        if (f_look - 1 < f_end) {
+#pragma unroll
+            for (int j = 0; j < S::kChunks / 2; ++j) {
+                const int i = j * 32 + lane, r = i / S::kChunks, c = i - r * S::kChunks;
+                const size_t at = static_cast<size_t>(__shfl_sync(0xFFFFFFFFu, row, r)) * HD + c * 8;
+                const bool live = mask >> r & 1u;
+                pa_cp16(dst + S::at(r, c), p.kp + at, live);
+                pa_cp16(dst + S::kTileBytes + S::at(r, c), p.vp + at, live);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    look();
+#pragma unroll 1
+    for (int s = 0; s < S::kStages - 1; ++s) {
+        issue(s);
+        look();
+    }
+
+    uint32_t qa[KS][4];
+    float acc[HD / 8][4], m = -INFINITY, l = 0.f;
+    Cursor cur = f < f_end ? locate(f) : c0;
+    bool fresh = true, from_start = false;
+    int stage = 0, fill = S::kStages - 1;
+    const int pair_heads = min(PA_HEADS, group);
+    auto heads_of = [&](int pair) { return min(pair_heads, group - pair % sets * PA_HEADS); };
+    auto first_head = [&](int pair) { return pair / sets * group + pair % sets * PA_HEADS; };
+    if (f >= f_end && !merged && lane < PA_HEADS) p.stat[(wid * 2) * PA_HEADS + lane] = make_float2(-INFINITY, 0.f);   // a warp without tiles
+#pragma unroll 1
+    for (; f < f_end; ++f) {
+        if (fresh) {                                                    // a new pair: its queries, rotated, in two bfloat16 parts
+            fresh = false;
+            from_start = cur.tile == 0;
+            m = -INFINITY;
+            l = 0.f;
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+            const bool on = gid < heads_of(cur.pair);
+            const __nv_bfloat16* qr = p.q + cur.t * p.q_row + (first_head(cur.pair) + (on ? gid : 0)) * p.q_head;
+            const __nv_bfloat16 *cr = p.cs + cur.t * p.cs_row, *sr = p.sn + cur.t * p.cs_row;
+            auto val = [](const __nv_bfloat16* a) { return __bfloat162float(*a); };
+#pragma unroll
+            for (int ks = 0; ks < KS / 2; ++ks) {
+                float a[4], b[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int d = ks * 16 + tig * 2 + (i & 1) + (i >> 1) * 8;
+                    const float x = on ? val(qr + d) : 0.f, y = on ? val(qr + d + HD / 2) : 0.f;
+                    a[i] = x;
+                    b[i] = y;
+                    if (p.cs) {
+                        a[i] = x * val(cr + d) - y * val(sr + d);
+                        b[i] = y * val(cr + d + HD / 2) + x * val(sr + d + HD / 2);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    qa[ks][2 * i] = pa_split(a[2 * i], a[2 * i + 1], qa[ks][2 * i + 1]);
+                    qa[ks + KS / 2][2 * i] = pa_split(b[2 * i], b[2 * i + 1], qa[ks + KS / 2][2 * i + 1]);
+                }
+            }
+        }
+        pa_cp_wait<S::kStages - 2>();
+        __syncwarp();                                                   // the tile is there, and the stage before it has been read by all lanes
+        issue(fill);
+        look();
+        const uint32_t mask = mk[stage];
+        if (mask) {
+            const uint32_t kt = ring + static_cast<uint32_t>(stage) * (2 * S::kTileBytes), vt = kt + S::kTileBytes;
+            float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t b[4];
+                pa_ldm4(kt + S::at((lane >> 4) * 8 + (lane & 7), 2 * ks + (lane >> 3 & 1)), b);
+                mma_bf16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
+                mma_bf16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
+            }
+            // head gid at positions 2 tig, 2 tig + 1 and the same + 8
+            float w[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = mask >> (tig * 2 + (i & 1) + (i >> 1) * 8) & 1u ? w[i] * p.scale2 : -INFINITY;
+                mx = fmaxf(mx, w[i]);
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+            if (__any_sync(0xFFFFFFFFu, mx > m)) {
+                const float mn = fmaxf(m, mx), fac = exp2f(m - mn);
+                m = mn;
+                l *= fac;
+#pragma unroll
+                for (int j = 0; j < HD / 8; ++j) {
+                    acc[j][0] *= fac;
+                    acc[j][1] *= fac;
+                    acc[j][2] *= fac;
+                    acc[j][3] *= fac;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = exp2f(w[i] - m);
+                l += w[i];
+            }
+            uint32_t pa[4];
+            pa[0] = pa_split(w[0], w[1], pa[1]);
+            pa[2] = pa_split(w[2], w[3], pa[3]);
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+                uint32_t b[4];
+                pa_ldm4t(vt + S::at((lane >> 3 & 1) * 8 + (lane & 7), 2 * j + (lane >> 4)), b);
+                mma_bf16(acc[2 * j], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+                mma_bf16(acc[2 * j + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+            }
+        }
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
+        fill = fill + 1 == S::kStages ? 0 : fill + 1;
+        const bool pair_ends = cur.tile + 1 == cur.nt;
+        if (pair_ends || f + 1 == f_end) {
+            l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+            l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+            const int heads = heads_of(cur.pair);
+            if (!merged) {
+                if (from_start && pair_ends) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    if (gid < heads) {
+                        __nv_bfloat16* o = p.out + (static_cast<long long>(cur.t) * p.q_heads + first_head(cur.pair) + gid) * HD + tig * 2;
+#pragma unroll
+                        for (int j = 0; j < HD / 8; ++j)
+                            *reinterpret_cast<uint32_t*>(o + j * 8) = pack_bf2((acc[j][0] + acc[j][2]) * inv, (acc[j][1] + acc[j][3]) * inv);
+                    }
+                } else {
+                    const int slot = wid * 2 + (from_start ? 1 : 0);
+                    if (gid < heads) {
+                        float* o = p.part + (static_cast<size_t>(slot) * PA_HEADS + gid) * HD + tig * 2;
+#pragma unroll
+                        for (int j = 0; j < HD / 8; ++j)
+                            *reinterpret_cast<float2*>(o + j * 8) = make_float2(acc[j][0] + acc[j][2], acc[j][1] + acc[j][3]);
+                        if (tig == 0) p.stat[slot * PA_HEADS + gid] = make_float2(m, l);
+                    }
+                    if (from_start) meta = chain(cur);
+                }
+            }
+            fresh = true;
+        }
+        advance(cur);
+    }
+    if (merged) {
+        // the warps' parts through shared memory (the ring is free: every copy has arrived), added in the order of the warps
+        pa_cp_wait<0>();
+        __syncwarp();
+        float* mine_acc = reinterpret_cast<float*>(pa_smem) + static_cast<size_t>(warp) * (S::kStages * 2 * S::kTileBytes / 4);
+        const bool any = F0 + (F1 - F0) * warp / NW < f_end;
+        const int heads = heads_of(c0.pair), h0 = first_head(c0.pair);
+        if (any && gid < heads) {
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j)
+                *reinterpret_cast<float2*>(mine_acc + gid * HD + j * 8 + tig * 2) = make_float2(acc[j][0] + acc[j][2], acc[j][1] + acc[j][3]);
+        }
+        if (tig == 0) mstat[warp * PA_HEADS + gid] = any ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        __syncthreads();
+        const bool whole = F0 == pair_begin(c0) && F1 == pair_begin(c0) + c0.nt, begins = F0 == pair_begin(c0);
+        const int slot = cta * NW * 2 + (begins ? 1 : 0);
+        for (int i = tid; i < heads * HD; i += NT) {
+            const int h = i / HD, d = i - h * HD;
+            float mm = -INFINITY, num = 0.f, den = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) mm = fmaxf(mm, mstat[w * PA_HEADS + h].x);
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float2 st = mstat[w * PA_HEADS + h];
+                if (st.x == -INFINITY) continue;
+                const float fac = exp2f(st.x - mm);
+                num += fac * reinterpret_cast<const float*>(pa_smem)[static_cast<size_t>(w) * (S::kStages * 2 * S::kTileBytes / 4) + i];
+                den += fac * st.y;
+            }
+            if (whole) {
+                p.out[(static_cast<long long>(c0.t) * p.q_heads + h0 + h) * HD + d] = __float2bfloat16_rn(den == 0.f ? 0.f : num / den);
+            } else {
+                p.part[(static_cast<size_t>(slot) * PA_HEADS + h) * HD + d] = num;
+                if (d == 0) p.stat[slot * PA_HEADS + h] = make_float2(mm, den);
+            }
+        }
+        if (warp == 0 && begins && !whole) meta = chain(c0);
+    }
+    if (lane == 0) p.meta[wid] = meta;
+}
+
+// Joins the parts of one pair that begins in warp blockIdx.x of the first launch and goes on in others: its own second slot, then the first slots of
+// the warps behind it (one per CTA where the CTA has joined its warps).  Up to eight heads, the parts of a head over as many warps as are left.
+template <int HD>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const PagedAttnParams p) {
+    constexpr int NW = PaShape<HD>::kWarps;
+    __shared__ float sums[8][HD + 1];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int w0 = blockIdx.x;
+    const int4 meta = p.meta[w0];
+    if (meta.x == 0) return;
+    const int t = meta.x - 1, pair = meta.y, last = meta.z;
+    const int group = p.q_heads / p.kv_heads, sets = (group + PA_HEADS - 1) / PA_HEADS;
+    const int heads = min(PA_HEADS, group - pair % sets * PA_HEADS), h0 = pair / sets * group + pair % sets * PA_HEADS;
+    const int ca = w0 / NW, cb = last / NW;
+    const int own = meta.w & 1 ? 0 : min(last, ca * NW + NW - 1) - w0;                       // further warps of the first CTA
+    const int middle = max(cb - ca - 1, 0);
+    const int n = 1 + own + (cb > ca ? middle + (meta.w & 2 ? 1 : last - cb * NW + 1) : 0);
+    auto slot = [&](int i) {
+        if (i == 0) return w0 * 2 + 1;
+        if (i <= own) return (w0 + i) * 2;
+        i -= own + 1;
+        return i < middle ? (ca + 1 + i) * NW * 2 : (cb * NW + i - middle) * 2;
+    };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int share = heads > 4 ? 1 : heads > 2 ? 2 : heads > 1 ? 4 : 8, h = warp / share, part = warp % share;
+    constexpr int V = (HD + 127) / 128;                                                       // 16-byte pieces of a head per lane
+    float4 acc[V];
+    float den = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (h < heads) {
+        float mm = -INFINITY;
+        for (int i = lane; i < n; i += 32) mm = fmaxf(mm, p.stat[slot(i) * PA_HEADS + h].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
+#pragma unroll 8
+        for (int i = part; i < n; i += share) {
+            const int s = slot(i);
+            const float2 st = p.stat[s * PA_HEADS + h];
+            const bool on = st.x != -INFINITY;
+            const float fac = on ? exp2f(st.x - mm) : 0.f;
+            den += on ? fac * st.y : 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int d = lane * 4 + v * 128;
+                if (d < HD && on) {
+                    const float4 a = *reinterpret_cast<const float4*>(p.part + (static_cast<size_t>(s) * PA_HEADS + h) * HD + d);
+                    acc[v].x += fac * a.x;
+                    acc[v].y += fac * a.y;
+                    acc[v].z += fac * a.z;
+                    acc[v].w += fac * a.w;
+                }
+            }
+        }
+        if (share > 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int d = lane * 4 + v * 128;
+                if (d < HD) {
+                    sums[warp][d] = acc[v].x;
+                    sums[warp][d + 1] = acc[v].y;
+                    sums[warp][d + 2] = acc[v].z;
+                    sums[warp][d + 3] = acc[v].w;
+                }
+            }
+            if (lane == 0) sums[warp][HD] = den;
+        }
+    }
+    if (share > 1) __syncthreads();
+    if (h >= heads || part) return;
+    if (share > 1) {
+        den = 0.f;
+        for (int w = warp; w < warp + share; ++w) den += sums[w][HD];
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    __nv_bfloat16* o = p.out + (static_cast<long long>(t) * p.q_heads + h0 + h) * HD;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int d = lane * 4 + v * 128;
+        if (d >= HD) continue;
+        float a[4] = {acc[v].x, acc[v].y, acc[v].z, acc[v].w};
+        if (share > 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = 0.f;
+                for (int w = warp; w < warp + share; ++w) a[i] += sums[w][d + i];
+            }
+        }
+        *reinterpret_cast<uint2*>(o + d) = make_uint2(pack_bf2(a[0] * inv, a[1] * inv), pack_bf2(a[2] * inv, a[3] * inv));
+    }
+}
+
+}  // namespace ade

@@ -6,6 +6,7 @@
 #include "logprobs.cuh"
 #include "multi_delta.cuh"
 #include "paged.cuh"
+#include "paged_attn.cuh"
 
 using ade_host::aligned16;
 using ade_host::cuda_ok;
@@ -15,6 +16,43 @@ namespace {
 int launched() { return cuda_ok(cudaGetLastError()) ? ADE_OK : ADE_ERR_CUDA; }
 
 bool dim_ok(int head_dim) { return head_dim >= 32 && head_dim <= 256 && head_dim % 32 == 0; }
+
+constexpr size_t kAttnWarps = static_cast<size_t>(ade::PA_MAX_CTAS) * 8;
+
+// Both launches of the attention for up to PA_MAX_ROWS rows.  The second begins while the first runs and waits for its end.
+template <int HD>
+int launch_attn(ade::PagedAttnParams p, int sms, cudaStream_t st) {
+    using S = ade::PaShape<HD>;
+    const int ctas = sms < ade::PA_MAX_CTAS ? sms : ade::PA_MAX_CTAS;
+    const size_t smem = ade::pa_smem_bytes(S::kRing, S::kWarps, S::kStages, p.T);
+    const int most = static_cast<int>(ade::pa_smem_bytes(S::kRing, S::kWarps, S::kStages, ade::PA_MAX_ROWS));
+    if (!cuda_ok(cudaFuncSetAttribute(ade::paged_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, most))) return ADE_ERR_CUDA;
+    ade::paged_attn_kernel<HD><<<ctas, S::kWarps * 32, smem, st>>>(p);
+    if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas * S::kWarps);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cuda_ok(cudaLaunchKernelEx(&cfg, ade::paged_attn_join_kernel<HD>, p)) ? ADE_OK : ADE_ERR_CUDA;
+}
+
+int launch_attn_dim(int head_dim, const ade::PagedAttnParams& p, int sms, cudaStream_t st) {
+    switch (head_dim) {
+        case 32: return launch_attn<32>(p, sms, st);
+        case 64: return launch_attn<64>(p, sms, st);
+        case 96: return launch_attn<96>(p, sms, st);
+        case 128: return launch_attn<128>(p, sms, st);
+        case 160: return launch_attn<160>(p, sms, st);
+        case 192: return launch_attn<192>(p, sms, st);
+        case 224: return launch_attn<224>(p, sms, st);
+        default: return launch_attn<256>(p, sms, st);
+    }
+}
 
 }  // namespace
 
@@ -62,7 +100,8 @@ int ade_b200_paged_write(const void* k, const void* v, const void* cos_t, const 
 }
 
 size_t ade_b200_paged_attn_workspace_bytes(int T, int q_heads, int kv_heads, int head_dim) {
-    return T < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || !dim_ok(head_dim) ? 0 : 16;
+    if (T < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || !dim_ok(head_dim)) return 0;
+    return kAttnWarps * (2 * ade::PA_HEADS * (head_dim * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
 
 int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, const int32_t* block_table, const int32_t* requests,
@@ -76,16 +115,28 @@ int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, con
     if (!work) return ADE_ERR_NULL;
     if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(work)) return ADE_ERR_ALIGN;
     if (work_bytes < ade_b200_paged_attn_workspace_bytes(T, q_heads, kv_heads, head_dim)) return ADE_ERR_SCRATCH;
-    if (static_cast<long long>(T) * q_heads > 0x7FFFFFFFll) return ADE_ERR_SHAPE;
+    // positions count in 31 bits, rows of the cache in 32
+    if (static_cast<long long>(width) * page_size > 0x7FFFFFFFll || static_cast<unsigned long long>(pages) * kv_heads > 0xFFFFFFFFull / page_size)
+        return ADE_ERR_SHAPE;
     int sms = 0;
     const int rc = ade_host::sm_count(&sms);
     if (rc) return rc;
     using bf = __nv_bfloat16;
-    ade::PagedAttnParams p = {static_cast<const bf*>(q), static_cast<const bf*>(cos_t), static_cast<const bf*>(sin_t), block_table, requests, positions,
-                              static_cast<const bf*>(k_pages), static_cast<const bf*>(v_pages), static_cast<bf*>(out), table_row_stride, q_row_stride,
-                              q_head_stride, cs_row_stride, T, B, width, pages, page_size, q_heads, kv_heads, head_dim, scale};
-    ade::paged_attn_kernel<<<T * q_heads, 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    return launched();
+    float* part = static_cast<float*>(work);
+    float2* stat = reinterpret_cast<float2*>(part + kAttnWarps * 2 * ade::PA_HEADS * head_dim);
+    int4* meta = reinterpret_cast<int4*>(stat + kAttnWarps * 2 * ade::PA_HEADS);
+    for (int t0 = 0; t0 < T; t0 += ade::PA_MAX_ROWS) {
+        const bf *cs = static_cast<const bf*>(cos_t), *sn = static_cast<const bf*>(sin_t);
+        const long long o = t0;
+        const ade::PagedAttnParams p = {static_cast<const bf*>(q) + o * q_row_stride, cs ? cs + o * cs_row_stride : nullptr,
+                                        sn ? sn + o * cs_row_stride : nullptr, block_table, requests + o, positions + o, static_cast<const bf*>(k_pages),
+                                        static_cast<const bf*>(v_pages), static_cast<bf*>(out) + o * q_heads * head_dim, part, stat, meta,
+                                        table_row_stride, q_row_stride, q_head_stride, cs_row_stride, T - t0 < ade::PA_MAX_ROWS ? T - t0 : ade::PA_MAX_ROWS, B,
+                                        width, pages, page_size, q_heads, kv_heads, scale * 1.44269504088896340736f};
+        const int rc_launch = launch_attn_dim(head_dim, p, sms, static_cast<cudaStream_t>(stream));
+        if (rc_launch) return rc_launch;
+    }
+    return ADE_OK;
 }
 
 size_t ade_b200_multi_delta_workspace_bytes(int T, int N) {
