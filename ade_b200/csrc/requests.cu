@@ -17,6 +17,22 @@ int launched() { return cuda_ok(cudaGetLastError()) ? ADE_OK : ADE_ERR_CUDA; }
 
 bool dim_ok(int head_dim) { return head_dim >= 32 && head_dim <= 256 && head_dim % 32 == 0; }
 
+// A launch whose blocks may start while the kernel before it still runs; the kernel waits for that one's results itself.
+template <typename... Params, typename... Args>
+int launch_early(void (*kernel)(Params...), int grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, args...)) ? ADE_OK : ADE_ERR_CUDA;
+}
+
 constexpr size_t kAttnWarps = static_cast<size_t>(ade::PA_MAX_CTAS) * 8;
 
 // Both launches of the attention for up to PA_MAX_ROWS rows.  The second begins while the first runs and waits for its end.
@@ -29,16 +45,7 @@ int launch_attn(ade::PagedAttnParams p, int sms, cudaStream_t st) {
     if (!cuda_ok(cudaFuncSetAttribute(ade::paged_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, most))) return ADE_ERR_CUDA;
     ade::paged_attn_kernel<HD><<<ctas, S::kWarps * 32, smem, st>>>(p);
     if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas * S::kWarps);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    return cuda_ok(cudaLaunchKernelEx(&cfg, ade::paged_attn_join_kernel<HD>, p)) ? ADE_OK : ADE_ERR_CUDA;
+    return launch_early(ade::paged_attn_join_kernel<HD>, ctas * S::kWarps, 256, 0, st, p);
 }
 
 int launch_attn_dim(int head_dim, const ade::PagedAttnParams& p, int sms, cudaStream_t st) {
@@ -140,7 +147,7 @@ int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, con
 }
 
 size_t ade_b200_multi_delta_workspace_bytes(int T, int N) {
-    return T < 1 || T > ADE_B200_MAX_TOKENS || N < 1 ? 0 : static_cast<size_t>(T) * ADE_B200_MAX_RANK * sizeof(float);
+    return T < 1 || T > ADE_B200_MAX_TOKENS || N < 1 ? 0 : static_cast<size_t>(ade::md_slices(N)) * T * ade::MD_H * sizeof(float);
 }
 
 int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_bank_t* bank, const int32_t* ids, void* out, void* work, size_t work_bytes,
@@ -162,9 +169,13 @@ int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_ban
                                reinterpret_cast<const bf*>(d.us), reinterpret_cast<const bf*>(d.vs), d.start, ids, static_cast<float*>(work),
                                d.M, d.N, d.groups, d.deltas, T};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    ade::multi_delta_v_kernel<<<dim3(T, d.groups < ade::MD_MAX_GROUPS ? d.groups : ade::MD_MAX_GROUPS), 256, 0, st>>>(p);
-    ade::multi_delta_u_kernel<<<dim3(T, (d.M + 255) / 256), 256, 0, st>>>(p);
-    return launched();
+    if (!cuda_ok(cudaFuncSetAttribute(ade::multi_delta_v_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ade::md_v_smem()))) ||
+        !cuda_ok(cudaFuncSetAttribute(ade::multi_delta_u_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ade::md_u_smem()))))
+        return ADE_ERR_CUDA;
+    const int slices = ade::md_slices(d.N);
+    ade::multi_delta_v_kernel<<<2 * sms, ade::MD_THREADS, ade::md_v_smem(), st>>>(p, slices);
+    if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
+    return launch_early(ade::multi_delta_u_kernel, 2 * sms, ade::MD_THREADS, ade::md_u_smem(), st, p, slices);
 }
 
 int ade_b200_token_logprobs(const void* logits, int dtype, const long long* tokens, float* logprobs, float* entropy, float* top_logprobs,
