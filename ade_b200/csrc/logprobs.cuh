@@ -1,5 +1,11 @@
 // Log probabilities of given tokens, the entropy of the distribution and the likeliest tokens, from a row of logits:
 //   m = max x, s = sum exp(x - m), lse = m + log s;   log p = x - lse;   H = log s - sum exp(x - m) (x - m) / s.
+//
+// One CTA per row and one pass over it: every thread keeps the maximum of what it has seen, the sum and the weighted sum relative to
+// it, and rescales them when the maximum grows.  The maxima of 32 groups of threads bound the k-th largest logit from below (k of
+// them are reached by k logits), so only the few threads whose own maximum reaches that bound look at their logits again, and
+// the handful that they list is ranked by counting.  A row whose list would not fit (thousands of equal logits at the bound) or
+// that holds a NaN is walked once for every alternative instead.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -8,8 +14,8 @@
 
 namespace ade {
 
-constexpr int LP_THREADS = 256;
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_LIST = 512;       // logits that may reach the bound
 
 struct LogprobParams {
     const void* x;                 // [rows][vocab], rows `stride` elements apart
@@ -25,6 +31,17 @@ __device__ __forceinline__ float lp_float(float v) { return v; }
 __device__ __forceinline__ float lp_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float lp_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// the logits of a 16-byte piece
+template <typename T>
+struct LpPiece {
+    static constexpr int N = 16 / sizeof(T);
+    static __device__ __forceinline__ void get(const uint4& w, float (&v)[N]) {
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = lp_float(e[i]);
+    }
+};
+
 // Order of the alternatives: larger logits first, NaN before all, equal ones by the lower index.  The larger key comes first.
 __device__ __forceinline__ unsigned long long lp_key(float v, int i) {
     uint32_t u = __float_as_uint(v + 0.0f);                  // -0 counts as +0
@@ -32,58 +49,184 @@ __device__ __forceinline__ unsigned long long lp_key(float v, int i) {
     return static_cast<unsigned long long>(u) << 32 | ~static_cast<uint32_t>(i);
 }
 
-template <typename Op, typename T>
-__device__ __forceinline__ T lp_reduce(T v, T* ws, Op op) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = ws[0];
-    for (int w = 1; w < LP_THREADS / 32; ++w) v = op(v, ws[w]);
-    return v;
-}
-
-// One CTA per row: a pass for the maximum, one for the sums, one for each alternative.
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprob_kernel(const LogprobParams p) {
-    __shared__ float wf[LP_THREADS / 32];
-    __shared__ unsigned long long wk[LP_THREADS / 32];
-    const int tid = threadIdx.x;
-    const T* x = static_cast<const T*>(p.x) + blockIdx.x * p.stride;
-    auto add = [](float a, float b) { return a + b; };
-    float m = -INFINITY;
-    for (int i = tid; i < p.vocab; i += LP_THREADS) m = fmaxf(m, lp_float(x[i]));
-    m = lp_reduce(m, wf, [](float a, float b) { return fmaxf(a, b); });
-    float s = 0.f, e = 0.f;
-    for (int i = tid; i < p.vocab; i += LP_THREADS) {
-        const float z = lp_float(x[i]) - m, w = expf(z);
-        s += w;
-        e += w == 0.f ? 0.f : w * z;                           // a token of no probability adds nothing, -inf among them
+// (maximum, sum of exp(x - maximum), sum of exp(x - maximum) (x - maximum)) of some logits
+struct LpSums {
+    float m, s, e;
+    // the same relative to another maximum, which is at least as large; the difference is kept where its product with a sum is finite (a logit may
+    // be the lowest float32), exp is 0 long before that
+    __device__ __forceinline__ void move(float to) {
+        const float d = fmaxf(m - to, -1e30f), f = exp2f(d * 1.44269504088896340736f);
+        if (m != -INFINITY) {                                // without a maximum the sums are 0, or NaN
+            e = f * (e + s * d);
+            s *= f;
+        }
+        m = to;
     }
-    s = lp_reduce(s, wf, add);
-    e = lp_reduce(e, wf, add);
+    // what the logits are taken relative to: without a maximum (nothing but -inf so far, which adds nothing, and NaN, which shows) the logits themselves
+    __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+    __device__ __forceinline__ void add(float x, float base) {
+        const float z = x - base, w = exp2f(z * 1.44269504088896340736f);
+        s += w;
+        e += w * fmaxf(z, -1e30f);                           // a token of no probability adds nothing, -inf among them
+    }
+};
+
+// THREADS threads per row: 1024 where there are few rows.  Pieces of 16 bytes from the first 16-byte boundary of the row; what stands before it
+// and behind the last whole piece goes to the first threads one by one.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 5) logprob_kernel(const LogprobParams p) {
+    using P = LpPiece<T>;
+    constexpr int NW = THREADS / 32, U = 4, G = THREADS / 32;                // pieces in flight; threads of a group (32 groups)
+    __shared__ LpSums ws[NW];
+    __shared__ float gmax[32];
+    __shared__ unsigned long long list[LP_LIST], wk[NW];
+    __shared__ int listed;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const T* x = static_cast<const T*>(p.x) + blockIdx.x * p.stride;
+    const int V = p.vocab;
+    const int head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
+    const int pieces = (V - head) / P::N, tail = head + pieces * P::N;
+    const uint4* body = reinterpret_cast<const uint4*>(x + head);
+    const int edge = tid < head ? tid : tail + tid - head;                   // this thread's logit outside the pieces, if below V
+    if (tid == 0) listed = 0;
+
+    LpSums a = {-INFINITY, 0.f, 0.f};
+    if (edge < V) {
+        const float v = lp_float(x[edge]);
+        a.m = fmaxf(a.m, v);
+        a.add(v, a.base());
+    }
+    int i = tid;
+    for (; i + (U - 1) * THREADS < pieces; i += U * THREADS) {
+        uint4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = __ldg(body + i + u * THREADS);
+        float v[U][P::N], mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            P::get(w[u], v[u]);
+#pragma unroll
+            for (int j = 0; j < P::N; ++j) mx = fmaxf(mx, v[u][j]);
+        }
+        if (mx > a.m) a.move(mx);
+        const float base = a.base();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < P::N; ++j) a.add(v[u][j], base);
+    }
+    for (; i < pieces; i += THREADS) {
+        float v[P::N];
+        P::get(__ldg(body + i), v);
+        float mx = v[0];
+#pragma unroll
+        for (int j = 1; j < P::N; ++j) mx = fmaxf(mx, v[j]);
+        if (mx > a.m) a.move(mx);
+        const float base = a.base();
+#pragma unroll
+        for (int j = 0; j < P::N; ++j) a.add(v[j], base);
+    }
+    const float mine = a.m;
+    // maxima of the groups, then everything relative to the row's maximum
+    float g = mine;
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+    if (tid % G == 0) gmax[tid / G] = g;
+    __syncthreads();
+    g = gmax[lane];
+    float m = g;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    a.move(m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xFFFFFFFFu, a.s, o);
+        a.e += __shfl_xor_sync(0xFFFFFFFFu, a.e, o);
+    }
+    if (lane == 0) ws[warp] = a;
+    __syncthreads();
+    float s = 0.f, e = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        s += ws[w].s;
+        e += ws[w].e;
+    }
     const float ls = logf(s);
+    auto logp = [&](float v) { return (v - m) - ls; };
     if (tid == 0) {
         p.entropy[blockIdx.x] = ls - e / s;
         if (p.tokens) {
             const long long k = p.tokens[blockIdx.x];
-            p.logprob[blockIdx.x] = k < 0 ? 0.f : k >= p.vocab ? __uint_as_float(0x7FC00000u) : (lp_float(x[k]) - m) - ls;
+            p.logprob[blockIdx.x] = k < 0 ? 0.f : k >= V ? __uint_as_float(0x7FC00000u) : logp(lp_float(x[k]));
         }
     }
+    if (p.top == 0) return;
+    auto put = [&](int j, unsigned long long key) {
+        const uint32_t at = ~static_cast<uint32_t>(key);
+        p.top_token[static_cast<long long>(blockIdx.x) * p.top + j] = at;
+        p.top_logprob[static_cast<long long>(blockIdx.x) * p.top + j] = logp(lp_float(x[at]));
+    };
+    bool walk = !(s > 0.f);                                                  // NaN, an infinity, or nothing but -inf
+    if (!walk) {
+        // the top-th largest of the 32 maxima (equal ones by their place)
+        int rank = 0;
+#pragma unroll
+        for (int o = 0; o < 32; ++o) {
+            const float u = __shfl_sync(0xFFFFFFFFu, g, o);
+            rank += u > g || (u == g && o < lane);
+        }
+        const float bound = __shfl_sync(0xFFFFFFFFu, g, __ffs(__ballot_sync(0xFFFFFFFFu, rank == p.top - 1)) - 1);
+        if (mine >= bound) {
+            auto list_it = [&](float v, int at) {
+                if (!(v >= bound)) return;
+                const int n = atomicAdd(&listed, 1);
+                if (n < LP_LIST) list[n] = lp_key(v, at);
+            };
+            if (edge < V) list_it(lp_float(x[edge]), edge);
+            for (int k = tid; k < pieces && listed <= LP_LIST; k += THREADS) {
+                float v[P::N];
+                P::get(__ldg(body + k), v);
+#pragma unroll
+                for (int j = 0; j < P::N; ++j) list_it(v[j], head + k * P::N + j);
+            }
+        }
+        __syncthreads();
+        const int n = listed;
+        walk = n > LP_LIST;
+        if (!walk)
+            for (int k = tid; k < n; k += THREADS) {
+                const unsigned long long key = list[k];
+                int before = 0;
+                for (int j = 0; j < n; ++j) before += list[j] > key;
+                if (before < p.top) put(before, key);
+            }
+    }
+    if (!walk) return;
     unsigned long long below = ~0ull;
     for (int j = 0; j < p.top; ++j) {
         unsigned long long best = 0;
-        for (int i = tid; i < p.vocab; i += LP_THREADS) {
-            const unsigned long long k = lp_key(lp_float(x[i]), i);
-            if ((j == 0 || k < below) && k > best) best = k;
+        auto look = [&](float v, int at) {
+            const unsigned long long key = lp_key(v, at);
+            if ((j == 0 || key < below) && key > best) best = key;
+        };
+        if (edge < V) look(lp_float(x[edge]), edge);
+        for (int k = tid; k < pieces; k += THREADS) {
+            float v[P::N];
+            P::get(__ldg(body + k), v);
+#pragma unroll
+            for (int q = 0; q < P::N; ++q) look(v[q], head + k * P::N + q);
         }
-        below = lp_reduce(best, wk, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-        if (tid == 0) {
-            const uint32_t i = ~static_cast<uint32_t>(below);
-            p.top_token[static_cast<long long>(blockIdx.x) * p.top + j] = i;
-            p.top_logprob[static_cast<long long>(blockIdx.x) * p.top + j] = (lp_float(x[i]) - m) - ls;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long u = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+            best = u > best ? u : best;
         }
+        __syncthreads();
+        if (lane == 0) wk[warp] = best;
+        __syncthreads();
+        below = wk[0];
+        for (int w = 1; w < NW; ++w) below = wk[w] > below ? wk[w] : below;
+        if (tid == 0) put(j, below);
     }
 }
 
