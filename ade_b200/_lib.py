@@ -47,7 +47,7 @@ EXPORTS = (
     "ade_b200_factored_static", "ade_b200_factored_static_status", "ade_b200_recon", "ade_b200_expand_codes",
     "ade_b200_recon_expanded", "ade_b200_expand_codes_f8", "ade_b200_recon_expanded_f8", "ade_b200_set_option",
     "ade_b200_rmsnorm", "ade_b200_add_rmsnorm", "ade_b200_rope", "ade_b200_silu_mul", "ade_b200_attn_decode",
-    "ade_b200_paged_extend", "ade_b200_paged_write", "ade_b200_paged_attn", "ade_b200_paged_attn_workspace_bytes",
+    "ade_b200_paged_extend", "ade_b200_paged_extend_workspace_bytes", "ade_b200_paged_write", "ade_b200_paged_attn", "ade_b200_paged_attn_workspace_bytes",
     "ade_b200_multi_delta", "ade_b200_multi_delta_workspace_bytes", "ade_b200_token_logprobs",
 )
 
@@ -138,7 +138,8 @@ def load() -> ctypes.CDLL:
     lib.ade_b200_attn_decode.argtypes = [vp] * 11 + [ci] * 5 + [ll] * 5 + [ctypes.c_float, vp]
     for name in ("ade_b200_rmsnorm", "ade_b200_add_rmsnorm", "ade_b200_rope", "ade_b200_silu_mul", "ade_b200_attn_decode"):
         getattr(lib, name).restype = ci
-    lib.ade_b200_paged_extend.argtypes = [vp] * 11 + [ci, ci, ll, ci, ci, ci, vp]
+    lib.ade_b200_paged_extend.argtypes = [vp] * 12 + [sz, ci, ci, ll, ci, ci, ci, vp]
+    lib.ade_b200_paged_extend_workspace_bytes.argtypes = [ci]
     lib.ade_b200_paged_write.argtypes = [vp] * 7 + [ci] * 5 + [ll] * 5 + [vp]
     lib.ade_b200_paged_attn.argtypes = [vp] * 10 + [sz] + [ci] * 3 + [ll] + [ci] * 5 + [ll] * 3 + [ctypes.c_float, vp]
     lib.ade_b200_paged_attn_workspace_bytes.argtypes = [ci] * 4
@@ -147,7 +148,7 @@ def load() -> ctypes.CDLL:
     lib.ade_b200_token_logprobs.argtypes = [vp, ci, vp, vp, vp, vp, vp, ci, ci, ll, ci, vp]
     for name in ("ade_b200_paged_extend", "ade_b200_paged_write", "ade_b200_paged_attn", "ade_b200_multi_delta", "ade_b200_token_logprobs"):
         getattr(lib, name).restype = ci
-    for name in ("ade_b200_paged_attn_workspace_bytes", "ade_b200_multi_delta_workspace_bytes"):
+    for name in ("ade_b200_paged_extend_workspace_bytes", "ade_b200_paged_attn_workspace_bytes", "ade_b200_multi_delta_workspace_bytes"):
         getattr(lib, name).restype = sz
     lib.ade_b200_set_option.argtypes = [ci, ctypes.c_longlong]
     lib.ade_b200_set_option.restype = ci

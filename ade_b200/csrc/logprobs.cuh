@@ -3,7 +3,7 @@
 //
 // One CTA per row and one pass over it: every thread keeps the maximum of what it has seen, the sum and the weighted sum relative to
 // it, and rescales them when the maximum grows.  The maxima of 32 groups of threads bound the k-th largest logit from below (k of
-// them are reached by k logits), so only the few threads whose own maximum reaches that bound look at their logits again, and
+// them are reached by k logits), so only the logits of the few threads whose own maximum reaches that bound are looked at again, and
 // the handful that they list is ranked by counting.  A row whose list would not fit (thousands of equal logits at the bound) or
 // that holds a NaN is walked once for every alternative instead.
 #pragma once
@@ -11,6 +11,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 namespace ade {
 
@@ -35,6 +37,11 @@ __device__ __forceinline__ float lp_float(__nv_bfloat16 v) { return __bfloat162f
 template <typename T>
 struct LpPiece {
     static constexpr int N = 16 / sizeof(T);
+    // a piece of nothing but -inf
+    static __device__ __forceinline__ uint4 none() {
+        constexpr uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+        return make_uint4(w, w, w, w);
+    }
     static __device__ __forceinline__ void get(const uint4& w, float (&v)[N]) {
         const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
@@ -49,13 +56,19 @@ __device__ __forceinline__ unsigned long long lp_key(float v, int i) {
     return static_cast<unsigned long long>(u) << 32 | ~static_cast<uint32_t>(i);
 }
 
-// (maximum, sum of exp(x - maximum), sum of exp(x - maximum) (x - maximum)) of some logits
+__device__ __forceinline__ float lp_exp2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// maximum m of some logits, sum of w = 2^z and of w z, where z = (x - m) log2(e)
 struct LpSums {
     float m, s, e;
     // the same relative to another maximum, which is at least as large; the difference is kept where its product with a sum is finite (a logit may
     // be the lowest float32), exp is 0 long before that
     __device__ __forceinline__ void move(float to) {
-        const float d = fmaxf(m - to, -1e30f), f = exp2f(d * 1.44269504088896340736f);
+        const float d = fmaxf((m - to) * 1.44269504088896340736f, -1e30f), f = lp_exp2(d);
         if (m != -INFINITY) {                                // without a maximum the sums are 0, or NaN
             e = f * (e + s * d);
             s *= f;
@@ -65,18 +78,18 @@ struct LpSums {
     // what the logits are taken relative to: without a maximum (nothing but -inf so far, which adds nothing, and NaN, which shows) the logits themselves
     __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
     __device__ __forceinline__ void add(float x, float base) {
-        const float z = x - base, w = exp2f(z * 1.44269504088896340736f);
+        const float z = (x - base) * 1.44269504088896340736f, w = lp_exp2(z);
         s += w;
         e += w * fmaxf(z, -1e30f);                           // a token of no probability adds nothing, -inf among them
     }
 };
 
 // THREADS threads per row: 1024 where there are few rows.  Pieces of 16 bytes from the first 16-byte boundary of the row; what stands before it
-// and behind the last whole piece goes to the first threads one by one.
+// and behind the last whole piece goes to the first threads one by one.  A batch of pieces is requested while the one before it is added.
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 5) logprob_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 4) logprob_kernel(const LogprobParams p) {
     using P = LpPiece<T>;
-    constexpr int NW = THREADS / 32, U = 4, G = THREADS / 32;                // pieces in flight; threads of a group (32 groups)
+    constexpr int NW = THREADS / 32, U = 4, G = THREADS / 32;                // pieces of a batch; threads of a group (32 groups)
     __shared__ LpSums ws[NW];
     __shared__ float gmax[32];
     __shared__ unsigned long long list[LP_LIST], wk[NW];
@@ -96,35 +109,32 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 5) logprob_kern
         a.m = fmaxf(a.m, v);
         a.add(v, a.base());
     }
-    int i = tid;
-    for (; i + (U - 1) * THREADS < pieces; i += U * THREADS) {
-        uint4 w[U];
+    uint4 cur[U], next[U];
+    auto load = [&](uint4 (&w)[U], int i) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) w[u] = __ldg(body + i + u * THREADS);
+        for (int u = 0; u < U; ++u) {
+            w[u] = P::none();
+            if (i + u * THREADS < pieces) w[u] = __ldg(body + i + u * THREADS);
+        }
+    };
+    load(cur, tid);
+    for (int i = tid; i < pieces; i += U * THREADS) {
+        load(next, i + U * THREADS);
         float v[U][P::N], mx = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            P::get(w[u], v[u]);
+            P::get(cur[u], v[u]);
 #pragma unroll
             for (int j = 0; j < P::N; ++j) mx = fmaxf(mx, v[u][j]);
         }
         if (mx > a.m) a.move(mx);
         const float base = a.base();
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int j = 0; j < P::N; ++j) a.add(v[u][j], base);
-    }
-    for (; i < pieces; i += THREADS) {
-        float v[P::N];
-        P::get(__ldg(body + i), v);
-        float mx = v[0];
-#pragma unroll
-        for (int j = 1; j < P::N; ++j) mx = fmaxf(mx, v[j]);
-        if (mx > a.m) a.move(mx);
-        const float base = a.base();
-#pragma unroll
-        for (int j = 0; j < P::N; ++j) a.add(v[j], base);
+            cur[u] = next[u];
+        }
     }
     const float mine = a.m;
     // maxima of the groups, then everything relative to the row's maximum
@@ -154,7 +164,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 5) logprob_kern
     const float ls = logf(s);
     auto logp = [&](float v) { return (v - m) - ls; };
     if (tid == 0) {
-        p.entropy[blockIdx.x] = ls - e / s;
+        p.entropy[blockIdx.x] = ls - 0.69314718055994530942f * (e / s);
         if (p.tokens) {
             const long long k = p.tokens[blockIdx.x];
             p.logprob[blockIdx.x] = k < 0 ? 0.f : k >= V ? __uint_as_float(0x7FC00000u) : logp(lp_float(x[k]));
@@ -176,14 +186,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 5) logprob_kern
             rank += u > g || (u == g && o < lane);
         }
         const float bound = __shfl_sync(0xFFFFFFFFu, g, __ffs(__ballot_sync(0xFFFFFFFFu, rank == p.top - 1)) - 1);
-        if (mine >= bound) {
-            auto list_it = [&](float v, int at) {
-                if (!(v >= bound)) return;
-                const int n = atomicAdd(&listed, 1);
-                if (n < LP_LIST) list[n] = lp_key(v, at);
-            };
-            if (edge < V) list_it(lp_float(x[edge]), edge);
-            for (int k = tid; k < pieces && listed <= LP_LIST; k += THREADS) {
+        auto list_it = [&](float v, int at) {
+            if (!(v >= bound)) return;
+            const int n = atomicAdd(&listed, 1);
+            if (n < LP_LIST) list[n] = lp_key(v, at);
+        };
+        if (edge < V) list_it(lp_float(x[edge]), edge);
+        // the warp goes through the pieces of each of its threads that reach the bound, a piece per lane
+        for (uint32_t who = __ballot_sync(0xFFFFFFFFu, mine >= bound); who; who &= who - 1) {
+            const int t = warp * 32 + __ffs(who) - 1;
+            for (int k = t + lane * THREADS; k < pieces; k += 32 * THREADS) {
                 float v[P::N];
                 P::get(__ldg(body + k), v);
 #pragma unroll

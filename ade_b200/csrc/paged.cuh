@@ -19,9 +19,7 @@ __device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
 }
 
 // ------------------------------------------------------------------ page allocation, block tables, slot maps
-constexpr int PX_THREADS = 1024;
 constexpr int PX_MAX_REQUESTS = 4096;
-constexpr int PX_ITEMS = PX_MAX_REQUESTS / PX_THREADS;       // requests per thread of the scans
 
 struct ExtendParams {
     const int* lengths;          // [B] tokens each request has
@@ -32,36 +30,20 @@ struct ExtendParams {
     int *lengths_out, *count_out, *status;
     long long *slots, *positions;    // [total]
     int* requests;                   // [total]
+    int* work;                       // [4 + 4 B] scalars and sums, from the first launch of two to the second
     int B, width, pages, page_size, total;
     long long table_stride;
 };
 
 enum { PX_OK = 0, PX_NO_PAGE = 1, PX_TABLE_FULL = 2, PX_NO_ROW = 3, PX_BAD_LENGTH = 4 };
 
-// inclusive prefix sums over the CTA of `v`, one value per thread; `ws`: 33 words
-__device__ __forceinline__ long long px_scan(long long v, long long* ws) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xFFFFFFFFu, v, o);
-        if (lane >= o) v += u;
-    }
-    if (lane == 31) ws[warp] = v;
-    __syncthreads();
-    if (warp == 0) {
-        long long s = ws[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xFFFFFFFFu, s, o);
-            if (lane >= o) s += u;
-        }
-        ws[lane] = s;
-    }
-    __syncthreads();
-    const long long base = warp ? ws[warp - 1] : 0;
-    __syncthreads();
-    return base + v;
-}
+// What the requests come to, in shared memory: inclusive sums over the requests of the rows of the packed batch, the pages handed back and
+// the pages taken, and each request's old length (-1: it has no rows).
+struct PxSums {
+    int *row_end, *back_end, *need_end, *len;
+    int count, available, used;          // height of the stack before, with the pages handed back, and pages taken from it
+};
+inline size_t px_smem_bytes(int B) { return 4 * static_cast<size_t>(B) * sizeof(int); }
 
 // smallest b with sums[b] > i, for ascending sums
 __device__ __forceinline__ int px_find(const int* sums, int n, int i) {
@@ -74,25 +56,40 @@ __device__ __forceinline__ int px_find(const int* sums, int n, int i) {
     return lo;
 }
 
-// One CTA.  Three prefix sums over the requests (rows of the packed batch, pages handed back, pages needed) say which row, page
-// and stack entry belongs to whom; everything behind them is independent per row and per page.  The sums are kept in 64
-// bits until they are compared with `total` and the number of pages, and saturated to 31 bits behind that.
-__global__ void __launch_bounds__(PX_THREADS) paged_extend_kernel(const ExtendParams p) {
-    extern __shared__ int px_smem[];
-    int* row_end = px_smem;              // [B] inclusive sums of the rows
-    int* back_end = row_end + p.B;       // [B] ... of the pages handed back
-    int* need_end = back_end + p.B;      // [B] ... of the pages needed
-    __shared__ long long ws[33];
-    __shared__ int s_used;
-    const int tid = threadIdx.x, b0 = tid * PX_ITEMS;
+// Inclusive prefix sums over a CTA of NT threads; `ws`: a word per warp that nothing else uses.
+template <int NT>
+__device__ __forceinline__ long long px_scan(long long v, long long* ws) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) ws[warp] = v;
+    __syncthreads();
+    long long base = lane < warp ? ws[lane] : 0;                 // at most 32 warps
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xFFFFFFFFu, base, o);
+    return v + base;
+}
+
+// The sums, the new lengths and the states, by one CTA.  Sums are kept in 64 bits until they are compared with `total` and the number
+// of pages, and saturated to 31 bits behind that.  Every thread has read lengths and free_count before any writes them: the outputs may be
+// the same arrays.
+template <int NT, int ITEMS>
+__device__ __forceinline__ PxSums px_sum(const ExtendParams& p, int* smem) {
+    __shared__ long long ws[3][NT / 32];
+    __shared__ int s_used, s_back;
+    PxSums r = {smem, smem + p.B, smem + 2 * p.B, smem + 3 * p.B, 0, 0, 0};
+    const int tid = threadIdx.x, b0 = tid * ITEMS;
     const long long kSat = 0x7FFFFFFF;
     if (tid == 0) s_used = 0;
-    int len[PX_ITEMS], grow[PX_ITEMS], have[PX_ITEMS], last[PX_ITEMS], st[PX_ITEMS];
-    bool rel[PX_ITEMS];
-    const int count = min(max(*p.free_count, 0), p.pages);
+    int len[ITEMS], grow[ITEMS], have[ITEMS], last[ITEMS], st[ITEMS];
+    bool rel[ITEMS];
+    r.count = min(max(*p.free_count, 0), p.pages);
     long long rows = 0, back = 0;
 #pragma unroll
-    for (int i = 0; i < PX_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         const int b = b0 + i;
         len[i] = grow[i] = have[i] = last[i] = 0;
         st[i] = PX_OK;
@@ -100,10 +97,10 @@ __global__ void __launch_bounds__(PX_THREADS) paged_extend_kernel(const ExtendPa
         if (b < p.B) {
             len[i] = p.lengths[b];
             const int f = p.fresh[b];
-            if (len[i] < 0 || len[i] > static_cast<long long>(p.width) * p.page_size) {
+            if (len[i] < 0 || len[i] > p.width * p.page_size) {
                 st[i] = PX_BAD_LENGTH;
             } else {
-                have[i] = static_cast<int>((len[i] + static_cast<long long>(p.page_size) - 1) / p.page_size);
+                have[i] = (len[i] + p.page_size - 1) / p.page_size;
                 rel[i] = f < 0;
                 grow[i] = max(f, 0);
                 const long long end = (static_cast<long long>(len[i]) + grow[i] + p.page_size - 1) / p.page_size;
@@ -114,83 +111,102 @@ __global__ void __launch_bounds__(PX_THREADS) paged_extend_kernel(const ExtendPa
         rows += grow[i];
         back += rel[i] ? have[i] : 0;
     }
-    long long row_at = px_scan(rows, ws) - rows, back_at = px_scan(back, ws) - back;
-    long long need = 0;
+    long long row_at = px_scan<NT>(rows, ws[0]) - rows, back_at = px_scan<NT>(back, ws[1]) - back, need = 0;
 #pragma unroll
-    for (int i = 0; i < PX_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         const int b = b0 + i;
         row_at += grow[i];
         back_at += rel[i] ? have[i] : 0;
         if (b < p.B) {
             if (row_at > p.total && !rel[i] && st[i] != PX_BAD_LENGTH) st[i] = PX_NO_ROW;
-            row_end[b] = static_cast<int>(min(row_at, kSat));
-            back_end[b] = static_cast<int>(min(back_at, kSat));
+            r.row_end[b] = static_cast<int>(min(row_at, kSat));
+            r.back_end[b] = static_cast<int>(min(back_at, kSat));
+            if (b == p.B - 1) s_back = r.back_end[b];
             if (st[i] == PX_OK && !rel[i]) need += last[i] - have[i];
         }
     }
-    long long need_at = px_scan(need, ws) - need;
-    const int back_total = back_end[p.B - 1];
-    const int available = static_cast<int>(min(static_cast<long long>(count) + back_total, static_cast<long long>(p.pages)));
+    long long need_at = px_scan<NT>(need, ws[2]) - need;
+    r.available = static_cast<int>(min(static_cast<long long>(r.count) + s_back, static_cast<long long>(p.pages)));
     int used = 0;
 #pragma unroll
-    for (int i = 0; i < PX_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         const int b = b0 + i;
         if (b < p.B) {
-            const bool asks = st[i] == PX_OK && !rel[i] && last[i] > have[i];
-            if (asks) {
+            if (st[i] == PX_OK && !rel[i] && last[i] > have[i]) {
                 need_at += last[i] - have[i];
-                if (need_at > available) st[i] = PX_NO_PAGE;
+                if (need_at > r.available) st[i] = PX_NO_PAGE;
                 else used = static_cast<int>(need_at);
             }
-            need_end[b] = static_cast<int>(min(need_at, kSat));
+            const bool grows = st[i] == PX_OK && !rel[i];
+            r.need_end[b] = static_cast<int>(min(need_at, kSat));
+            r.len[b] = grows ? len[i] : -1;
             p.status[b] = st[i];
+            p.lengths_out[b] = rel[i] ? 0 : grows ? len[i] + grow[i] : len[i];
         }
     }
     if (used) atomicMax(&s_used, used);
-    __syncthreads();                         // every thread has read lengths and free_count: they may be the outputs
-    used = s_used;
-#pragma unroll
-    for (int i = 0; i < PX_ITEMS; ++i)
-        if (b0 + i < p.B) p.lengths_out[b0 + i] = rel[i] ? 0 : st[i] == PX_OK ? len[i] + grow[i] : len[i];
-    if (tid == 0) *p.count_out = available - used;
-    __syncthreads();                         // status and lengths_out of every request are in place
+    __syncthreads();
+    r.used = s_used;
+    if (tid == 0) *p.count_out = r.available - r.used;
+    return r;
+}
+
+// Stack, table and rows from the sums, by `threads` threads of which this is number `at`; all of it independent.  What is read of the stack lies
+// below its old height and what is read of the table belongs to requests that end or to pages that a request had, and neither is
+// written here.
+__device__ __forceinline__ void px_place(const ExtendParams& p, const PxSums& r, int at, int threads) {
     // entry i of the stack once the pages handed back lie on it
     auto stack = [&](int i) {
-        if (i < count) return p.free_pages[i];
-        const int b = px_find(back_end, p.B, i - count);
-        return p.table[b * p.table_stride + (i - count - (b ? back_end[b - 1] : 0))];
+        if (i < r.count) return p.free_pages[i];
+        const int b = px_find(r.back_end, p.B, i - r.count);
+        return p.table[b * p.table_stride + (i - r.count - (b ? r.back_end[b - 1] : 0))];
     };
-    for (int i = tid; i < available - count; i += PX_THREADS) p.free_pages[count + i] = stack(count + i);
-    // pages taken: the i-th of all comes from the i-th place below the top.  A request's own entries lie behind those it has,
-    // so no entry that is read here (a released request's) is written.
-    for (int i = tid; i < used; i += PX_THREADS) {
-        const int b = px_find(need_end, p.B, i);
-        const int first = b ? need_end[b - 1] : 0;
-        const long long len_b = p.lengths_out[b] - p.fresh[b];
-        const int col = static_cast<int>((len_b + p.page_size - 1) / p.page_size) + i - first;
-        p.table[b * p.table_stride + col] = stack(available - 1 - i);
+    for (int i = r.count + at; i < r.available; i += threads) p.free_pages[i] = stack(i);
+    // the i-th page of all that are taken comes from the i-th place below the top
+    for (int i = at; i < r.used; i += threads) {
+        const int b = px_find(r.need_end, p.B, i);
+        const int col = (r.len[b] + p.page_size - 1) / p.page_size + i - (b ? r.need_end[b - 1] : 0);
+        p.table[b * p.table_stride + col] = stack(r.available - 1 - i);
     }
-    // rows of the packed batch
-    for (int r = tid; r < p.total; r += PX_THREADS) {
+    for (int row = at; row < p.total; row += threads) {
         long long slot = -1, pos = 0;
         int req = -1;
-        const int b = px_find(row_end, p.B, r);
-        if (b < p.B && p.status[b] == PX_OK) {
-            const int start = b ? row_end[b - 1] : 0;
-            const int len_b = p.lengths_out[b] - p.fresh[b];
-            const int at = len_b + r - start, col = at / p.page_size;
-            const int have_b = (len_b + p.page_size - 1) / p.page_size;
-            const int page = col < have_b ? p.table[b * p.table_stride + col] : stack(available - 1 - ((b ? need_end[b - 1] : 0) + col - have_b));
+        const int b = px_find(r.row_end, p.B, row);
+        if (b < p.B && r.len[b] >= 0) {
+            const int len = r.len[b], to = len + row - (b ? r.row_end[b - 1] : 0), col = to / p.page_size;
+            const int have = (len + p.page_size - 1) / p.page_size;
+            const int page = col < have ? p.table[b * p.table_stride + col] : stack(r.available - 1 - ((b ? r.need_end[b - 1] : 0) + col - have));
             if (page >= 0 && page < p.pages) {
-                slot = static_cast<long long>(page) * p.page_size + at % p.page_size;
-                pos = at;
+                slot = static_cast<long long>(page) * p.page_size + to - col * p.page_size;
+                pos = to;
                 req = b;
             }
         }
-        p.slots[r] = slot;
-        p.positions[r] = pos;
-        p.requests[r] = req;
+        p.slots[row] = slot;
+        p.positions[row] = pos;
+        p.requests[row] = req;
     }
+}
+
+// One CTA for all of it (a decode step), or, with `split`, for the sums alone, which paged_place_kernel takes from `work`.
+template <int NT, int ITEMS>
+__global__ void __launch_bounds__(NT) paged_extend_kernel(const ExtendParams p, bool split) {
+    extern __shared__ int px_smem[];
+    const PxSums r = px_sum<NT, ITEMS>(p, px_smem);
+    if (!split) return px_place(p, r, threadIdx.x, NT);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) *reinterpret_cast<int4*>(p.work) = make_int4(r.count, r.available, r.used, 0);
+    for (int i = threadIdx.x; i < 4 * p.B; i += NT) p.work[4 + i] = px_smem[i];
+}
+
+// The second of two launches for many rows.
+__global__ void __launch_bounds__(256) paged_place_kernel(const ExtendParams p) {
+    extern __shared__ int px_smem[];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = threadIdx.x; i < 4 * p.B; i += 256) px_smem[i] = p.work[4 + i];
+    const int4 s = *reinterpret_cast<const int4*>(p.work);
+    __syncthreads();
+    px_place(p, {px_smem, px_smem + p.B, px_smem + 2 * p.B, px_smem + 3 * p.B, s.x, s.y, s.z}, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ------------------------------------------------------------------ keys and values of new tokens into their pages

@@ -33,6 +33,9 @@ int launch_early(void (*kernel)(Params...), int grid, int threads, size_t smem, 
     return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, args...)) ? ADE_OK : ADE_ERR_CUDA;
 }
 
+// Rows that one CTA of the page allocation still places itself.
+constexpr int kExtendOneCta = 2048;
+
 template <typename T>
 void launch_logprobs(const ade::LogprobParams& p, int sms, cudaStream_t st) {
     if (p.rows <= sms) ade::logprob_kernel<T, 1024><<<p.rows, 1024, 0, st>>>(p);
@@ -71,23 +74,39 @@ int launch_attn_dim(int head_dim, const ade::PagedAttnParams& p, int sms, cudaSt
 
 extern "C" {
 
+size_t ade_b200_paged_extend_workspace_bytes(int B) { return B < 1 || B > ADE_B200_MAX_REQUESTS ? 0 : 16 + ade::px_smem_bytes(B); }
+
 int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
                           int32_t* lengths_out, int32_t* free_count_out, int32_t* status, long long* slots, long long* positions, int32_t* requests,
-                          int B, int width, long long table_row_stride, int pages, int page_size, int total, void* stream) {
+                          void* work, size_t work_bytes, int B, int width, long long table_row_stride, int pages, int page_size, int total,
+                          void* stream) {
     if (!lengths || !new_tokens || !block_table || !free_pages || !free_count || !lengths_out || !free_count_out || !status) return ADE_ERR_NULL;
     if (total > 0 && (!slots || !positions || !requests)) return ADE_ERR_NULL;
     if (B < 1 || B > ADE_B200_MAX_REQUESTS || width < 1 || table_row_stride < width || pages < 1 || page_size < 1 || total < 0) return ADE_ERR_SHAPE;
     if (static_cast<long long>(width) * page_size > 0x7FFFFFFFll || total > (1 << 30)) return ADE_ERR_SHAPE;
+    if (!work) return ADE_ERR_NULL;
+    if (!aligned16(work)) return ADE_ERR_ALIGN;
+    if (work_bytes < ade_b200_paged_extend_workspace_bytes(B)) return ADE_ERR_SCRATCH;
     int sms = 0;
     const int rc = ade_host::sm_count(&sms);
     if (rc) return rc;
-    ade::ExtendParams p = {lengths, new_tokens, block_table, free_pages, free_count, lengths_out, free_count_out, status, slots, positions, requests,
-                           B, width, pages, page_size, total, table_row_stride};
-    const size_t smem = 3 * static_cast<size_t>(B) * sizeof(int);
-    if (smem > 40 * 1024 && !cuda_ok(cudaFuncSetAttribute(ade::paged_extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))))
+    const ade::ExtendParams p = {lengths, new_tokens, block_table, free_pages, free_count, lengths_out, free_count_out, status, slots, positions,
+                                 requests, static_cast<int*>(work), B, width, pages, page_size, total, table_row_stride};
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const size_t smem = ade::px_smem_bytes(B);
+    const bool split = total > kExtendOneCta;
+    if (B <= 128 && !split) {
+        ade::paged_extend_kernel<128, 1><<<1, 128, smem, st>>>(p, false);
+        return launched();
+    }
+    if (smem > 40 * 1024 &&
+        (!cuda_ok(cudaFuncSetAttribute(ade::paged_extend_kernel<1024, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))) ||
+         !cuda_ok(cudaFuncSetAttribute(ade::paged_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))))
         return ADE_ERR_CUDA;
-    ade::paged_extend_kernel<<<1, ade::PX_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(p);
-    return launched();
+    ade::paged_extend_kernel<1024, 4><<<1, 1024, smem, st>>>(p, split);
+    if (!split || !cuda_ok(cudaGetLastError())) return launched();
+    const int ctas = (total + 511) / 512;
+    return launch_early(ade::paged_place_kernel, ctas < 2 * sms ? ctas : 2 * sms, 256, smem, st, p);
 }
 
 int ade_b200_paged_write(const void* k, const void* v, const void* cos_t, const void* sin_t, const long long* slots, void* k_pages, void* v_pages,

@@ -91,11 +91,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> paged_extend(const Te
     const auto i32 = lengths.options(), i64 = lengths.options().dtype(at::kLong);
     Tensor slots = at::empty({total}, i64), positions = at::empty({total}, i64), requests = at::empty({total}, i32), status = at::empty({B}, i32);
     Tensor len_out = at::empty({in_place ? 0 : B}, i32), count_out = at::empty({in_place ? 0 : 1}, i32);       // an operator may not return an argument
+    const size_t bytes = ade_b200_paged_extend_workspace_bytes(as_int(B, "requests"));
+    const Tensor work = at::empty({static_cast<int64_t>(bytes)}, lengths.options().dtype(at::kByte));
     auto i = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
     auto l = [](const Tensor& t) { return static_cast<long long*>(t.data_ptr()); };
     check_rc(ade_b200_paged_extend(i(lengths), i(new_tokens), i(table), i(free_pages), i(free_count), i(in_place ? lengths : len_out),
                                    i(in_place ? free_count : count_out), i(status), l(slots),
-                                   l(positions), i(requests), as_int(B, "requests"), as_int(table.size(1), "width"), table_stride(table),
+                                   l(positions), i(requests), work.data_ptr(), bytes, as_int(B, "requests"), as_int(table.size(1), "width"),
+                                   table_stride(table),
                                    as_int(free_pages.size(0), "pages"), as_int(page_size, "page_size"), n, stream_of(table)),
              "ade_b200_paged_extend");
     return {slots, positions, requests, len_out, count_out, status};
