@@ -7,13 +7,17 @@
 //
 // Two launches, h = V^^T x and out = y + U^ h; the second is set up under the first.  Both find out on the device which rows share a
 // delta (ids may change from replay to replay of a graph) and cut them into entries of up to eight rows, so that a delta's codes
-// are read once for each entry, and from DRAM once.  Both are streams of 4-bit codes against a handful of token columns, on the warp matrix
-// instruction m16n8k16: the codes, as bfloat16 128 + c (one or two integer instructions for a pair), are its 16 rows, four token rows its
-// eight columns: columns 0-3 hold the bfloat16 rounding of a float32 operand (x vs, or h), columns 4-7 what that rounding left over, which
-// is free as long as an entry has at most four rows.  The zero-points come off afterwards: sum a (c - z) = sum a (128 + c) - sum a (128 + z),
-// whose second term is one more row of the product for V and a multiple of sum a for U; both sums are float32.
+// are read once for each entry, and from DRAM once.
+//
+// Both are streams of 4-bit codes against a handful of token columns, and what costs is the unpacking: integer instructions issue every other
+// cycle.  As bytes, eight codes take three of them (two ANDs and a shift) for the warp matrix instruction m16n8k32 of 8-bit
+// integers, which has twice the rate of m16n8k16; as bfloat16 pairs they take eleven (128 rows of 48 deltas, 11008 x 4096: 87 us then, half of that now).
+// So the codes are the instruction's 16 rows, and the token rows enter in fixed point: x vs over 128 columns, or h over the 128 ranks of a
+// group, scaled by a power of two to 16 bits, the upper eight in columns 0-3 (four rows of the entry), the lower eight in columns 4-7.  An operand
+// is thus held to 2^-16 to 2^-15 of the largest of its 128; the products and their sums, zero-points included, are exact integers, and
+// what is added across groups, columns and warps is float32.
 // Every thread copies the 16-byte pieces of codes that it will use itself with cp.async into a queue of its own, so the
-// stream runs through the barriers of an item and into the next one.  Sums have a fixed order; there are no atomics.
+// stream runs through the barriers of an item and into the next one.  Sums have a fixed order; there are no floating-point atomics.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -29,12 +33,12 @@ constexpr int MD_THREADS = 256;
 constexpr int MD_ENTRY = 8;                       // rows of an entry
 constexpr int MD_COLS = 1024;                     // columns of V^T that one item covers, 128 per warp
 constexpr int MD_H = MD_MAX_GROUPS * 128;         // floats of h kept per row and slice of columns
-constexpr int MD_CHUNK = 8;                       // rank groups of h in shared memory at a time
-constexpr int MD_UROWS = 256;                     // rows of U that one item covers, 32 per warp
 constexpr int MD_PART = 132;                      // row pitch of the warps' partial h, in floats
-constexpr int MD_HCOL = MD_CHUNK * 256 + 64;      // bytes of a column of h in shared memory; 64 over a multiple of 128: no bank conflicts
+constexpr int MD_HCOL = MD_MAX_GROUPS * 128 + 64; // bytes of a column of h in shared memory; 64 over a multiple of 128: no bank conflicts
+constexpr int MD_STAGE = 36;                      // row pitch of a warp's results, in floats
 constexpr int MD_UDEPTH = 4;                      // steps in the queue of the second launch
-constexpr uint32_t kMd128 = 0x43004300u;          // bf16x2 (128, 128)
+constexpr float kMdMagic = 12582912.f;            // 1.5 * 2^23: an integer below 2^22 added to its bits is added to its value
+constexpr int kMdMagicBits = 0x4B400000;
 
 struct MultiDeltaParams {
     const __nv_bfloat16 *x, *y;           // [T][N], [T][M]
@@ -52,11 +56,12 @@ struct MdEntries {
     int first[MD_MAX_ROWS], ng[MD_MAX_ROWS], rows[MD_MAX_ROWS];   // first rank group, their number, rows of the entry
     int groups_end[MD_MAX_ROWS];                                  // rank groups of this entry and those before it
     uint8_t row[MD_MAX_ROWS][MD_ENTRY];
-    int key[MD_MAX_ROWS], base[MD_MAX_ROWS], wsum[8];
+    alignas(16) int key[MD_MAX_ROWS];
+    int base[MD_MAX_ROWS], wsum[8];
 };
 
-constexpr size_t md_v_smem() { return 8 * 2 * MD_THREADS * 16 + 8 * MD_ENTRY * MD_PART * sizeof(float); }
-constexpr size_t md_u_smem() { return MD_UDEPTH * 4 * MD_THREADS * 16 + 16 * MD_HCOL + MD_CHUNK * 16 * sizeof(float); }
+constexpr size_t md_v_smem() { return 8 * 2 * MD_THREADS * 16 + 8 * MD_ENTRY * MD_PART * sizeof(float) + 8 * 384; }
+constexpr size_t md_u_smem() { return MD_UDEPTH * 4 * MD_THREADS * 16 + 16 * MD_HCOL + MD_MAX_GROUPS * 16 * sizeof(float2) + 8 * MD_ENTRY * MD_STAGE * sizeof(float); }
 inline int md_slices(int N) { return (N + MD_COLS - 1) / MD_COLS; }
 
 __device__ __forceinline__ void md_cp16(uint32_t dst, const void* src) {
@@ -73,8 +78,30 @@ __device__ __forceinline__ uint32_t md_pack(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// codes 2 j, 2 j + 1 of a packed word as bfloat16 128 + c
-__device__ __forceinline__ uint32_t md_pair(uint32_t w, int j) { return (w >> (4 * j) & 0x000F000Fu) | kMd128; }
+// D(16x8, s32) = A(16x32, u8, row) * B(32x8, s8, col) + C
+__device__ __forceinline__ void md_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const int (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+// The product of a packed word of two rows (eight codes each, as bytes 0 4 1 5 and 2 6 3 7) with those of a column, added to d.
+__device__ __forceinline__ void md_mma_word(int (&d)[4], uint32_t w0, uint32_t w1, uint32_t b0, uint32_t b1, const int (&c)[4]) {
+    md_mma(d, w0 & 0x0F0F0F0Fu, w1 & 0x0F0F0F0Fu, w0 >> 4 & 0x0F0F0F0Fu, w1 >> 4 & 0x0F0F0F0Fu, b0, b1, c);
+}
+__device__ __forceinline__ float md_max(float a, float b) {              // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Fixed point for values of magnitude up to m: v * scale is at most 32637, so its upper and lower eight bits are signed bytes; `unit` = 1 / scale, a
+// power of two (infinite or NaN where m is, so that results show it).
+struct MdFixed {
+    float scale, unit;
+};
+__device__ __forceinline__ MdFixed md_fixed(float m) {
+    const int e = max(static_cast<int>(__float_as_uint(m * 1.004f) >> 23 & 255u), 27);
+    return {__uint_as_float(static_cast<uint32_t>(268 - e) << 23), e == 255 ? m : __uint_as_float(static_cast<uint32_t>(e - 14) << 23)};
+}
 
 __device__ __forceinline__ void md_entries(const MultiDeltaParams& p, MdEntries& e) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -86,17 +113,25 @@ __device__ __forceinline__ void md_entries(const MultiDeltaParams& p, MdEntries&
             ng = max(0, min(min(p.start[d + 1], p.G) - first, MD_MAX_GROUPS));
         }
         e.key[t] = ng ? d : -1;                             // rows without a delta share an entry of no groups
+    } else if (t < MD_MAX_ROWS) {
+        e.key[t] = -2;
     }
     __syncthreads();
     int before = 0, same = 0, leader = t;
     if (t < p.T) {
         const int mine = e.key[t];
-        for (int u = p.T - 1; u >= 0; --u)
-            if (e.key[u] == mine) {
-                ++same;
-                before += u < t;
-                leader = u;
-            }
+#pragma unroll 4
+        for (int u = (p.T - 1) & ~3; u >= 0; u -= 4) {
+            const int4 k = *reinterpret_cast<const int4*>(&e.key[u]);
+            const int is[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+            for (int i = 3; i >= 0; --i)
+                if (is[i] == mine) {
+                    ++same;
+                    before += u + i < t;
+                    leader = u + i;
+                }
+        }
     }
     // entries and rank groups of each group of rows, at its first row, summed over the rows
     const int mine = t < p.T && leader == t ? (same + MD_ENTRY - 1) / MD_ENTRY : 0;
@@ -130,98 +165,129 @@ __device__ __forceinline__ void md_entries(const MultiDeltaParams& p, MdEntries&
 
 // ------------------------------------------------------------------ h = V^T x
 // An item is one rank group of one entry over MD_COLS columns: a warp multiplies the group's 128 ranks with 128 columns, eight tiles of 16
-// ranks one behind the other, and the warps' sums are added through shared memory.
-template <int N>
-struct MdTiles {
-    static constexpr int value = N;
-};
-
+// ranks one behind the other, and the warps' sums are added through shared memory.  Items go entry by entry, slice by slice, group by group, and a
+// CTA has a run of them.  The codes, scales and zero-points of an item are under way while the item before it is computed.
 struct MdVItem {
-    int e, j, slice;                       // entry, its rank group, slice of columns
+    int e, slice, j;                       // entry, slice of columns, rank group of the entry
 };
 
 __device__ __forceinline__ MdVItem md_v_item(const MdEntries& e, int item, int slices) {
-    const int g = item / slices;
-    int lo = 0, hi = e.n - 1;              // first entry with groups_end > g
+    int lo = 0, hi = e.n - 1;              // first entry with groups_end * slices > item
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (e.groups_end[mid] > g) hi = mid;
+        if (e.groups_end[mid] * slices > item) hi = mid;
         else lo = mid + 1;
     }
-    return {lo, g - (e.groups_end[lo] - e.ng[lo]), item - g * slices};
+    const int rest = item - (e.groups_end[lo] - e.ng[lo]) * slices;
+    return {lo, rest / e.ng[lo], rest % e.ng[lo]};
 }
 
-template <int NT>
-__device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const MdEntries& e, const MdVItem& it, int cb, uint32_t fifo, float* part, bool more,
-                                             const uint8_t* next) {
-    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-    const size_t g = e.first[it.e] + it.j, col = static_cast<size_t>(cb) * 128 + tig * 32;
-    uint32_t xs[NT][16], z[16];
-    {
-        uint4 zv[2], sv[4];
-        const uint4* zp = reinterpret_cast<const uint4*>(p.vz + g * p.N + col);
-        const uint4* sp = reinterpret_cast<const uint4*>(p.vs + g * p.N + col);
-        zv[0] = ldg16(zp);
-        zv[1] = ldg16(zp + 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sv[i] = ldg16(sp + i);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int r = n * 4 + (gid & 3);
-            uint4 xv[4] = {};
-            if (r < e.rows[it.e]) {
-                const uint4* xp = reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(e.row[it.e][r]) * p.N + col);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) xv[i] = ldg16(xp + i);
-            }
-            const uint32_t *xw = reinterpret_cast<const uint32_t*>(xv), *sw = reinterpret_cast<const uint32_t*>(sv);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float a = md_lo(xw[i]) * md_lo(sw[i]), b = md_hi(xw[i]) * md_hi(sw[i]);
-                const uint32_t hi = md_pack(a, b);
-                xs[n][i] = gid < 4 ? hi : md_pack(a - md_lo(hi), b - md_hi(hi));
-            }
+// The copies of one item: a warp's scales and zero-points, then the tiles of codes, each thread its own pieces.
+struct MdVCopy {
+    const uint8_t *codes, *scale;          // nullptr where there is nothing to copy
+    uint32_t fifo, side;                   // this thread's place in the queue; the warp's scales (256 bytes) and zero-points (128)
+    size_t pitch;                          // bytes of a row of codes
+    const uint8_t* zero;
+
+    __device__ __forceinline__ void sides(int lane) const {
+        if (codes) {
+            if (lane < 16) md_cp16(side + lane * 16, scale + lane * 16);
+            else if (lane < 24) md_cp16(side + lane * 16, zero + (lane - 16) * 16);
         }
-        const uint32_t* zw = reinterpret_cast<const uint32_t*>(zv);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {                                 // zero-points 4 i .. 4 i + 3 as bfloat16 128 + z
-            z[2 * i] = __byte_perm(zw[i], 0, 0x4140) | kMd128;
-            z[2 * i + 1] = __byte_perm(zw[i], 0, 0x4342) | kMd128;
-        }
+        md_commit();
     }
-    float zero[NT][4];
+    __device__ __forceinline__ void tile(int mt) const {
+        if (codes) {
+            md_cp16(fifo + (mt * 2) * MD_THREADS * 16, codes + static_cast<size_t>(mt * 16) * pitch);
+            md_cp16(fifo + (mt * 2 + 1) * MD_THREADS * 16, codes + static_cast<size_t>(mt * 16 + 8) * pitch);
+        }
+        md_commit();
+    }
+};
+
+template <int NT>
+__device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const MdEntries& e, const MdVItem& it, int cb, float* part, const MdVCopy& next) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    uint4 xv[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        zero[n][0] = zero[n][1] = zero[n][2] = zero[n][3] = 0.f;
+        const int r = n * 4 + (gid & 3);
+        const uint4* xp = reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(e.row[it.e][r < e.rows[it.e] ? r : 0]) * p.N + cb * 128 + tig * 32);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mma_bf16(zero[n], z[2 * i], z[2 * i], z[2 * i + 1], z[2 * i + 1], xs[n][2 * i], xs[n][2 * i + 1]);
+        for (int i = 0; i < 4; ++i) xv[n][i] = r < e.rows[it.e] ? ldg16(xp + i) : make_uint4(0u, 0u, 0u, 0u);
     }
+    md_wait<8>();                                                     // the scales and zero-points are there; the tiles may be under way
+    __syncwarp();
+    uint32_t z[8];                                                    // zero-points in the order of the codes' bytes
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint4 v = lds16(next.side + 256 + (tig * 2 + i) * 16);
+        z[i * 4] = __byte_perm(v.x, v.y, 0x5140);
+        z[i * 4 + 1] = __byte_perm(v.x, v.y, 0x7362);
+        z[i * 4 + 2] = __byte_perm(v.z, v.w, 0x5140);
+        z[i * 4 + 3] = __byte_perm(v.z, v.w, 0x7362);
+    }
+    // x vs of row gid % 4 at this lane's 32 columns: the largest of the row's 128, then the upper (gid < 4) or lower bytes of the fixed-point values
+    uint32_t xs[NT][8];
+    float weight[NT][2];                                              // what an integer counts in columns 2 tig and 2 tig + 1
+    int base[NT][4];                                                  // the float bits of an integer, less the zero-points' part
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 sv = lds16(next.side + (tig * 4 + i) * 16);
+            const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w}, xw[4] = {xv[n][i].x, xv[n][i].y, xv[n][i].z, xv[n][i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m = md_max(m, md_max(fabsf(md_lo(xw[k]) * md_lo(sw[k])), fabsf(md_hi(xw[k]) * md_hi(sw[k]))));
+        }
+        m = md_max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        m = md_max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+        const MdFixed fx = md_fixed(m);
+        const float add = gid < 4 ? kMdMagic + 128.f : kMdMagic;        // the upper byte is the one of v + 128
+        const uint32_t pick = gid < 4 ? 0x51u : 0x40u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 sv = lds16(next.side + (tig * 4 + i) * 16);
+            const uint32_t sw[4] = {sv.x, sv.y, sv.z, sv.w}, xw[4] = {xv[n][i].x, xv[n][i].y, xv[n][i].z, xv[n][i].w};
+            uint32_t q[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                q[2 * k] = __float_as_uint(fmaf(md_lo(xw[k]) * md_lo(sw[k]), fx.scale, add));
+                q[2 * k + 1] = __float_as_uint(fmaf(md_hi(xw[k]) * md_hi(sw[k]), fx.scale, add));
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                xs[n][i * 2 + k] = __byte_perm(__byte_perm(q[2 * k], q[2 * k + 4], pick), __byte_perm(q[2 * k + 1], q[2 * k + 5], pick), 0x5410);
+        }
+        // columns 0-3 are upper bytes
+        weight[n][0] = __shfl_sync(0xFFFFFFFFu, fx.unit, (2 * tig & 3) * 4) * (tig < 2 ? 256.f : 1.f);
+        weight[n][1] = __shfl_sync(0xFFFFFFFFu, fx.unit, (2 * tig + 1 & 3) * 4) * (tig < 2 ? 256.f : 1.f);
+        int zero[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) md_mma(zero, z[2 * i], z[2 * i], z[2 * i + 1], z[2 * i + 1], xs[n][2 * i], xs[n][2 * i + 1], zero);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) base[n][i] = kMdMagicBits - zero[i];
+    }
+    __syncwarp();                                                     // every lane has read the scales and zero-points
+    next.sides(lane);
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
-        md_wait<7>();
-        const uint4 r0 = lds16(fifo + (mt * 2) * MD_THREADS * 16), r1 = lds16(fifo + (mt * 2 + 1) * MD_THREADS * 16);
+        md_wait<8>();
+        const uint4 r0 = lds16(next.fifo + (mt * 2) * MD_THREADS * 16), r1 = lds16(next.fifo + (mt * 2 + 1) * MD_THREADS * 16);
         const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
-        float d[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+        int d[NT][4];
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const uint32_t a0 = md_pair(w0[w], 2 * q), a1 = md_pair(w1[w], 2 * q), a2 = md_pair(w0[w], 2 * q + 1), a3 = md_pair(w1[w], 2 * q + 1);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) mma_bf16(d[n], a0, a1, a2, a3, xs[n][w * 4 + 2 * q], xs[n][w * 4 + 2 * q + 1]);
-            }
-        if (more) {                                                   // the same tile of the next item into the pieces just used
-            md_cp16(fifo + (mt * 2) * MD_THREADS * 16, next + static_cast<size_t>(mt * 16) * (p.N / 2));
-            md_cp16(fifo + (mt * 2 + 1) * MD_THREADS * 16, next + static_cast<size_t>(mt * 16 + 8) * (p.N / 2));
-        }
-        md_commit();
+            for (int n = 0; n < NT; ++n) md_mma_word(d[n], w0[w], w1[w], xs[n][2 * w], xs[n][2 * w + 1], w == 0 ? base[n] : d[n]);
+        next.tile(mt);                                                // into the pieces just used
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float v = d[n][i] - zero[n][i];                        // rank gid + 8 (i / 2), column 2 tig + i % 2
+                // rank gid + 8 (i / 2), column 2 tig + i % 2; the weight is a power of two, so this is exact
+                float v = fmaf(__int_as_float(d[n][i]), weight[n][i & 1], -kMdMagic * weight[n][i & 1]);
                 v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
                 if (tig < 2) part[(n * 4 + tig * 2 + (i & 1)) * MD_PART + mt * 16 + gid + (i >> 1) * 8] = v;
             }
@@ -233,47 +299,53 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_v_kernel(const Mult
     __shared__ MdEntries e;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     float* part = reinterpret_cast<float*>(md_smem + 8 * 2 * MD_THREADS * 16);
-    const uint32_t fifo = smem_u32(md_smem) + tid * 16;
+    const uint32_t side = smem_u32(md_smem) + 8 * 2 * MD_THREADS * 16 + 8 * MD_ENTRY * MD_PART * 4 + warp * 384;
     md_entries(p, e);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int blocks = p.N / 128, items = (e.n ? e.groups_end[e.n - 1] : 0) * slices;
-    // this thread's first piece of an item's codes, or nullptr where the warp has no columns
-    auto codes = [&](const MdVItem& it) -> const uint8_t* {
+    int item = static_cast<int>(static_cast<long long>(items) * blockIdx.x / gridDim.x);
+    const int end = static_cast<int>(static_cast<long long>(items) * (blockIdx.x + 1) / gridDim.x);
+    if (item >= end) return;
+    auto copy = [&](const MdVItem& it, bool on) {
+        MdVCopy c = {nullptr, nullptr, smem_u32(md_smem) + tid * 16, side, static_cast<size_t>(p.N / 2), nullptr};
         const int cb = it.slice * (MD_COLS / 128) + warp;
-        if (cb >= blocks) return nullptr;
-        return p.vt + (static_cast<size_t>(e.first[it.e] + it.j) * 128 + gid) * (p.N / 2) + cb * 64 + tig * 16;
-    };
-    int item = blockIdx.x;
-    if (item >= items) return;
-    MdVItem it = md_v_item(e, item, slices);
-    const uint8_t* src = codes(it);
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-        if (src) {
-            md_cp16(fifo + (mt * 2) * MD_THREADS * 16, src + static_cast<size_t>(mt * 16) * (p.N / 2));
-            md_cp16(fifo + (mt * 2 + 1) * MD_THREADS * 16, src + static_cast<size_t>(mt * 16 + 8) * (p.N / 2));
+        if (on && cb < blocks) {
+            const size_t g = e.first[it.e] + it.j;
+            c.codes = p.vt + (g * 128 + gid) * c.pitch + cb * 64 + tig * 16;
+            c.scale = reinterpret_cast<const uint8_t*>(p.vs + g * p.N + cb * 128);
+            c.zero = p.vz + g * p.N + cb * 128;
         }
-        md_commit();
+        return c;
+    };
+    MdVItem it = md_v_item(e, item, slices);
+    {
+        const MdVCopy c = copy(it, true);
+        c.sides(lane);
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) c.tile(mt);
     }
     while (true) {
-        const int next_item = item + gridDim.x;
-        const bool go_on = next_item < items;
-        const MdVItem nx = go_on ? md_v_item(e, next_item, slices) : it;
-        const uint8_t* nsrc = go_on ? codes(nx) : nullptr;
-        const int cb = it.slice * (MD_COLS / 128) + warp, rows = e.rows[it.e];
-        if (src) {
-            float* mine = part + warp * (MD_ENTRY * MD_PART);
-            if (rows <= 4) md_v_compute<1>(p, e, it, cb, fifo, mine, nsrc != nullptr, nsrc);
-            else md_v_compute<2>(p, e, it, cb, fifo, mine, nsrc != nullptr, nsrc);
-        } else {
-#pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
-                if (nsrc) {
-                    md_cp16(fifo + (mt * 2) * MD_THREADS * 16, nsrc + static_cast<size_t>(mt * 16) * (p.N / 2));
-                    md_cp16(fifo + (mt * 2 + 1) * MD_THREADS * 16, nsrc + static_cast<size_t>(mt * 16 + 8) * (p.N / 2));
-                }
-                md_commit();
+        MdVItem nx = it;
+        if (++nx.j == e.ng[nx.e]) {
+            nx.j = 0;
+            if (++nx.slice == slices) {
+                nx.slice = 0;
+                do {
+                    ++nx.e;
+                } while (nx.e < e.n && e.ng[nx.e] == 0);
             }
+        }
+        const bool go_on = ++item < end;
+        const MdVCopy next = copy(nx, go_on);
+        const int cb = it.slice * (MD_COLS / 128) + warp, rows = e.rows[it.e];
+        if (cb < blocks) {
+            float* mine = part + warp * (MD_ENTRY * MD_PART);
+            if (rows <= 4) md_v_compute<1>(p, e, it, cb, mine, next);
+            else md_v_compute<2>(p, e, it, cb, mine, next);
+        } else {
+            next.sides(lane);
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) next.tile(mt);
         }
         __syncthreads();
         const int warps = min(8, blocks - it.slice * (MD_COLS / 128));
@@ -285,48 +357,58 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_v_kernel(const Mult
         }
         if (!go_on) return;
         __syncthreads();
-        item = next_item;
         it = nx;
-        src = nsrc;
     }
 }
 
 // ------------------------------------------------------------------ out = y + U h
-// An item is MD_UROWS rows of one entry's U: a warp multiplies 32 of them, in two tiles of 16, with the entry's columns of h, a rank group at a
-// step, and adds us (sum - (128 + uz) sum h) to its float32 results.
+// A tile is 32 rows of one entry's U: a warp multiplies them, as two tiles of 16, with the entry's columns of h, a rank group at a step,
+// and adds us (sum - uz sum h) to its float32 results.  `us`, `usz`: scale, and scale times zero-point, of row `lane` of the tile; `hsum`: for each
+// rank group and column what an integer counts, and the column's sum.
+template <int N>
+struct MdTiles {
+    static constexpr int value = N;
+};
+
 template <int NT>
-__device__ __forceinline__ void md_u_step(const uint4 (&c)[4], const uint8_t* hcol, const float* hsum, int j, const float (&us)[4], const float (&uz)[4],
-                                          float (&acc)[2][NT][4]) {
+__device__ __forceinline__ void md_u_step(const uint4 (&c)[4], const uint8_t* hcol, const float2* hsum, int j, float us, float usz, float (&acc)[2][NT][4]) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-    float d[2][NT][4];
+    int base[4] = {kMdMagicBits, kMdMagicBits, kMdMagicBits, kMdMagicBits};
+    int d[2][NT][4];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) d[m][n][0] = d[m][n][1] = d[m][n][2] = d[m][n][3] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int h = 0; h < 2; ++h) {                                       // words 2 h, 2 h + 1 of the four pieces
         uint4 b[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) b[n] = *reinterpret_cast<const uint4*>(hcol + (n * 8 + gid) * MD_HCOL + j * 256 + (w * 4 + tig) * 16);
+        for (int n = 0; n < NT; ++n) b[n] = *reinterpret_cast<const uint4*>(hcol + (n * 8 + gid) * MD_HCOL + j * 128 + (h * 4 + tig) * 16);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            const uint32_t w0 = reinterpret_cast<const uint32_t*>(&c[m * 2])[w], w1 = reinterpret_cast<const uint32_t*>(&c[m * 2 + 1])[w];
+            const uint4 &p0 = c[m * 2], &p1 = c[m * 2 + 1];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma_bf16(d[m][n], md_pair(w0, 0), md_pair(w1, 0), md_pair(w0, 1), md_pair(w1, 1), b[n].x, b[n].y);
-                mma_bf16(d[m][n], md_pair(w0, 2), md_pair(w1, 2), md_pair(w0, 3), md_pair(w1, 3), b[n].z, b[n].w);
+                md_mma_word(d[m][n], h ? p0.z : p0.x, h ? p1.z : p1.x, b[n].x, b[n].y, h ? d[m][n] : base);
+                md_mma_word(d[m][n], h ? p0.w : p0.y, h ? p1.w : p1.y, b[n].z, b[n].w, d[m][n]);
             }
         }
     }
+    float4 s[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const float2 s = *reinterpret_cast<const float2*>(hsum + j * 16 + n * 8 + tig * 2);
+    for (int n = 0; n < NT; ++n) s[n] = *reinterpret_cast<const float4*>(hsum + j * 16 + n * 8 + tig * 2);
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+    for (int i = 0; i < 4; ++i) {                                       // rows gid + 8 i of the tile
+        const float f = __shfl_sync(0xFFFFFFFFu, us, gid + 8 * i), z = __shfl_sync(0xFFFFFFFFu, usz, gid + 8 * i);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][n][i] += us[m * 2 + (i >> 1)] * (d[m][n][i] - uz[m * 2 + (i >> 1)] * (i & 1 ? s.y : s.x));
+        for (int n = 0; n < NT; ++n) {
+            float(&a)[4] = acc[i >> 1][n];
+            const int(&v)[4] = d[i >> 1][n];
+            a[(i & 1) * 2] += f * fmaf(__int_as_float(v[(i & 1) * 2]), s[n].x, -kMdMagic * s[n].x) - z * s[n].y;
+            a[(i & 1) * 2 + 1] += f * fmaf(__int_as_float(v[(i & 1) * 2 + 1]), s[n].z, -kMdMagic * s[n].z) - z * s[n].w;
+        }
     }
 }
+
+// Tiles go entry by entry, and a CTA has a run of them that costs about what the others' runs cost; h of an entry is brought into shared
+// memory once for the tiles of a run, which the warps take in turn.
+__device__ __forceinline__ int md_u_cost(const MdEntries& e, int i) { return e.ng[i] * (e.rows[i] <= 4 ? 5 : 6) + 2; }    // of a tile
 
 __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_u_kernel(const MultiDeltaParams p, int slices) {
     extern __shared__ __align__(16) uint8_t md_smem[];
@@ -334,107 +416,210 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_u_kernel(const Mult
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const uint32_t fifo = smem_u32(md_smem) + tid * 16;
     uint8_t* hcol = md_smem + MD_UDEPTH * 4 * MD_THREADS * 16;                   // [16 columns][MD_HCOL]
-    float* hsum = reinterpret_cast<float*>(hcol + 16 * MD_HCOL);                 // [MD_CHUNK][16 columns]
+    float2* hsum = reinterpret_cast<float2*>(hcol + 16 * MD_HCOL);               // [MD_MAX_GROUPS][16 columns]
+    float* stage = reinterpret_cast<float*>(hsum + MD_MAX_GROUPS * 16) + warp * (MD_ENTRY * MD_STAGE);      // [MD_ENTRY][MD_STAGE] results of the warp's tile
     md_entries(p, e);
-    const int chunks = (p.M + MD_UROWS - 1) / MD_UROWS, items = e.n * chunks;
-    // the stream of (item, rank group) steps, MD_UDEPTH - 1 ahead of the arithmetic
-    int a_item = blockIdx.x, a_j = 0;
-    auto settle = [&] {                                                          // items of entries without rank groups have no steps
-        while (a_item < items && a_j >= e.ng[a_item / chunks]) {
-            a_item += gridDim.x;
-            a_j = 0;
+    const int tiles = (p.M + 31) / 32;
+    // costs summed over the entries, by the first warp
+    int* sum = e.key;
+    if (warp == 0) {
+        int at = 0;
+        for (int b = 0; b < e.n; b += 32) {
+            int v = b + lane < e.n ? md_u_cost(e, b + lane) : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+                if (lane >= o) v += u;
+            }
+            v += at;
+            if (b + lane < e.n) sum[b + lane] = v;
+            at = __shfl_sync(0xFFFFFFFFu, v, 31);
+        }
+    }
+    __syncthreads();
+    struct Place {
+        int en, tile;
+    };
+    // first tile that begins at or behind `cost`
+    auto place = [&](long long cost) {
+        int lo = 0, hi = e.n;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (static_cast<long long>(sum[mid]) * tiles > cost) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo == e.n) return Place{lo, 0};
+        const int per = md_u_cost(e, lo);
+        const int tile = static_cast<int>((cost - static_cast<long long>(sum[lo] - per) * tiles + per - 1) / per);
+        return tile < tiles ? Place{lo, tile} : Place{lo + 1, 0};
+    };
+    const long long all = static_cast<long long>(sum[e.n - 1]) * tiles;
+    const Place first = place(all * blockIdx.x / gridDim.x), last = place(all * (blockIdx.x + 1) / gridDim.x);
+    auto tile_begin = [&](int en) { return en == first.en ? first.tile : 0; };
+    auto tile_end = [&](int en) { return en < last.en ? tiles : en == last.en ? last.tile : 0; };
+    // the warp's stream of codes, MD_UDEPTH - 1 steps ahead of the arithmetic
+    const size_t pitch = static_cast<size_t>(p.M) * 64;
+    Place ahead = {first.en, first.tile + warp};
+    int left = 0;                                                                // steps of the tile ahead
+    const uint8_t* src = nullptr;
+    auto aim = [&] {                                                             // at the warp's next tile with rank groups
+        while (ahead.en < e.n && (ahead.tile >= tile_end(ahead.en) || e.ng[ahead.en] == 0)) {
+            if (tile_end(ahead.en) < tiles) {                                    // the run ends here
+                ahead.en = e.n;
+                break;
+            }
+            ++ahead.en;
+            ahead.tile = warp;
+        }
+        if (ahead.en < e.n) {
+            left = e.ng[ahead.en];
+            src = p.uq + e.first[ahead.en] * pitch + static_cast<size_t>(ahead.tile * 32 + gid) * 64 + tig * 16;
         }
     };
     auto issue = [&](int slot) {
-        settle();
-        if (a_item < items) {
-            const int en = a_item / chunks, m = (a_item - en * chunks) * MD_UROWS + warp * 32 + gid;
-            const uint8_t* src = p.uq + (static_cast<size_t>(e.first[en] + a_j) * p.M + m) * 64 + tig * 16;
+        if (left) {
+            const int m = ahead.tile * 32 + gid;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (m + 8 * i < p.M) md_cp16(fifo + (slot * 4 + i) * MD_THREADS * 16, src + i * 8 * 64);
-            ++a_j;
+            src += pitch;
+            if (--left == 0) {
+                ahead.tile += MD_THREADS / 32;
+                aim();
+            }
         }
         md_commit();
     };
+    aim();
 #pragma unroll
     for (int s = 0; s < MD_UDEPTH - 1; ++s) issue(s);
     int slot = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    auto work = [&](int item, auto tiles) {
-        constexpr int NT = decltype(tiles)::value;                               // tiles of eight columns: two parts of four rows each
-        const int en = item / chunks, ng = e.ng[en], rows = e.rows[en], first = e.first[en];
-        const int m0 = (item - en * chunks) * MD_UROWS + warp * 32 + gid;          // rows m0 + 8 i of U, i = 0 .. 3
-        float acc[2][NT][4] = {};
-        for (int j0 = 0; j0 < ng; j0 += MD_CHUNK) {
-            const int jn = min(MD_CHUNK, ng - j0);
-            __syncthreads();                                                       // nobody reads the columns of h in place any more
-            // h of (row, rank group), one of them per warp and round, four ranks per lane: the slices' sums, as two bfloat16 parts in the
-            // order in which the products take them
-            for (int i = warp; i < rows * jn; i += MD_THREADS / 32) {
-                const int r = i / jn, j = i - r * jn;
-                const float* src = p.h + static_cast<size_t>(e.row[en][r]) * MD_H + (j0 + j) * 128 + lane * 4;
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    // the columns of h of an entry: one (row, rank group) per warp and round, four ranks per lane; the slices' sums in fixed point, bytes in the
+    // order of the codes' (0 4 1 5 and 2 6 3 7 of eight, which two lanes share)
+    auto bring = [&](int en, int ng) {
+        __syncthreads();                                                         // nobody reads the columns in place any more
+        for (int i = warp; i < e.rows[en] * ng; i += MD_THREADS / 32) {
+            const int r = i / ng, j = i - r * ng;
+            const float* from = p.h + static_cast<size_t>(e.row[en][r]) * MD_H + j * 128 + lane * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-                for (int s = 0; s < slices; ++s) {
-                    const float4 a = *reinterpret_cast<const float4*>(src + static_cast<size_t>(s) * p.T * MD_H);
-                    v.x += a.x;
-                    v.y += a.y;
-                    v.z += a.z;
-                    v.w += a.w;
-                }
-                const uint32_t h0 = md_pack(v.x, v.y), h1 = md_pack(v.z, v.w);
-                const uint32_t l0 = md_pack(v.x - md_lo(h0), v.y - md_hi(h0)), l1 = md_pack(v.z - md_lo(h1), v.w - md_hi(h1));
-                float sh = md_lo(h0) + md_hi(h0) + md_lo(h1) + md_hi(h1), sl = md_lo(l0) + md_hi(l0) + md_lo(l1) + md_hi(l1);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    sh += __shfl_xor_sync(0xFFFFFFFFu, sh, o);
-                    sl += __shfl_xor_sync(0xFFFFFFFFu, sl, o);
-                }
-                const int c = (r >> 2) * 8 + (r & 3);                              // column of the rounded part; the rest stands four behind it
-                uint8_t* to = hcol + c * MD_HCOL + j * 256 + ((lane >> 1 & 3) * 4 + (lane >> 3)) * 16 + (lane & 1) * 8;
-                *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
-                *reinterpret_cast<uint2*>(to + 4 * MD_HCOL) = make_uint2(l0, l1);
-                if (lane == 0) {
-                    hsum[j * 16 + c] = sh;
-                    hsum[j * 16 + c + 4] = sl;
-                }
+            for (int s = 0; s < slices; ++s) {
+                const float4 a = *reinterpret_cast<const float4*>(from + static_cast<size_t>(s) * p.T * MD_H);
+                v.x += a.x;
+                v.y += a.y;
+                v.z += a.z;
+                v.w += a.w;
             }
-            __syncthreads();
-            for (int j = 0; j < jn; ++j) {
-                float us[4], uz[4];
+            float m = md_max(md_max(fabsf(v.x), fabsf(v.y)), md_max(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const size_t at = static_cast<size_t>(first + j0 + j) * p.M + min(m0 + 8 * i, p.M - 1);
-                    us[i] = __bfloat162float(p.us[at]);
-                    uz[i] = 128.f + p.uz[at];
-                }
-                md_wait<MD_UDEPTH - 2>();
-                uint4 c[4];
+            for (int o = 16; o > 0; o >>= 1) m = md_max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            const MdFixed fx = md_fixed(m);
+            const float w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t q[4], q8[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) c[i] = lds16(fifo + (slot * 4 + i) * MD_THREADS * 16);
-                issue(slot == 0 ? MD_UDEPTH - 1 : slot - 1);
-                slot = slot + 1 == MD_UDEPTH ? 0 : slot + 1;
-                md_u_step<NT>(c, hcol, hsum, j, us, uz, acc);
+            for (int k = 0; k < 4; ++k) {
+                q[k] = __float_as_uint(fmaf(w[k], fx.scale, kMdMagic));
+                q8[k] = q[k] + 128u;                                             // the upper byte is the one of v + 128
+            }
+            const uint32_t up = __byte_perm(__byte_perm(q8[0], q8[1], 0x51), __byte_perm(q8[2], q8[3], 0x51), 0x5410);
+            const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x40), __byte_perm(q[2], q[3], 0x40), 0x5410);
+            const uint32_t up2 = __shfl_xor_sync(0xFFFFFFFFu, up, 1), lo2 = __shfl_xor_sync(0xFFFFFFFFu, lo, 1);
+            const int c = (r >> 2) * 8 + (r & 3);                                // column of the upper bytes; the lower stand four behind it
+            uint8_t* to = hcol + c * MD_HCOL + j * 128 + (lane >> 2 & 1) * 64 + (lane >> 3) * 16 + (lane >> 1 & 1) * 8 + (lane & 1) * 4;
+            *reinterpret_cast<uint32_t*>(to) = lane & 1 ? __byte_perm(up2, up, 0x7362) : __byte_perm(up, up2, 0x5140);
+            *reinterpret_cast<uint32_t*>(to + 4 * MD_HCOL) = lane & 1 ? __byte_perm(lo2, lo, 0x7362) : __byte_perm(lo, lo2, 0x5140);
+            const int su = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(up), 0x01010101, 0));
+            const int sl = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(lo), 0x01010101, 0));
+            if (lane == 0) {
+                hsum[j * 16 + c] = make_float2(fx.unit * 256.f, fx.unit * 256.f * su);
+                hsum[j * 16 + c + 4] = make_float2(fx.unit, fx.unit * sl);
             }
         }
-        // the two parts of a column are added; lane (gid, tig < 2) then has rows 2 tig, 2 tig + 1 of the entry at outputs m0 + 8 i
+        __syncthreads();
+    };
+    const bool vec = (p.M & 3) == 0;                                             // four outputs are an aligned piece of 8 bytes
+    auto work = [&](int en, int tile, auto nt) {
+        constexpr int NT = decltype(nt)::value;                                  // tiles of eight columns: two parts of four rows each
+        const int ng = e.ng[en], rows = e.rows[en], m0 = tile * 32;
+        // y of row n * 4 + lane / 8 at outputs m0 + lane % 8 * 4 + 0 .. 3, before anything is waited for
+        const int mo = m0 + (lane & 7) * 4;
+        uint2 y[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 4 + (lane >> 3);
+            y[n] = make_uint2(0u, 0u);
+            if (r < rows && mo < p.M) {
+                const __nv_bfloat16* yp = p.y + static_cast<size_t>(e.row[en][r]) * p.M + mo;
+                if (vec) {
+                    y[n] = *reinterpret_cast<const uint2*>(yp);
+                } else {
+                    uint32_t v[4] = {};
+                    for (int i = 0; i < 4; ++i)
+                        if (mo + i < p.M) v[i] = __bfloat16_as_ushort(yp[i]);
+                    y[n] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+                }
+            }
+        }
+        const size_t row = static_cast<size_t>(e.first[en]) * p.M + min(m0 + lane, p.M - 1);
+        const __nv_bfloat16* sp = p.us + row;
+        const uint8_t* zp = p.uz + row;
+        __nv_bfloat16 s_next = __nv_bfloat16();
+        uint8_t z_next = 0;
+        auto look = [&] {
+            s_next = *sp;
+            z_next = *zp;
+            sp += p.M;
+            zp += p.M;
+        };
+        if (ng) look();
+        float acc[2][NT][4] = {};
+        for (int j = 0; j < ng; ++j) {
+            const float us = __bfloat162float(s_next), usz = us * z_next;
+            if (j + 1 < ng) look();
+            md_wait<MD_UDEPTH - 2>();
+            uint4 c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = lds16(fifo + (slot * 4 + i) * MD_THREADS * 16);
+            issue(slot == 0 ? MD_UDEPTH - 1 : slot - 1);
+            slot = slot + 1 == MD_UDEPTH ? 0 : slot + 1;
+            md_u_step<NT>(c, hcol, hsum, j, us, usz, acc);
+        }
+        // the two parts of a column are added; lane (gid, tig < 2) then has rows 2 tig, 2 tig + 1 of the entry at outputs gid + 8 i, which go through shared
+        // memory into the order in which they are stored
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {                                           // tile i / 4, upper or lower rows, column
+            for (int i = 0; i < 8; ++i) {
                 float v = acc[i >> 2][n][i & 3];
                 v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-                const int r = n * 4 + tig * 2 + (i & 1), m = m0 + 8 * (i >> 1);
-                if (tig < 2 && r < rows && m < p.M) {
-                    const size_t at = static_cast<size_t>(e.row[en][r]) * p.M + m;
-                    p.out[at] = __float2bfloat16_rn(__bfloat162float(p.y[at]) + v);
+                if (tig < 2) stage[(n * 4 + tig * 2 + (i & 1)) * MD_STAGE + gid + 8 * (i >> 1)] = v;
+            }
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 4 + (lane >> 3);
+            const float4 v = *reinterpret_cast<const float4*>(stage + r * MD_STAGE + (lane & 7) * 4);
+            if (r < rows && mo < p.M) {
+                __nv_bfloat16* o = p.out + static_cast<size_t>(e.row[en][r]) * p.M + mo;
+                const uint2 w = make_uint2(md_pack(md_lo(y[n].x) + v.x, md_hi(y[n].x) + v.y), md_pack(md_lo(y[n].y) + v.z, md_hi(y[n].y) + v.w));
+                if (vec) {
+                    *reinterpret_cast<uint2*>(o) = w;
+                } else {
+                    const uint32_t b[4] = {w.x & 0xFFFFu, w.x >> 16, w.y & 0xFFFFu, w.y >> 16};
+                    for (int i = 0; i < 4; ++i)
+                        if (mo + i < p.M) o[i] = __ushort_as_bfloat16(static_cast<unsigned short>(b[i]));
                 }
             }
+        }
+        __syncwarp();
     };
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        if (e.rows[item / chunks] <= 4) work(item, MdTiles<1>{});
-        else work(item, MdTiles<2>{});
+    for (int en = first.en; en < e.n && tile_end(en) > 0; ++en) {
+        if (e.ng[en]) bring(en, e.ng[en]);
+        for (int t = tile_begin(en) + warp; t < tile_end(en); t += MD_THREADS / 32) {
+            if (e.rows[en] <= 4) work(en, t, MdTiles<1>{});
+            else work(en, t, MdTiles<2>{});
+        }
     }
 }
 
