@@ -13,7 +13,8 @@
 // cycle.  As bytes, eight codes take three of them (two ANDs and a shift) for the warp matrix instruction m16n8k32 of 8-bit
 // integers, which has twice the rate of m16n8k16; as bfloat16 pairs they take eleven (128 rows of 48 deltas, 11008 x 4096: 87 us then, half of that now).
 // So the codes are the instruction's 16 rows, and the token rows enter in fixed point: x vs over 128 columns, or h over the 128 ranks of a
-// group, scaled by a power of two to 16 bits, the upper eight in columns 0-3 (four rows of the entry), the lower eight in columns 4-7.  An operand
+// group, scaled by a power of two to 16 bits, the upper eight in an even column, the lower eight in the odd one beside it (so one thread has both
+// results of a token row, and four rows fill the eight columns).  An operand
 // is thus held to 2^-16 to 2^-15 of the largest of its 128; the products and their sums, zero-points included, are exact integers, and
 // what is added across groups, columns and warps is float32.
 // Every thread copies the 16-byte pieces of codes that it will use itself with cp.async into a queue of its own, so the
@@ -35,8 +36,10 @@ constexpr int MD_COLS = 1024;                     // columns of V^T that one ite
 constexpr int MD_H = MD_MAX_GROUPS * 128;         // floats of h kept per row and slice of columns
 constexpr int MD_PART = 132;                      // row pitch of the warps' partial h, in floats
 constexpr int MD_HCOL = MD_MAX_GROUPS * 128 + 64; // bytes of a column of h in shared memory; 64 over a multiple of 128: no bank conflicts
-constexpr int MD_STAGE = 36;                      // row pitch of a warp's results, in floats
-constexpr int MD_UDEPTH = 4;                      // steps in the queue of the second launch
+constexpr int MD_TILE = 64;                       // rows of U that a warp takes at a time
+constexpr int MD_UDEPTH = 2;                      // steps in the queue of the second launch
+constexpr int MD_STAGE = 36;                      // row pitch of half a tile's results, in floats
+constexpr int MD_SIDE = 224;                      // bytes of a step's scales (nine pieces) and zero-points (five)
 constexpr float kMdMagic = 12582912.f;            // 1.5 * 2^23: an integer below 2^22 added to its bits is added to its value
 constexpr int kMdMagicBits = 0x4B400000;
 
@@ -53,19 +56,28 @@ struct MultiDeltaParams {
 // Rows that share a delta, in entries of up to MD_ENTRY rows.
 struct MdEntries {
     int n;
-    int first[MD_MAX_ROWS], ng[MD_MAX_ROWS], rows[MD_MAX_ROWS];   // first rank group, their number, rows of the entry
-    int groups_end[MD_MAX_ROWS];                                  // rank groups of this entry and those before it
-    uint8_t row[MD_MAX_ROWS][MD_ENTRY];
     alignas(16) int key[MD_MAX_ROWS];
-    int base[MD_MAX_ROWS], wsum[8];
+    int first[MD_MAX_ROWS];                                       // first rank group
+    int groups_end[MD_MAX_ROWS];                                  // rank groups of this entry and those before it
+    int cost_end[MD_MAX_ROWS];                                    // md_u_cost, summed the same way
+    uint8_t ng[MD_MAX_ROWS], rows[MD_MAX_ROWS];                   // rank groups and rows of the entry
+    uint8_t row[MD_MAX_ROWS][MD_ENTRY], base[MD_MAX_ROWS];
+    int wsum[8], wcost[8];
 };
 
+// What a tile of the second launch costs with an entry of so many rank groups and rows, in about 25 cycles of a warp.
+__device__ __forceinline__ int md_u_cost(int ng, int rows) { return ng == 0 ? 10 : rows <= 4 ? ng * 8 + 7 : ng * 11 + 6; }
+
 constexpr size_t md_v_smem() { return 8 * 2 * MD_THREADS * 16 + 8 * MD_ENTRY * MD_PART * sizeof(float) + 8 * 384; }
-constexpr size_t md_u_smem() { return MD_UDEPTH * 4 * MD_THREADS * 16 + 16 * MD_HCOL + MD_MAX_GROUPS * 16 * sizeof(float2) + 8 * MD_ENTRY * MD_STAGE * sizeof(float); }
+constexpr size_t md_u_smem() { return MD_UDEPTH * 8 * MD_THREADS * 16 + 16 * MD_HCOL + MD_MAX_GROUPS * MD_ENTRY * sizeof(float2) + 8 * (4 * MD_STAGE * sizeof(float) + MD_UDEPTH * MD_SIDE); }
 inline int md_slices(int N) { return (N + MD_COLS - 1) / MD_COLS; }
 
 __device__ __forceinline__ void md_cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// the first `bytes` of 16, zeros behind them
+__device__ __forceinline__ void md_cp16_part(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void md_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -80,7 +92,7 @@ __device__ __forceinline__ uint32_t md_pack(float a, float b) {
 }
 // D(16x8, s32) = A(16x32, u8, row) * B(32x8, s8, col) + C
 __device__ __forceinline__ void md_mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const int (&c)[4]) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
@@ -92,6 +104,11 @@ __device__ __forceinline__ float md_max(float a, float b) {              // NaN 
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
+}
+// What the integers of upper and lower bytes, given as the bits of kMdMagic plus each, come to; `unit` is a power of two, so only the sum is rounded.
+__device__ __forceinline__ float md_join(int up, int lo, float unit) {
+    const float u = unit * 256.f;
+    return fmaf(__int_as_float(up), u, -kMdMagic * u) + fmaf(__int_as_float(lo), unit, -kMdMagic * unit);
 }
 // Fixed point for values of magnitude up to m: v * scale is at most 32637, so its upper and lower eight bits are signed bytes; `unit` = 1 / scale, a
 // power of two (infinite or NaN where m is, so that results show it).
@@ -105,17 +122,17 @@ __device__ __forceinline__ MdFixed md_fixed(float m) {
 
 __device__ __forceinline__ void md_entries(const MultiDeltaParams& p, MdEntries& e) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    // the table of first rank groups is fetched beside the ids where it is short enough to keep (cost_end is free until the end)
+    const bool kept = p.deltas < MD_MAX_ROWS;
+    if (kept && t <= p.deltas) e.cost_end[t] = p.start[t];
+    const int d = t < p.T ? p.ids[t] : -1;
+    if (kept) __syncthreads();
     int first = 0, ng = 0;
-    if (t < p.T) {
-        const int d = p.ids[t];
-        if (d >= 0 && d < p.deltas) {
-            first = max(p.start[d], 0);
-            ng = max(0, min(min(p.start[d + 1], p.G) - first, MD_MAX_GROUPS));
-        }
-        e.key[t] = ng ? d : -1;                             // rows without a delta share an entry of no groups
-    } else if (t < MD_MAX_ROWS) {
-        e.key[t] = -2;
+    if (d >= 0 && d < p.deltas) {
+        first = max(kept ? e.cost_end[d] : p.start[d], 0);
+        ng = max(0, min(min(kept ? e.cost_end[d + 1] : p.start[d + 1], p.G) - first, MD_MAX_GROUPS));
     }
+    if (t < MD_MAX_ROWS) e.key[t] = t >= p.T ? -2 : ng ? d : -1;     // rows without a delta share an entry of no groups
     __syncthreads();
     int before = 0, same = 0, leader = t;
     if (t < p.T) {
@@ -133,34 +150,51 @@ __device__ __forceinline__ void md_entries(const MultiDeltaParams& p, MdEntries&
                 }
         }
     }
-    // entries and rank groups of each group of rows, at its first row, summed over the rows
+    // entries, rank groups and cost of each group of rows, at its first row, summed over the rows
     const int mine = t < p.T && leader == t ? (same + MD_ENTRY - 1) / MD_ENTRY : 0;
-    int run = mine << 16 | mine * ng;                       // at most 128 entries, 128 * 16 rank groups
+    const int full = md_u_cost(ng, MD_ENTRY), my_cost = mine ? (mine - 1) * full + md_u_cost(ng, same - (mine - 1) * MD_ENTRY) : 0;
+    int run = mine << 16 | mine * ng, cost = my_cost;       // at most 128 entries, 128 * 16 rank groups
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xFFFFFFFFu, run, o);
-        if (lane >= o) run += u;
+        const int u = __shfl_up_sync(0xFFFFFFFFu, run, o), v = __shfl_up_sync(0xFFFFFFFFu, cost, o);
+        if (lane >= o) {
+            run += u;
+            cost += v;
+        }
     }
-    if (lane == 31) e.wsum[warp] = run;
+    if (lane == 31) {
+        e.wsum[warp] = run;
+        e.wcost[warp] = cost;
+    }
     __syncthreads();
     run -= mine << 16 | mine * ng;
-    for (int w = 0; w < warp; ++w) run += e.wsum[w];
-    if (t < p.T) e.base[t] = run;
-    if (t == 0) {
-        int all = 0;
-        for (int w = 0; w < MD_MAX_ROWS / 32; ++w) all += e.wsum[w];
-        e.n = all >> 16;
-    }
+    cost -= my_cost;
+#pragma unroll
+    for (int w = 0; w < MD_MAX_ROWS / 32; ++w)
+        if (w < warp) {
+            run += e.wsum[w];
+            cost += e.wcost[w];
+        }
+    if (t < p.T) e.base[t] = static_cast<uint8_t>(run >> 16);
+    if (t == MD_MAX_ROWS) e.n = run >> 16;
     for (int k = 0; k < mine; ++k) {
-        const int i = (run >> 16) + k;
+        const int i = (run >> 16) + k, rows = min(MD_ENTRY, same - k * MD_ENTRY);
+        cost += md_u_cost(ng, rows);
         e.first[i] = first;
-        e.ng[i] = ng;
-        e.rows[i] = min(MD_ENTRY, same - k * MD_ENTRY);
+        e.ng[i] = static_cast<uint8_t>(ng);
+        e.rows[i] = static_cast<uint8_t>(rows);
         e.groups_end[i] = (run & 0xFFFF) + (k + 1) * ng;
+        e.cost_end[i] = cost;
     }
     __syncthreads();
-    if (t < p.T) e.row[(e.base[leader] >> 16) + before / MD_ENTRY][before % MD_ENTRY] = static_cast<uint8_t>(t);
+    if (t < p.T) e.row[e.base[leader] + before / MD_ENTRY][before % MD_ENTRY] = static_cast<uint8_t>(t);
     __syncthreads();
+}
+
+// where the share of block b of n things begins
+__device__ __forceinline__ int md_share(int n, int b) {
+    const int each = n / static_cast<int>(gridDim.x), more = n - each * static_cast<int>(gridDim.x);
+    return each * b + min(b, more);
 }
 
 // ------------------------------------------------------------------ h = V^T x
@@ -211,7 +245,7 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
     uint4 xv[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = n * 4 + (gid & 3);
+        const int r = n * 4 + (gid >> 1);
         const uint4* xp = reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(e.row[it.e][r < e.rows[it.e] ? r : 0]) * p.N + cb * 128 + tig * 32);
 #pragma unroll
         for (int i = 0; i < 4; ++i) xv[n][i] = r < e.rows[it.e] ? ldg16(xp + i) : make_uint4(0u, 0u, 0u, 0u);
@@ -227,9 +261,9 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
         z[i * 4 + 2] = __byte_perm(v.z, v.w, 0x5140);
         z[i * 4 + 3] = __byte_perm(v.z, v.w, 0x7362);
     }
-    // x vs of row gid % 4 at this lane's 32 columns: the largest of the row's 128, then the upper (gid < 4) or lower bytes of the fixed-point values
+    // x vs of row gid / 2 at this lane's 32 columns: the largest of the row's 128, then the upper (gid even) or lower bytes of the fixed-point values
     uint32_t xs[NT][8];
-    float weight[NT][2];                                              // what an integer counts in columns 2 tig and 2 tig + 1
+    float weight[NT];                                                 // what an integer of lower bytes counts for row tig
     int base[NT][4];                                                  // the float bits of an integer, less the zero-points' part
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -244,8 +278,8 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
         m = md_max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
         m = md_max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
         const MdFixed fx = md_fixed(m);
-        const float add = gid < 4 ? kMdMagic + 128.f : kMdMagic;        // the upper byte is the one of v + 128
-        const uint32_t pick = gid < 4 ? 0x51u : 0x40u;
+        const float add = gid & 1 ? kMdMagic : kMdMagic + 128.f;        // the upper byte is the one of v + 128
+        const uint32_t pick = gid & 1 ? 0x40u : 0x51u;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint4 sv = lds16(next.side + (tig * 4 + i) * 16);
@@ -260,9 +294,7 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
             for (int k = 0; k < 2; ++k)
                 xs[n][i * 2 + k] = __byte_perm(__byte_perm(q[2 * k], q[2 * k + 4], pick), __byte_perm(q[2 * k + 1], q[2 * k + 5], pick), 0x5410);
         }
-        // columns 0-3 are upper bytes
-        weight[n][0] = __shfl_sync(0xFFFFFFFFu, fx.unit, (2 * tig & 3) * 4) * (tig < 2 ? 256.f : 1.f);
-        weight[n][1] = __shfl_sync(0xFFFFFFFFu, fx.unit, (2 * tig + 1 & 3) * 4) * (tig < 2 ? 256.f : 1.f);
+        weight[n] = __shfl_sync(0xFFFFFFFFu, fx.unit, tig * 8);
         int zero[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i) md_mma(zero, z[2 * i], z[2 * i], z[2 * i + 1], z[2 * i + 1], xs[n][2 * i], xs[n][2 * i + 1], zero);
@@ -285,12 +317,7 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // rank gid + 8 (i / 2), column 2 tig + i % 2; the weight is a power of two, so this is exact
-                float v = fmaf(__int_as_float(d[n][i]), weight[n][i & 1], -kMdMagic * weight[n][i & 1]);
-                v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-                if (tig < 2) part[(n * 4 + tig * 2 + (i & 1)) * MD_PART + mt * 16 + gid + (i >> 1) * 8] = v;
-            }
+            for (int i = 0; i < 2; ++i) part[(n * 4 + tig) * MD_PART + mt * 16 + gid + i * 8] = md_join(d[n][2 * i], d[n][2 * i + 1], weight[n]);
     }
 }
 
@@ -303,8 +330,8 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_v_kernel(const Mult
     md_entries(p, e);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int blocks = p.N / 128, items = (e.n ? e.groups_end[e.n - 1] : 0) * slices;
-    int item = static_cast<int>(static_cast<long long>(items) * blockIdx.x / gridDim.x);
-    const int end = static_cast<int>(static_cast<long long>(items) * (blockIdx.x + 1) / gridDim.x);
+    int item = md_share(items, blockIdx.x);
+    const int end = md_share(items, blockIdx.x + 1);
     if (item >= end) return;
     auto copy = [&](const MdVItem& it, bool on) {
         MdVCopy c = {nullptr, nullptr, smem_u32(md_smem) + tid * 16, side, static_cast<size_t>(p.N / 2), nullptr};
@@ -362,127 +389,131 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_v_kernel(const Mult
 }
 
 // ------------------------------------------------------------------ out = y + U h
-// A tile is 32 rows of one entry's U: a warp multiplies them, as two tiles of 16, with the entry's columns of h, a rank group at a step,
-// and adds us (sum - uz sum h) to its float32 results.  `us`, `usz`: scale, and scale times zero-point, of row `lane` of the tile; `hsum`: for each
-// rank group and column what an integer counts, and the column's sum.
+// A tile is MD_TILE rows of one entry's U: a warp multiplies them, 16 at a time, with the entry's columns of h, a rank group at a step,
+// and adds us (sum - uz sum h) to its float32 results.  `us`, `usz`: scale, and scale times zero-point, of rows `lane` and lane + 32 of
+// the tile; `hsum`: for each rank group and row of the entry what an integer of lower bytes counts, and the sum of h.
 template <int N>
 struct MdTiles {
     static constexpr int value = N;
 };
 
-template <int NT>
-__device__ __forceinline__ void md_u_step(const uint4 (&c)[4], const uint8_t* hcol, const float2* hsum, int j, float us, float usz, float (&acc)[2][NT][4]) {
+template <int NT, typename Refill>
+__device__ __forceinline__ void md_u_step(uint32_t codes, const uint8_t* hcol, const float2* hsum, int j, const float (&us)[2], const float (&usz)[2],
+                                          float (&acc)[NT][8], Refill refill) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     int base[4] = {kMdMagicBits, kMdMagicBits, kMdMagicBits, kMdMagicBits};
-    int d[2][NT][4];
+    uint4 b[NT][2];
+    float2 s[NT];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {                                       // words 2 h, 2 h + 1 of the four pieces
-        uint4 b[NT];
+    for (int n = 0; n < NT; ++n) {
+        s[n] = hsum[j * 8 + n * 4 + tig];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) b[n] = *reinterpret_cast<const uint4*>(hcol + (n * 8 + gid) * MD_HCOL + j * 128 + (h * 4 + tig) * 16);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const uint4 &p0 = c[m * 2], &p1 = c[m * 2 + 1];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                md_mma_word(d[m][n], h ? p0.z : p0.x, h ? p1.z : p1.x, b[n].x, b[n].y, h ? d[m][n] : base);
-                md_mma_word(d[m][n], h ? p0.w : p0.y, h ? p1.w : p1.y, b[n].z, b[n].w, d[m][n]);
-            }
-        }
+        for (int h = 0; h < 2; ++h) b[n][h] = *reinterpret_cast<const uint4*>(hcol + (n * 8 + gid) * MD_HCOL + j * 128 + (h * 4 + tig) * 16);
     }
-    float4 s[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n] = *reinterpret_cast<const float4*>(hsum + j * 16 + n * 8 + tig * 2);
+    for (int m = 0; m < 4; ++m) {
+        const uint4 p0 = lds16(codes + (m * 2) * MD_THREADS * 16), p1 = lds16(codes + (m * 2 + 1) * MD_THREADS * 16);
+        int d[NT][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {                                       // rows gid + 8 i of the tile
-        const float f = __shfl_sync(0xFFFFFFFFu, us, gid + 8 * i), z = __shfl_sync(0xFFFFFFFFu, usz, gid + 8 * i);
+        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.x, p1.x, b[n][0].x, b[n][0].y, base);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float(&a)[4] = acc[i >> 1][n];
-            const int(&v)[4] = d[i >> 1][n];
-            a[(i & 1) * 2] += f * fmaf(__int_as_float(v[(i & 1) * 2]), s[n].x, -kMdMagic * s[n].x) - z * s[n].y;
-            a[(i & 1) * 2 + 1] += f * fmaf(__int_as_float(v[(i & 1) * 2 + 1]), s[n].z, -kMdMagic * s[n].z) - z * s[n].w;
+        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.y, p1.y, b[n][0].z, b[n][0].w, d[n]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.z, p1.z, b[n][1].x, b[n][1].y, d[n]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.w, p1.w, b[n][1].z, b[n][1].w, d[n]);
+        refill(m);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                                   // rows gid + 8 (2 m + i) of the tile
+            const int from = gid + 8 * (m * 2 + i & 3);
+            const float f = __shfl_sync(0xFFFFFFFFu, us[m >> 1], from), z = __shfl_sync(0xFFFFFFFFu, usz[m >> 1], from);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][m * 2 + i] += f * md_join(d[n][i * 2], d[n][i * 2 + 1], s[n].x) - z * s[n].y;
         }
     }
 }
 
 // Tiles go entry by entry, and a CTA has a run of them that costs about what the others' runs cost; h of an entry is brought into shared
 // memory once for the tiles of a run, which the warps take in turn.
-__device__ __forceinline__ int md_u_cost(const MdEntries& e, int i) { return e.ng[i] * (e.rows[i] <= 4 ? 5 : 6) + 2; }    // of a tile
-
 __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_u_kernel(const MultiDeltaParams p, int slices) {
     extern __shared__ __align__(16) uint8_t md_smem[];
     __shared__ MdEntries e;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const uint32_t fifo = smem_u32(md_smem) + tid * 16;
-    uint8_t* hcol = md_smem + MD_UDEPTH * 4 * MD_THREADS * 16;                   // [16 columns][MD_HCOL]
-    float2* hsum = reinterpret_cast<float2*>(hcol + 16 * MD_HCOL);               // [MD_MAX_GROUPS][16 columns]
-    float* stage = reinterpret_cast<float*>(hsum + MD_MAX_GROUPS * 16) + warp * (MD_ENTRY * MD_STAGE);      // [MD_ENTRY][MD_STAGE] results of the warp's tile
+    uint8_t* hcol = md_smem + MD_UDEPTH * 8 * MD_THREADS * 16;                   // [16 columns][MD_HCOL]
+    float2* hsum = reinterpret_cast<float2*>(hcol + 16 * MD_HCOL);               // [MD_MAX_GROUPS][MD_ENTRY]
+    uint8_t* own = reinterpret_cast<uint8_t*>(hsum + MD_MAX_GROUPS * MD_ENTRY) + warp * (4 * MD_STAGE * sizeof(float) + MD_UDEPTH * MD_SIDE);
+    float* stage = reinterpret_cast<float*>(own);                                // [4][MD_STAGE] results of the warp's tile, four rows and 32 outputs at a time
+    const uint8_t* side = own + 4 * MD_STAGE * sizeof(float);                    // scales and zero-points of the steps in the queue
+    // Of a step's scales (and zero-points) the aligned pieces of 16 bytes that hold them are copied, nine and five, a piece per lane.
+    const bool is_scale = lane < 9;
+    const uint8_t* side_base = is_scale ? reinterpret_cast<const uint8_t*>(p.us) : p.uz;
+    const int side_log = is_scale ? 1 : 0, side_piece = is_scale ? lane : lane - 9;
+    const size_t side_size = (static_cast<size_t>(p.G) * p.M) << side_log;
     md_entries(p, e);
-    const int tiles = (p.M + 31) / 32;
-    // costs summed over the entries, by the first warp
-    int* sum = e.key;
-    if (warp == 0) {
-        int at = 0;
-        for (int b = 0; b < e.n; b += 32) {
-            int v = b + lane < e.n ? md_u_cost(e, b + lane) : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
-                if (lane >= o) v += u;
-            }
-            v += at;
-            if (b + lane < e.n) sum[b + lane] = v;
-            at = __shfl_sync(0xFFFFFFFFu, v, 31);
-        }
-    }
-    __syncthreads();
+    const int tiles = (p.M + MD_TILE - 1) / MD_TILE;
     struct Place {
         int en, tile;
     };
     // first tile that begins at or behind `cost`
-    auto place = [&](long long cost) {
+    auto place = [&](int cost) {
         int lo = 0, hi = e.n;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (static_cast<long long>(sum[mid]) * tiles > cost) hi = mid;
+            if (e.cost_end[mid] * tiles > cost) hi = mid;
             else lo = mid + 1;
         }
         if (lo == e.n) return Place{lo, 0};
-        const int per = md_u_cost(e, lo);
-        const int tile = static_cast<int>((cost - static_cast<long long>(sum[lo] - per) * tiles + per - 1) / per);
+        const int before = lo ? e.cost_end[lo - 1] : 0, per = e.cost_end[lo] - before, tile = (cost - before * tiles + per - 1) / per;
         return tile < tiles ? Place{lo, tile} : Place{lo + 1, 0};
     };
-    const long long all = static_cast<long long>(sum[e.n - 1]) * tiles;
-    const Place first = place(all * blockIdx.x / gridDim.x), last = place(all * (blockIdx.x + 1) / gridDim.x);
-    auto tile_begin = [&](int en) { return en == first.en ? first.tile : 0; };
+    const int all = e.cost_end[e.n - 1] * tiles;
+    const Place first = place(md_share(all, blockIdx.x)), last = place(md_share(all, blockIdx.x + 1));
+    if (first.en == last.en && first.tile == last.tile) return;
     auto tile_end = [&](int en) { return en < last.en ? tiles : en == last.en ? last.tile : 0; };
-    // the warp's stream of codes, MD_UDEPTH - 1 steps ahead of the arithmetic
+    // the warp's stream of codes: 16 rows of a step make room for 16 rows of the step MD_UDEPTH behind it as soon as they have been used
     const size_t pitch = static_cast<size_t>(p.M) * 64;
+    // The warps take the tiles of the run in turn.  Entries without rank groups have tiles too (y alone), but no steps.
+    auto settle = [&](Place& at) {                                               // from a place that may lie behind its entry's tiles
+        while (at.en < e.n && at.tile >= tile_end(at.en)) {
+            if (at.en >= last.en) at.en = e.n;                                   // the run ends here
+            else at.tile -= tile_end(at.en++);
+        }
+    };
     Place ahead = {first.en, first.tile + warp};
     int left = 0;                                                                // steps of the tile ahead
     const uint8_t* src = nullptr;
+    uint32_t side_at = 0;                                                        // place of the tile's first scale (the codes of 2^32 rows would not fit a device)
+    const uint32_t side_dst = smem_u32(side) + lane * 16;
     auto aim = [&] {                                                             // at the warp's next tile with rank groups
-        while (ahead.en < e.n && (ahead.tile >= tile_end(ahead.en) || e.ng[ahead.en] == 0)) {
-            if (tile_end(ahead.en) < tiles) {                                    // the run ends here
-                ahead.en = e.n;
-                break;
-            }
-            ++ahead.en;
-            ahead.tile = warp;
+        settle(ahead);
+        while (ahead.en < e.n && e.ng[ahead.en] == 0) {
+            ahead.tile += MD_THREADS / 32;
+            settle(ahead);
         }
         if (ahead.en < e.n) {
             left = e.ng[ahead.en];
-            src = p.uq + e.first[ahead.en] * pitch + static_cast<size_t>(ahead.tile * 32 + gid) * 64 + tig * 16;
+            src = p.uq + e.first[ahead.en] * pitch + static_cast<size_t>(ahead.tile * MD_TILE + gid) * 64 + tig * 16;
+            side_at = static_cast<uint32_t>(e.first[ahead.en]) * p.M + ahead.tile * MD_TILE;
         }
     };
-    auto issue = [&](int slot) {
+    // rows 16 m .. 16 m + 15 of the step ahead
+    auto piece = [&](int slot, int m) {
+        if (!left) return;
+        const uint32_t dst = fifo + slot * (8 * MD_THREADS * 16) + m * (2 * MD_THREADS * 16);
+        const int row = ahead.tile * MD_TILE + gid + 16 * m;
+        if (row < p.M) md_cp16(dst, src + m * 16 * 64);
+        if (row + 8 < p.M) md_cp16(dst + MD_THREADS * 16, src + m * 16 * 64 + 8 * 64);
+    };
+    auto rest = [&](int slot) {                                                  // its scales and zero-points; on to the next
         if (left) {
-            const int m = ahead.tile * 32 + gid;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (m + 8 * i < p.M) md_cp16(fifo + (slot * 4 + i) * MD_THREADS * 16, src + i * 8 * 64);
+            if (lane < 14) {
+                const size_t from = (static_cast<size_t>(side_at) << side_log & ~static_cast<size_t>(15)) + side_piece * 16;
+                if (from + 16 <= side_size) md_cp16(side_dst + slot * MD_SIDE, side_base + from);
+                else if (from < side_size) md_cp16_part(side_dst + slot * MD_SIDE, side_base + from, static_cast<int>(side_size - from));
+            }
             src += pitch;
+            side_at += p.M;
             if (--left == 0) {
                 ahead.tile += MD_THREADS / 32;
                 aim();
@@ -492,16 +523,20 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_u_kernel(const Mult
     };
     aim();
 #pragma unroll
-    for (int s = 0; s < MD_UDEPTH - 1; ++s) issue(s);
+    for (int s = 0; s < MD_UDEPTH; ++s) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) piece(s, m);
+        rest(s);
+    }
     int slot = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // the columns of h of an entry: one (row, rank group) per warp and round, four ranks per lane; the slices' sums in fixed point, bytes in the
-    // order of the codes' (0 4 1 5 and 2 6 3 7 of eight, which two lanes share)
-    auto bring = [&](int en, int ng) {
-        __syncthreads();                                                         // nobody reads the columns in place any more
+    // the columns of h of some entries, from rank group `at` in shared memory on: one (row, rank group) per warp and round, four ranks per lane; the
+    // slices' sums in fixed point, bytes in the order of the codes' (0 4 1 5 and 2 6 3 7 of eight, which two lanes share)
+    auto bring = [&](int en, int at) {
+        const int ng = e.ng[en];
         for (int i = warp; i < e.rows[en] * ng; i += MD_THREADS / 32) {
-            const int r = i / ng, j = i - r * ng;
-            const float* from = p.h + static_cast<size_t>(e.row[en][r]) * MD_H + j * 128 + lane * 4;
+            const int r = i / ng, jr = i - r * ng, j = at + jr;
+            const float* from = p.h + static_cast<size_t>(e.row[en][r]) * MD_H + jr * 128 + lane * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
             for (int s = 0; s < slices; ++s) {
@@ -525,101 +560,99 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_u_kernel(const Mult
             const uint32_t up = __byte_perm(__byte_perm(q8[0], q8[1], 0x51), __byte_perm(q8[2], q8[3], 0x51), 0x5410);
             const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x40), __byte_perm(q[2], q[3], 0x40), 0x5410);
             const uint32_t up2 = __shfl_xor_sync(0xFFFFFFFFu, up, 1), lo2 = __shfl_xor_sync(0xFFFFFFFFu, lo, 1);
-            const int c = (r >> 2) * 8 + (r & 3);                                // column of the upper bytes; the lower stand four behind it
+            const int c = r * 2;                                                 // column of the upper bytes; the lower stand behind it
             uint8_t* to = hcol + c * MD_HCOL + j * 128 + (lane >> 2 & 1) * 64 + (lane >> 3) * 16 + (lane >> 1 & 1) * 8 + (lane & 1) * 4;
             *reinterpret_cast<uint32_t*>(to) = lane & 1 ? __byte_perm(up2, up, 0x7362) : __byte_perm(up, up2, 0x5140);
-            *reinterpret_cast<uint32_t*>(to + 4 * MD_HCOL) = lane & 1 ? __byte_perm(lo2, lo, 0x7362) : __byte_perm(lo, lo2, 0x5140);
+            *reinterpret_cast<uint32_t*>(to + MD_HCOL) = lane & 1 ? __byte_perm(lo2, lo, 0x7362) : __byte_perm(lo, lo2, 0x5140);
             const int su = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(up), 0x01010101, 0));
             const int sl = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(lo), 0x01010101, 0));
-            if (lane == 0) {
-                hsum[j * 16 + c] = make_float2(fx.unit * 256.f, fx.unit * 256.f * su);
-                hsum[j * 16 + c + 4] = make_float2(fx.unit, fx.unit * sl);
-            }
+            if (lane == 0) hsum[j * 8 + r] = make_float2(fx.unit, fx.unit * (256.f * su + sl));
         }
-        __syncthreads();
     };
     const bool vec = (p.M & 3) == 0;                                             // four outputs are an aligned piece of 8 bytes
-    auto work = [&](int en, int tile, auto nt) {
+    auto work = [&](int en, int tile, int h_at, auto nt) {
         constexpr int NT = decltype(nt)::value;                                  // tiles of eight columns: two parts of four rows each
-        const int ng = e.ng[en], rows = e.rows[en], m0 = tile * 32;
-        // y of row n * 4 + lane / 8 at outputs m0 + lane % 8 * 4 + 0 .. 3, before anything is waited for
+        const int ng = e.ng[en], rows = e.rows[en], m0 = tile * MD_TILE;
+        // y of row n * 4 + lane / 8 at outputs m0 + 32 k + lane % 8 * 4 + 0 .. 3, before anything is waited for
         const int mo = m0 + (lane & 7) * 4;
-        uint2 y[NT];
+        uint2 y[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = n * 4 + (lane >> 3);
-            y[n] = make_uint2(0u, 0u);
-            if (r < rows && mo < p.M) {
-                const __nv_bfloat16* yp = p.y + static_cast<size_t>(e.row[en][r]) * p.M + mo;
-                if (vec) {
-                    y[n] = *reinterpret_cast<const uint2*>(yp);
-                } else {
-                    uint32_t v[4] = {};
-                    for (int i = 0; i < 4; ++i)
-                        if (mo + i < p.M) v[i] = __bfloat16_as_ushort(yp[i]);
-                    y[n] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+            const __nv_bfloat16* yp = p.y + static_cast<size_t>(e.row[en][r < rows ? r : 0]) * p.M + mo;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                y[n][k] = make_uint2(0u, 0u);
+                if (r < rows && mo + 32 * k < p.M) {
+                    if (vec) {
+                        y[n][k] = *reinterpret_cast<const uint2*>(yp + 32 * k);
+                    } else {
+                        uint32_t v[4] = {};
+                        for (int i = 0; i < 4; ++i)
+                            if (mo + 32 * k + i < p.M) v[i] = __bfloat16_as_ushort(yp[32 * k + i]);
+                        y[n][k] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+                    }
                 }
             }
         }
-        const size_t row = static_cast<size_t>(e.first[en]) * p.M + min(m0 + lane, p.M - 1);
-        const __nv_bfloat16* sp = p.us + row;
-        const uint8_t* zp = p.uz + row;
-        __nv_bfloat16 s_next = __nv_bfloat16();
-        uint8_t z_next = 0;
-        auto look = [&] {
-            s_next = *sp;
-            z_next = *zp;
-            sp += p.M;
-            zp += p.M;
-        };
-        if (ng) look();
-        float acc[2][NT][4] = {};
+        uint32_t at = static_cast<uint32_t>(e.first[en]) * p.M + m0;              // place of the step's first scale
+        float acc[NT][8] = {};
         for (int j = 0; j < ng; ++j) {
-            const float us = __bfloat162float(s_next), usz = us * z_next;
-            if (j + 1 < ng) look();
-            md_wait<MD_UDEPTH - 2>();
-            uint4 c[4];
+            md_wait<MD_UDEPTH - 1>();
+            __syncwarp();
+            const uint8_t* sz = side + slot * MD_SIDE;
+            float us[2], usz[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = lds16(fifo + (slot * 4 + i) * MD_THREADS * 16);
-            issue(slot == 0 ? MD_UDEPTH - 1 : slot - 1);
-            slot = slot + 1 == MD_UDEPTH ? 0 : slot + 1;
-            md_u_step<NT>(c, hcol, hsum, j, us, usz, acc);
-        }
-        // the two parts of a column are added; lane (gid, tig < 2) then has rows 2 tig, 2 tig + 1 of the entry at outputs gid + 8 i, which go through shared
-        // memory into the order in which they are stored
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float v = acc[i >> 2][n][i & 3];
-                v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-                if (tig < 2) stage[(n * 4 + tig * 2 + (i & 1)) * MD_STAGE + gid + 8 * (i >> 1)] = v;
+            for (int k = 0; k < 2; ++k) {
+                us[k] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(sz + (at * 2 & 15) + (lane + 32 * k) * 2));
+                usz[k] = us[k] * sz[144 + (at & 15) + lane + 32 * k];
             }
-        __syncwarp();
+            at += p.M;
+            __syncwarp();                                                        // every lane has read the scales and zero-points
+            md_u_step<NT>(fifo + slot * (8 * MD_THREADS * 16), hcol, hsum, h_at + j, us, usz, acc, [&](int m) { piece(slot, m); });
+            rest(slot);
+            slot ^= 1;
+        }
+        // lane (gid, tig) has row n * 4 + tig of the entry at outputs gid + 8 i, which go through shared memory into the order in which they are stored
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = n * 4 + (lane >> 3);
-            const float4 v = *reinterpret_cast<const float4*>(stage + r * MD_STAGE + (lane & 7) * 4);
-            if (r < rows && mo < p.M) {
-                __nv_bfloat16* o = p.out + static_cast<size_t>(e.row[en][r]) * p.M + mo;
-                const uint2 w = make_uint2(md_pack(md_lo(y[n].x) + v.x, md_hi(y[n].x) + v.y), md_pack(md_lo(y[n].y) + v.z, md_hi(y[n].y) + v.w));
-                if (vec) {
-                    *reinterpret_cast<uint2*>(o) = w;
-                } else {
-                    const uint32_t b[4] = {w.x & 0xFFFFu, w.x >> 16, w.y & 0xFFFFu, w.y >> 16};
-                    for (int i = 0; i < 4; ++i)
-                        if (mo + i < p.M) o[i] = __ushort_as_bfloat16(static_cast<unsigned short>(b[i]));
+            __nv_bfloat16* o = p.out + static_cast<size_t>(e.row[en][r < rows ? r : 0]) * p.M + mo;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) stage[tig * MD_STAGE + gid + 8 * i] = acc[n][4 * k + i];
+                __syncwarp();
+                const float4 v = *reinterpret_cast<const float4*>(stage + (lane >> 3) * MD_STAGE + (lane & 7) * 4);
+                __syncwarp();
+                if (r < rows && mo + 32 * k < p.M) {
+                    const uint2 w = make_uint2(md_pack(md_lo(y[n][k].x) + v.x, md_hi(y[n][k].x) + v.y), md_pack(md_lo(y[n][k].y) + v.z, md_hi(y[n][k].y) + v.w));
+                    if (vec) {
+                        *reinterpret_cast<uint2*>(o + 32 * k) = w;
+                    } else {
+                        const uint32_t b[4] = {w.x & 0xFFFFu, w.x >> 16, w.y & 0xFFFFu, w.y >> 16};
+                        for (int i = 0; i < 4; ++i)
+                            if (mo + 32 * k + i < p.M) o[32 * k + i] = __ushort_as_bfloat16(static_cast<unsigned short>(b[i]));
+                    }
                 }
             }
         }
-        __syncwarp();
     };
-    for (int en = first.en; en < e.n && tile_end(en) > 0; ++en) {
-        if (e.ng[en]) bring(en, e.ng[en]);
-        for (int t = tile_begin(en) + warp; t < tile_end(en); t += MD_THREADS / 32) {
-            if (e.rows[en] <= 4) work(en, t, MdTiles<1>{});
-            else work(en, t, MdTiles<2>{});
+    // entries by the batch: as many as have room for their rank groups in shared memory
+    Place at = {first.en, first.tile + warp};
+    for (int b0 = first.en; b0 < e.n && tile_end(b0) > 0;) {
+        const int g0 = e.groups_end[b0] - e.ng[b0];
+        int b1 = b0;
+        __syncthreads();                                                         // nobody reads the columns in place any more
+        for (; b1 < e.n && tile_end(b1) > 0 && e.groups_end[b1] - g0 <= MD_MAX_GROUPS; ++b1) bring(b1, e.groups_end[b1] - e.ng[b1] - g0);
+        __syncthreads();
+        for (settle(at); at.en < b1; settle(at)) {
+            const int h_at = e.groups_end[at.en] - e.ng[at.en] - g0;
+            if (e.rows[at.en] <= 4) work(at.en, at.tile, h_at, MdTiles<1>{});
+            else work(at.en, at.tile, h_at, MdTiles<2>{});
+            at.tile += MD_THREADS / 32;
         }
+        b0 = b1;
     }
 }
 
