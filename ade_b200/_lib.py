@@ -139,7 +139,7 @@ def load() -> ctypes.CDLL:
     for name in ("ade_b200_rmsnorm", "ade_b200_add_rmsnorm", "ade_b200_rope", "ade_b200_silu_mul", "ade_b200_attn_decode"):
         getattr(lib, name).restype = ci
     lib.ade_b200_paged_extend.argtypes = [vp] * 12 + [sz, ci, ci, ll, ci, ci, ci, vp]
-    lib.ade_b200_paged_extend_workspace_bytes.argtypes = [ci]
+    lib.ade_b200_paged_extend_workspace_bytes.argtypes = [ci, ci]
     lib.ade_b200_paged_write.argtypes = [vp] * 7 + [ci] * 5 + [ll] * 5 + [vp]
     lib.ade_b200_paged_attn.argtypes = [vp] * 10 + [sz] + [ci] * 3 + [ll] + [ci] * 5 + [ll] * 3 + [ctypes.c_float, vp]
     lib.ade_b200_paged_attn_workspace_bytes.argtypes = [ci] * 4

@@ -410,26 +410,39 @@ __device__ __forceinline__ void md_u_step(uint32_t codes, const uint8_t* hcol, c
 #pragma unroll
         for (int h = 0; h < 2; ++h) b[n][h] = *reinterpret_cast<const uint4*>(hcol + (n * 8 + gid) * MD_HCOL + j * 128 + (h * 4 + tig) * 16);
     }
+    constexpr int PAIR = 2 / NT;                                        // blocks of 16 rows at a time: two chains of products in flight
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        const uint4 p0 = lds16(codes + (m * 2) * MD_THREADS * 16), p1 = lds16(codes + (m * 2 + 1) * MD_THREADS * 16);
-        int d[NT][4];
+    for (int m0 = 0; m0 < 4; m0 += PAIR) {
+        uint4 q0[PAIR], q1[PAIR];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.x, p1.x, b[n][0].x, b[n][0].y, base);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.y, p1.y, b[n][0].z, b[n][0].w, d[n]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.z, p1.z, b[n][1].x, b[n][1].y, d[n]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) md_mma_word(d[n], p0.w, p1.w, b[n][1].z, b[n][1].w, d[n]);
-        refill(m);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {                                   // rows gid + 8 (2 m + i) of the tile
-            const int from = gid + 8 * (m * 2 + i & 3);
-            const float f = __shfl_sync(0xFFFFFFFFu, us[m >> 1], from), z = __shfl_sync(0xFFFFFFFFu, usz[m >> 1], from);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][m * 2 + i] += f * md_join(d[n][i * 2], d[n][i * 2 + 1], s[n].x) - z * s[n].y;
+        for (int k = 0; k < PAIR; ++k) {
+            q0[k] = lds16(codes + ((m0 + k) * 2) * MD_THREADS * 16);
+            q1[k] = lds16(codes + ((m0 + k) * 2 + 1) * MD_THREADS * 16);
         }
+        int d[PAIR][NT][4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int k = 0; k < PAIR; ++k) {
+                const uint32_t w0 = w == 0 ? q0[k].x : w == 1 ? q0[k].y : w == 2 ? q0[k].z : q0[k].w;
+                const uint32_t w1 = w == 0 ? q1[k].x : w == 1 ? q1[k].y : w == 2 ? q1[k].z : q1[k].w;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4& c = b[n][w >> 1];
+                    md_mma_word(d[k][n], w0, w1, w & 1 ? c.z : c.x, w & 1 ? c.w : c.y, w == 0 ? base : d[k][n]);
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k) refill(m0 + k);
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {                               // rows gid + 8 (2 m + i) of the tile
+                const int m = m0 + k, from = gid + 8 * (m * 2 + i & 3);
+                const float f = __shfl_sync(0xFFFFFFFFu, us[m >> 1], from), z = __shfl_sync(0xFFFFFFFFu, usz[m >> 1], from);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n][m * 2 + i] += f * md_join(d[k][n][i * 2], d[k][n][i * 2 + 1], s[n].x) - z * s[n].y;
+            }
     }
 }
 

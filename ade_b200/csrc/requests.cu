@@ -13,6 +13,18 @@ using ade_host::cuda_ok;
 
 namespace {
 
+// Dynamic shared memory of a kernel beyond 48 KB, asked for once per device.
+template <auto Kernel>
+bool allow_smem(size_t bytes) {
+    static bool done[64];
+    int dev = 0;
+    if (!cuda_ok(cudaGetDevice(&dev))) return false;
+    if (dev < 64 && done[dev]) return true;
+    if (!cuda_ok(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)))) return false;
+    if (dev < 64) done[dev] = true;
+    return true;
+}
+
 int launched() { return cuda_ok(cudaGetLastError()) ? ADE_OK : ADE_ERR_CUDA; }
 
 bool dim_ok(int head_dim) { return head_dim >= 32 && head_dim <= 256 && head_dim % 32 == 0; }
@@ -50,8 +62,7 @@ int launch_attn(ade::PagedAttnParams p, int sms, cudaStream_t st) {
     using S = ade::PaShape<HD>;
     const int ctas = sms < ade::PA_MAX_CTAS ? sms : ade::PA_MAX_CTAS;
     const size_t smem = ade::pa_smem_bytes(S::kRing, S::kWarps, S::kStages, p.T);
-    const int most = static_cast<int>(ade::pa_smem_bytes(S::kRing, S::kWarps, S::kStages, ade::PA_MAX_ROWS));
-    if (!cuda_ok(cudaFuncSetAttribute(ade::paged_attn_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, most))) return ADE_ERR_CUDA;
+    if (!allow_smem<ade::paged_attn_kernel<HD>>(ade::pa_smem_bytes(S::kRing, S::kWarps, S::kStages, ade::PA_MAX_ROWS))) return ADE_ERR_CUDA;
     ade::paged_attn_kernel<HD><<<ctas, S::kWarps * 32, smem, st>>>(p);
     if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
     return launch_early(ade::paged_attn_join_kernel<HD>, ctas * S::kWarps, 256, 0, st, p);
@@ -74,7 +85,9 @@ int launch_attn_dim(int head_dim, const ade::PagedAttnParams& p, int sms, cudaSt
 
 extern "C" {
 
-size_t ade_b200_paged_extend_workspace_bytes(int B) { return B < 1 || B > ADE_B200_MAX_REQUESTS ? 0 : 16 + ade::px_smem_bytes(B); }
+size_t ade_b200_paged_extend_workspace_bytes(int B, int total) {
+    return B < 1 || B > ADE_B200_MAX_REQUESTS || total <= kExtendOneCta ? 0 : 16 + ade::px_smem_bytes(B);
+}
 
 int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
                           int32_t* lengths_out, int32_t* free_count_out, int32_t* status, long long* slots, long long* positions, int32_t* requests,
@@ -84,9 +97,10 @@ int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int
     if (total > 0 && (!slots || !positions || !requests)) return ADE_ERR_NULL;
     if (B < 1 || B > ADE_B200_MAX_REQUESTS || width < 1 || table_row_stride < width || pages < 1 || page_size < 1 || total < 0) return ADE_ERR_SHAPE;
     if (static_cast<long long>(width) * page_size > 0x7FFFFFFFll || total > (1 << 30)) return ADE_ERR_SHAPE;
-    if (!work) return ADE_ERR_NULL;
+    const bool split = total > kExtendOneCta;
+    if (split && !work) return ADE_ERR_NULL;
     if (!aligned16(work)) return ADE_ERR_ALIGN;
-    if (work_bytes < ade_b200_paged_extend_workspace_bytes(B)) return ADE_ERR_SCRATCH;
+    if (work_bytes < ade_b200_paged_extend_workspace_bytes(B, total)) return ADE_ERR_SCRATCH;
     int sms = 0;
     const int rc = ade_host::sm_count(&sms);
     if (rc) return rc;
@@ -94,15 +108,12 @@ int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int
                                  requests, static_cast<int*>(work), B, width, pages, page_size, total, table_row_stride};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const size_t smem = ade::px_smem_bytes(B);
-    const bool split = total > kExtendOneCta;
     if (B <= 128 && !split) {
         ade::paged_extend_kernel<128, 1><<<1, 128, smem, st>>>(p, false);
         return launched();
     }
-    if (smem > 40 * 1024 &&
-        (!cuda_ok(cudaFuncSetAttribute(ade::paged_extend_kernel<1024, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem))) ||
-         !cuda_ok(cudaFuncSetAttribute(ade::paged_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))))
-        return ADE_ERR_CUDA;
+    const size_t most = ade::px_smem_bytes(ADE_B200_MAX_REQUESTS);
+    if (!allow_smem<ade::paged_extend_kernel<1024, 4>>(most) || !allow_smem<ade::paged_place_kernel>(most)) return ADE_ERR_CUDA;
     ade::paged_extend_kernel<1024, 4><<<1, 1024, smem, st>>>(p, split);
     if (!split || !cuda_ok(cudaGetLastError())) return launched();
     const int ctas = (total + 511) / 512;
@@ -194,9 +205,7 @@ int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_ban
                                reinterpret_cast<const bf*>(d.us), reinterpret_cast<const bf*>(d.vs), d.start, ids, static_cast<float*>(work),
                                d.M, d.N, d.groups, d.deltas, T};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!cuda_ok(cudaFuncSetAttribute(ade::multi_delta_v_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ade::md_v_smem()))) ||
-        !cuda_ok(cudaFuncSetAttribute(ade::multi_delta_u_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ade::md_u_smem()))))
-        return ADE_ERR_CUDA;
+    if (!allow_smem<ade::multi_delta_v_kernel>(ade::md_v_smem()) || !allow_smem<ade::multi_delta_u_kernel>(ade::md_u_smem())) return ADE_ERR_CUDA;
     const int slices = ade::md_slices(d.N);
     ade::multi_delta_v_kernel<<<2 * sms, ade::MD_THREADS, ade::md_v_smem(), st>>>(p, slices);
     if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;

@@ -8,9 +8,12 @@
 //   torch.ops.ade_b200.multi_delta(x, y_dense, uq, us, uz, vt, vs, vz, start, M, N, ids) -> out
 //   torch.ops.ade_b200.token_logprobs(logits, tokens?, top) -> (logprobs, entropy, top_logprobs, top_tokens)
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
+
+#include <array>
 
 #include "../../include/ade_b200.h"
 
@@ -48,6 +51,35 @@ int as_int(int64_t v, const char* name) {
 }
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+// A fresh contiguous tensor on the device of `like`, without the dispatcher (about a microsecond of host time for each output).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt); }
+
+// Several fresh contiguous tensors on the device of `like` in one allocation: they share a storage (and nothing else), which halves the host
+// time of an operator with six outputs.
+struct Out {
+    at::DimVector sizes;
+    at::ScalarType type;
+};
+template <size_t N>
+std::array<Tensor, N> fresh_all(const std::array<Out, N>& want, const Tensor& like) {
+    std::array<int64_t, N + 1> at_byte;
+    at_byte[0] = 0;
+    for (size_t i = 0; i < N; ++i) {
+        int64_t n = static_cast<int64_t>(c10::elementSize(want[i].type));
+        for (int64_t d : want[i].sizes) n *= d;
+        at_byte[i + 1] = at_byte[i] + (n + 15) / 16 * 16;
+    }
+    const Tensor all = fresh({at_byte[N]}, at::kByte, like);
+    std::array<Tensor, N> out;
+    for (size_t i = 0; i < N; ++i) {
+        out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                          c10::scalarTypeToTypeMeta(want[i].type));
+        out[i].unsafeGetTensorImpl()->set_storage_offset(at_byte[i] / static_cast<int64_t>(c10::elementSize(want[i].type)));
+        out[i].unsafeGetTensorImpl()->set_sizes_contiguous(want[i].sizes);
+    }
+    return out;
+}
 
 // stride of dimension `d`, or 0 where the tensor has a single entry there (torch gives such a dimension any stride)
 int64_t stride_of(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
@@ -88,16 +120,16 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> paged_extend(const Te
     check_whole(free_count, "free_count", at::kInt, {1}, table);
     const c10::cuda::CUDAGuard guard(table.device());
     const int n = as_int(total, "total");
-    const auto i32 = lengths.options(), i64 = lengths.options().dtype(at::kLong);
-    Tensor slots = at::empty({total}, i64), positions = at::empty({total}, i64), requests = at::empty({total}, i32), status = at::empty({B}, i32);
-    Tensor len_out = at::empty({in_place ? 0 : B}, i32), count_out = at::empty({in_place ? 0 : 1}, i32);       // an operator may not return an argument
-    const size_t bytes = ade_b200_paged_extend_workspace_bytes(as_int(B, "requests"));
-    const Tensor work = at::empty({static_cast<int64_t>(bytes)}, lengths.options().dtype(at::kByte));
+    auto [slots, positions, requests, len_out, count_out, status] =             // in place: an operator may not return an argument
+        fresh_all<6>({{{{total}, at::kLong}, {{total}, at::kLong}, {{total}, at::kInt}, {{in_place ? 0 : B}, at::kInt}, {{in_place ? 0 : 1}, at::kInt},
+                       {{B}, at::kInt}}}, table);
+    const size_t bytes = ade_b200_paged_extend_workspace_bytes(as_int(B, "requests"), n);
+    const Tensor work = bytes ? fresh({static_cast<int64_t>(bytes)}, at::kByte, table) : Tensor();
     auto i = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
     auto l = [](const Tensor& t) { return static_cast<long long*>(t.data_ptr()); };
     check_rc(ade_b200_paged_extend(i(lengths), i(new_tokens), i(table), i(free_pages), i(free_count), i(in_place ? lengths : len_out),
                                    i(in_place ? free_count : count_out), i(status), l(slots),
-                                   l(positions), i(requests), work.data_ptr(), bytes, as_int(B, "requests"), as_int(table.size(1), "width"),
+                                   l(positions), i(requests), bytes ? work.data_ptr() : nullptr, bytes, as_int(B, "requests"), as_int(table.size(1), "width"),
                                    table_stride(table),
                                    as_int(free_pages.size(0), "pages"), as_int(page_size, "page_size"), n, stream_of(table)),
              "ade_b200_paged_extend");
@@ -137,11 +169,11 @@ Tensor paged_attn(const Tensor& q, const Tensor& table, const Tensor& requests, 
     check_whole(positions, "positions", at::kLong, {T}, k_pages);
     check_angles(cos, sin, T, dim, k_pages);
     const c10::cuda::CUDAGuard guard(k_pages.device());
-    Tensor out = at::empty({T, hq * dim}, q.options());
+    Tensor out = fresh({T, hq * dim}, at::kBFloat16, q);
     if (T == 0) return out;
     const int t = as_int(T, "rows"), h = as_int(hq, "q_heads"), g = as_int(hk, "kv_heads"), d = as_int(dim, "head_dim");
     const size_t bytes = ade_b200_paged_attn_workspace_bytes(t, h, g, d);
-    const Tensor work = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    const Tensor work = fresh({static_cast<int64_t>(bytes)}, at::kByte, q);
     check_rc(ade_b200_paged_attn(q.data_ptr(), cos ? cos->data_ptr() : nullptr, sin ? sin->data_ptr() : nullptr, static_cast<const int32_t*>(table.data_ptr()),
                                  static_cast<const int32_t*>(requests.data_ptr()), static_cast<const long long*>(positions.data_ptr()), k_pages.data_ptr(),
                                  v_pages.data_ptr(), out.data_ptr(), work.data_ptr(), bytes, t, as_int(table.size(0), "requests"),
@@ -168,7 +200,7 @@ Tensor multi_delta(const Tensor& x, const Tensor& y, const Tensor& uq, const Ten
     check(start, "bank tensor start", at::kInt, 1, x);
     TORCH_CHECK(start.is_contiguous() && start.size(0) >= 2, "bank tensor start must be contiguous with an entry for each delta and one behind");
     const c10::cuda::CUDAGuard guard(x.device());
-    Tensor out = at::empty({T, M}, x.options());
+    Tensor out = fresh({T, M}, at::kBFloat16, x);
     if (T == 0) return out;
     const int t = as_int(T, "rows");
     const ade_delta_bank_t bank = {static_cast<const uint8_t*>(uq.data_ptr()), static_cast<const uint16_t*>(us.data_ptr()),
@@ -177,7 +209,7 @@ Tensor multi_delta(const Tensor& x, const Tensor& y, const Tensor& uq, const Ten
                                    static_cast<const int32_t*>(start.data_ptr()), as_int(M, "M"), as_int(N, "N"), as_int(G, "groups"),
                                    as_int(start.size(0) - 1, "deltas")};
     const size_t bytes = ade_b200_multi_delta_workspace_bytes(t, bank.N);
-    const Tensor work = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+    const Tensor work = fresh({static_cast<int64_t>(bytes)}, at::kByte, x);
     check_rc(ade_b200_multi_delta(x.data_ptr(), y.data_ptr(), &bank, static_cast<const int32_t*>(ids.data_ptr()), out.data_ptr(), work.data_ptr(), bytes, t,
                                   stream_of(x)),
              "ade_b200_multi_delta");
@@ -193,9 +225,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
     TORCH_CHECK(top >= 0 && top <= 32 && top <= vocab, "top must be in 0 .. 32 and at most the vocabulary; got ", top);
     if (tokens) check_whole(*tokens, "tokens", at::kLong, {rows}, logits);
     const c10::cuda::CUDAGuard guard(logits.device());
-    const auto f32 = logits.options().dtype(at::kFloat), i64 = logits.options().dtype(at::kLong);
-    Tensor logp = tokens ? at::empty({rows}, f32) : at::empty({0}, f32), entropy = at::empty({rows}, f32), tl = at::empty({rows, top}, f32),
-           tt = at::empty({rows, top}, i64);
+    auto [logp, entropy, tl, tt] = fresh_all<4>({{{{tokens ? rows : 0}, at::kFloat}, {{rows}, at::kFloat}, {{rows, top}, at::kFloat}, {{rows, top}, at::kLong}}}, logits);
     if (rows == 0) return {logp, entropy, tl, tt};
     check_rc(ade_b200_token_logprobs(logits.data_ptr(), type == at::kFloat ? ADE_DTYPE_F32 : type == at::kHalf ? ADE_DTYPE_F16 : ADE_DTYPE_BF16,
                                      tokens ? static_cast<const long long*>(tokens->data_ptr()) : nullptr, tokens ? logp.data_ptr<float>() : nullptr,

@@ -149,7 +149,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         float32, natural logarithms.  Equal logits come in the order of their tokens.  There is no backward pass: logits that
         require a gradient are refused outside ``torch.no_grad()``.
     """
-    return _call(_lib.ops().token_logprobs, logits, tokens, top)
+    return _call("token_logprobs", logits, tokens, top)
 
 
 def _attn_decode_ok(mod, x, cos, mask, layer) -> bool:

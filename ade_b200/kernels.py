@@ -327,13 +327,19 @@ def _kernel_error(e: RuntimeError) -> Exception:
     return _lib.AdeKernelError(msg) if msg.startswith("ade_b200_") else e
 
 
-def _call(op, *args):
-    """One call of a binding that checks its arguments itself.  What it refuses (and tensors that are on no CUDA device) is a
+_bound: dict = {}
+
+
+def _call(name, *args):
+    """One call of a binding that checks its arguments itself (its overload is looked up once: a microsecond per call).  What it refuses (and tensors that are on no CUDA device) is a
     ValueError here, a status of the C ABI an AdeKernelError; anything else, out of memory among it, stays what it is."""
+    op = _bound.get(name)
+    if op is None:
+        op = _bound[name] = getattr(_lib.ops(), name).default
     try:
         return op(*args)
     except NotImplementedError:
-        raise ValueError(f"{op.__name__}: the tensors must be on a CUDA device") from None
+        raise ValueError(f"{name}: the tensors must be on a CUDA device") from None
     except RuntimeError as e:
         if type(e) is not RuntimeError:
             raise
@@ -456,4 +462,4 @@ def multi_delta_forward(x: torch.Tensor, y_dense: torch.Tensor, bank: dict, ids:
     y_dense alone.  Returns a fresh (T, d_o) bfloat16 tensor.  Each delta in use is read once for all of its rows.  No
     counterpart in the reference, which serves one delta at a time (src/serving.py:133-194).
     """
-    return _call(_lib.ops().multi_delta, x, y_dense, *[bank[k] for k in BANK_KEYS], bank["M"], bank["N"], ids)
+    return _call("multi_delta", x, y_dense, *[bank[k] for k in BANK_KEYS], bank["M"], bank["N"], ids)

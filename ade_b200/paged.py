@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
 from .kernels import _call
 
 MAX_REQUESTS = 4096            # ADE_B200_MAX_REQUESTS
@@ -41,7 +40,7 @@ def paged_extend(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: t
         could not grow, have slot -1, position 0, request -1.  status (B,) int32 is 0, or a key of ``_lib.PAGED_STATUS`` that says
         why the request did not grow; its length then stays as it was.
     """
-    out = _call(_lib.ops().paged_extend, lengths, new_tokens, block_table, free_pages, free_count, total, page_size, in_place)
+    out = _call("paged_extend", lengths, new_tokens, block_table, free_pages, free_count, total, page_size, in_place)
     return (*out[:3], lengths, free_count, out[5]) if in_place else out
 
 
@@ -53,7 +52,7 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     `paged_extend`.  With cos and sin, (rows, head_dim), keys are rotated as the model does it, in float32 and rounded once; without,
     they are stored as they are.  Rows whose slot is no place of the cache are left out.  head_dim: a multiple of 32 up to 256.
     """
-    _call(_lib.ops().paged_write, k, v, slots, k_pages, v_pages, cos, sin)
+    _call("paged_write", k, v, slots, k_pages, v_pages, cos, sin)
 
 
 def paged_attn_decode(q: torch.Tensor, block_table: torch.Tensor, requests: torch.Tensor, positions: torch.Tensor, k_pages: torch.Tensor,
@@ -64,4 +63,4 @@ def paged_attn_decode(q: torch.Tensor, block_table: torch.Tensor, requests: torc
     heads of a key-value head are consecutive.  Rows without a request (requests[t] = -1) are zero.  Returns
     (rows, q_heads * head_dim) bfloat16; scores, probabilities and sums are float32.
     """
-    return _call(_lib.ops().paged_attn, q, block_table, requests, positions, k_pages, v_pages, scale, cos, sin)
+    return _call("paged_attn", q, block_table, requests, positions, k_pages, v_pages, scale, cos, sin)

@@ -319,8 +319,8 @@ int ade_b200_attn_decode(const void* q, const void* k, const void* v, const void
  *                  request b did not grow (its length then stays): ADE_PAGED_NO_PAGE (the stack does not reach to it),
  *                  ADE_PAGED_TABLE_FULL (width * page_size), ADE_PAGED_NO_ROW (its rows do not end within `total`),
  *                  ADE_PAGED_BAD_LENGTH (negative, or beyond its row of the table; nothing is handed back either).  lengths_out
- *                  and free_count_out may be lengths and free_count; work: 16-byte aligned, ade_b200_paged_extend_workspace_bytes,
- *                  contents of no meaning before and after the call.  B <= ADE_B200_MAX_REQUESTS, width * page_size < 2^31,
+ *                  and free_count_out may be lengths and free_count; work: 16-byte aligned, ade_b200_paged_extend_workspace_bytes
+ *                  (0 up to 2048 rows: work may be NULL), contents of no meaning before and after the call.  B <= ADE_B200_MAX_REQUESTS, width * page_size < 2^31,
  *                  total <= 2^30.
  *   ade_b200_paged_write   k [T][kv_heads][head_dim] (rotated with cos / sin [T][head_dim] in float32 and rounded once; both NULL:
  *                  as it is) and v into the slots of their rows; slots outside 0 .. pages * page_size - 1 are left out.  Of two rows
@@ -370,7 +370,7 @@ typedef struct ade_delta_bank {
     int M, N, groups, deltas;
 } ade_delta_bank_t;
 
-size_t ade_b200_paged_extend_workspace_bytes(int B);
+size_t ade_b200_paged_extend_workspace_bytes(int B, int total);
 int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
                           int32_t* lengths_out, int32_t* free_count_out, int32_t* status, long long* slots, long long* positions, int32_t* requests,
                           void* work, size_t work_bytes, int B, int width, long long table_row_stride, int pages, int page_size, int total,

@@ -54,7 +54,7 @@ def _logprobs(**kw):
     (lambda: _extend(B=0), SHAPE), (lambda: _extend(B=4097), SHAPE), (lambda: _extend(width=0), SHAPE), (lambda: _extend(stride=7), SHAPE),
     (lambda: _extend(pages=0), SHAPE), (lambda: _extend(page=0), SHAPE), (lambda: _extend(total=-1), SHAPE),
     (lambda: _extend(width=1 << 20, stride=1 << 20, page=2048), SHAPE), (lambda: _extend(total=(1 << 30) + 1), SHAPE),
-    (lambda: _extend(work=None), NULL), (lambda: _extend(work=P + 4), ALIGN), (lambda: _extend(work_bytes=16), SCRATCH),
+    (lambda: _extend(work=None, total=5000), NULL), (lambda: _extend(work=P + 4), ALIGN), (lambda: _extend(work_bytes=16, total=5000), SCRATCH),
     (lambda: _write(k=None), NULL), (lambda: _write(cos=None), NULL), (lambda: _write(slots=None), NULL), (lambda: _write(T=0), SHAPE),
     (lambda: _write(heads=0), SHAPE), (lambda: _write(dim=48), SHAPE), (lambda: _write(dim=288), SHAPE), (lambda: _write(dim=0), SHAPE),
     (lambda: _write(page=0), SHAPE), (lambda: _write(k_row=-128), SHAPE), (lambda: _write(kp=P + 8), ALIGN), (lambda: _write(vp=P + 2), ALIGN),
