@@ -8,7 +8,8 @@
 // free) and the two halves of a result are added in float32.  The running maximum and sum of the softmax stay in registers.
 //
 // The cache is cut into tiles of 16 positions; the tiles of all pairs, one pair behind the other, are shared out evenly over the
-// CTAs and there over the warps, whatever the lengths.  A warp streams its tiles through cp.async stages of its own and never waits
+// CTAs and there over the warps, whatever the lengths.  On that line of tiles every pair has PA_GAP places more in front of its tiles, for what
+// a pair costs besides them (its queries, its result): without them the warps that meet the short pairs of a ragged batch end last.  A warp streams its tiles through cp.async stages of its own and never waits
 // for another; what it has of a pair that others share goes to the workspace as (maximum, sum, weighted sum), and a second
 // launch joins those parts in the order of the tiles.  A CTA whose tiles all belong to one pair joins its warps' parts itself.
 #pragma once
@@ -18,9 +19,10 @@
 namespace ade {
 
 constexpr int PA_MAX_CTAS = 160;           // one CTA per SM; bounds the workspace
-constexpr int PA_MAX_ROWS = 1024;          // rows of one launch (their prefix sums lie in shared memory)
+constexpr int PA_MAX_ROWS = 1024;          // rows of one launch (their prefix sums lie in shared memory); the places of a launch fit 31 bits
 constexpr int PA_HEADS = 8;                // query heads that share one pass over the keys and values
 constexpr int PA_TILE = 16;                // positions of a tile
+constexpr int PA_GAP = 5;                  // places of the line in front of a pair's tiles (1: 107 us, 2: 91, 4: 83, 6: 84, 9: 83 with 32 rows of 16 to 4000 positions)
 
 struct PagedAttnParams {
     const __nv_bfloat16 *q, *cs, *sn;          // q [T][q_heads][dim] by strides; cs, sn [T][dim] or nullptr: q is used as it is
@@ -35,6 +37,7 @@ struct PagedAttnParams {
     long long table_stride, q_row, q_head, cs_row;
     int T, B, width, pages, page_size, q_heads, kv_heads;
     float scale2;                              // scale * log2(e)
+    bool pairs;                                // q, cs and sn begin every row and head at an even element of 4-byte aligned memory
 };
 
 template <int HD>
@@ -50,7 +53,7 @@ struct PaShape {
     }
 };
 inline size_t pa_smem_bytes(size_t ring, int warps, int stages, int T) {
-    return ring + static_cast<size_t>(T + 1) * 8 + static_cast<size_t>(T) * 8 + static_cast<size_t>(warps) * stages * 4 + static_cast<size_t>(warps) * PA_HEADS * 8;
+    return ring + (static_cast<size_t>(T) * 3 + 4) * 4 + static_cast<size_t>(warps) * stages * 4 + static_cast<size_t>(warps) * PA_HEADS * 8;
 }
 
 __device__ __forceinline__ void pa_ldm4(uint32_t a, uint32_t (&r)[4]) {
@@ -79,39 +82,55 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
     using S = PaShape<HD>;
     constexpr int KS = HD / 16, NW = S::kWarps, NT = NW * 32;
     extern __shared__ __align__(128) uint8_t pa_smem[];
-    long long* prefix = reinterpret_cast<long long*>(pa_smem + S::kRing);        // [T + 1] tiles of the rows before (one pair each)
-    int* rown = reinterpret_cast<int*>(prefix + p.T + 1);                          // [T] positions the row sees
-    int* rowreq = rown + p.T;                                                      // [T] its request
-    float2* mstat = reinterpret_cast<float2*>(rowreq + p.T);                       // [NW][PA_HEADS]
+    float2* mstat = reinterpret_cast<float2*>(pa_smem + S::kRing);                 // [NW][PA_HEADS]
     uint32_t* masks = reinterpret_cast<uint32_t*>(mstat + NW * PA_HEADS);          // [NW][stages] positions of a tile that count
-    __shared__ long long ws[NW];
+    int* prefix = reinterpret_cast<int*>(masks + NW * S::kStages);                 // [T + 1] places of the rows before, of all their pairs
+    int* rown = prefix + p.T + 1;                                                  // [T] positions the row sees
+    int* rowreq = rown + p.T;                                                      // [T] its request
+    __shared__ int ws[NW];
+    __shared__ int wmax[NW], wrows[NW];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int group = p.q_heads / p.kv_heads, sets = (group + PA_HEADS - 1) / PA_HEADS, H = p.kv_heads * sets;
 
-    // tiles of every row, summed
+    // places of every row, summed, the longest row and the rows that have any
+    auto places = [](int n) { return n ? (n + PA_TILE - 1) / PA_TILE + PA_GAP : 0; };              // of one pair
     const int per = (p.T + NT - 1) / NT, ta = min(tid * per, p.T), tb = min(ta + per, p.T);
-    long long mine = 0;
+    int mine = 0, longest = 0, live = 0;
     for (int t = ta; t < tb; ++t) {
         const int req = p.requests[t];
         const long long pos = p.positions[t];
-        const int n = req < 0 || req >= p.B || pos < 0 ? 0 : static_cast<int>(min(pos + 1, static_cast<long long>(p.width) * p.page_size));
+        const int n = req < 0 || req >= p.B || pos < 0 ? 0 : static_cast<int>(min(pos, static_cast<long long>(p.width) * p.page_size - 1)) + 1;
         rown[t] = n;
         rowreq[t] = req;
-        mine += (n + PA_TILE - 1) / PA_TILE;
+        mine += places(n) * H;
+        longest = max(longest, places(n));
+        live += n > 0;
     }
-    long long run = mine;
+    int run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xFFFFFFFFu, run, o);
+        const int u = __shfl_up_sync(0xFFFFFFFFu, run, o);
         if (lane >= o) run += u;
     }
-    if (lane == 31) ws[warp] = run;
+    longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+    live = __reduce_add_sync(0xFFFFFFFFu, live);
+    if (lane == 31) {
+        ws[warp] = run;
+        wmax[warp] = longest;
+        wrows[warp] = live;
+    }
     __syncthreads();
     run -= mine;
-    for (int w = 0; w < warp; ++w) run += ws[w];
+    live = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        longest = max(longest, wmax[w]);
+        live += wrows[w];
+        if (w < warp) run += ws[w];
+    }
     for (int t = ta; t < tb; ++t) {
         prefix[t] = run;
-        run += (rown[t] + PA_TILE - 1) / PA_TILE;
+        run += places(rown[t]) * H;
     }
     if (tid == NT - 1) prefix[p.T] = run;
     __syncthreads();
@@ -123,87 +142,94 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
             for (int i = tid; i < p.q_heads * HD / 8; i += NT)
                 reinterpret_cast<uint4*>(p.out + static_cast<long long>(t) * p.q_heads * HD)[i] = make_uint4(0u, 0u, 0u, 0u);
 
-    // this warp's tiles f .. f_end - 1 of all, and whether its whole CTA works on one pair
-    const long long total = prefix[p.T] * H;
-    const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total)), cta = blockIdx.x;
-    auto cta_begin = [&](int c) { return total * c / ctas; };
+    // This warp's places f .. f_end - 1 of all, and whether its whole CTA works on one pair.  Where every warp would have two tiles at most, a pair
+    // gets as many CTAs of its own as it takes: for short rows one, which then needs nobody else.
+    const int total = prefix[p.T], cta = blockIdx.x, pairs = live * H;
+    int most = gridDim.x;
+    if (total <= most * NW * 2 && pairs > 0 && pairs <= most) most = pairs * min(most / pairs, (longest + 2 * NW - 1) / (2 * NW));
+    const int ctas = min(most, total), each = ctas ? total / ctas : 0, more = total - each * ctas;
+    auto cta_begin = [&](int c) { return each * c + min(c, more); };
     const int wid = cta * NW + warp;
-    if (cta >= ctas) {
+    auto no_work = [&] {
         if (lane == 0) p.meta[wid] = make_int4(0, 0, 0, 0);
-        return;
-    }
-    const long long F0 = cta_begin(cta), F1 = cta_begin(cta + 1);
-    long long f = F0 + (F1 - F0) * warp / NW;
-    const long long f_end = F0 + (F1 - F0) * (warp + 1) / NW;
-    struct Cursor {
-        int t, pair, tile, nt;
     };
-    auto locate = [&](long long g) {
-        int lo = 0, hi = p.T - 1;                                       // the row with prefix[t] * H <= g < prefix[t + 1] * H
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (prefix[mid] * H <= g) lo = mid;
-            else hi = mid - 1;
-        }
+    if (cta >= ctas) return no_work();
+    const int F0 = cta_begin(cta), F1 = cta_begin(cta + 1);
+    auto warp_begin = [](int f0, int f1, int w) { return f0 + static_cast<int>(static_cast<unsigned>(f1 - f0) * w / NW); };
+    struct Cursor {
+        int at, t, pair, tile, nt;                                      // place of the tile, row, pair of the row, tile of the pair and their number
+    };
+    // the first tile at or behind a place, by the whole warp: the last row whose places begin at or before it, 32 rows at a time
+    auto locate = [&](int g) {
+        const int hi = 32 * lane < p.T && prefix[32 * lane] <= g;
+        const int from = 32 * (__popc(__ballot_sync(0xFFFFFFFFu, hi)) - 1) + lane;
+        const int row = from < p.T && prefix[from] <= g;
         Cursor c;
-        c.t = lo;
-        c.nt = static_cast<int>(prefix[lo + 1] - prefix[lo]);
-        const long long rest = g - prefix[lo] * H;
-        c.pair = static_cast<int>(rest / c.nt);
-        c.tile = static_cast<int>(rest - static_cast<long long>(c.pair) * c.nt);
+        c.t = from - lane + __popc(__ballot_sync(0xFFFFFFFFu, row)) - 1;
+        const int nv = places(rown[c.t]), rest = g - prefix[c.t];
+        c.nt = nv - PA_GAP;
+        c.pair = static_cast<unsigned>(rest) / static_cast<unsigned>(nv);
+        c.tile = max(rest - c.pair * nv - PA_GAP, 0);
+        c.at = prefix[c.t] + c.pair * nv + PA_GAP + c.tile;
         return c;
     };
     auto advance = [&](Cursor& c) {
+        ++c.at;
         if (++c.tile < c.nt) return;
         c.tile = 0;
+        c.at += PA_GAP;
         if (++c.pair < H) return;
         c.pair = 0;
         do {
             ++c.t;
-        } while (c.t < p.T && prefix[c.t + 1] == prefix[c.t]);
-        c.nt = c.t < p.T ? static_cast<int>(prefix[c.t + 1] - prefix[c.t]) : 1;
+        } while (c.t < p.T && rown[c.t] == 0);
+        c.nt = c.t < p.T ? places(rown[c.t]) - PA_GAP : 1;
     };
-    auto pair_begin = [&](const Cursor& c) { return prefix[c.t] * H + static_cast<long long>(c.pair) * c.nt; };
+    auto pair_begin = [&](const Cursor& c) { return c.at - c.tile; };     // its first tile
     const Cursor c0 = locate(F0);
-    const bool merged = F1 <= pair_begin(c0) + c0.nt;                     // the CTA's tiles are all of pair c0
+    if (c0.at >= F1) return no_work();                                  // nothing but places in front of a pair's tiles
+    const bool merged = F1 <= pair_begin(c0) + c0.nt + PA_GAP;            // the CTA's tiles are all of pair c0
     int4 meta = make_int4(0, 0, 0, 0);
     // (last warp, flags) of the pair of c, which goes on behind this CTA or this warp
     auto chain = [&](const Cursor& c) {
-        const long long fe = pair_begin(c) + c.nt;
-        const int last = static_cast<int>((fe * ctas + total - 1) / total) - 1;
-        const long long L0 = cta_begin(last), L1 = cta_begin(last + 1);
-        const int lw = static_cast<int>(((fe - L0) * NW + (L1 - L0) - 1) / (L1 - L0)) - 1;
-        const bool last_merged = L0 >= pair_begin(c) && L1 <= fe;
+        const int fe = pair_begin(c) + c.nt, cut = more * (each + 1);     // the CTA and the warp that its last tile falls to
+        const int last = fe <= cut ? (fe - 1) / (each + 1) : more + (fe - 1 - cut) / each;
+        const int L0 = cta_begin(last), L1 = cta_begin(last + 1);
+        const int lw = static_cast<int>((static_cast<unsigned>(fe - L0) * NW - 1) / (L1 - L0));
+        const bool last_merged = L1 <= fe + PA_GAP;
         return make_int4(c.t + 1, c.pair, last * NW + min(lw, NW - 1), (merged ? 1 : 0) | (last_merged ? 2 : 0));
     };
 
     const uint32_t ring = smem_u32(pa_smem) + static_cast<uint32_t>(warp) * (S::kStages * 2 * S::kTileBytes);
     uint32_t* mk = masks + warp * S::kStages;
     // ---- the copies, STAGES - 1 tiles ahead of the arithmetic, the look at the block table one more
-    Cursor ahead = f < f_end ? locate(f) : c0;
-    long long f_look = f;
-    int l_page = -1, l_off = 0, l_kvh = 0;
+    const int f_end = warp_begin(F0, F1, warp + 1);
+    Cursor cur = warp == 0 ? c0 : locate(warp_begin(F0, F1, warp)), ahead = cur;
+    struct Look {
+        bool on;                                                        // the tile is one of this warp's
+        int page, off, kvh;
+    };
     auto look = [&] {
-        l_page = -1;
-        if (f_look < f_end) {
+        Look l = {ahead.at < f_end, -1, 0, 0};
+        if (l.on) {
             const int pos = ahead.tile * PA_TILE + (lane & 15);
-            l_kvh = ahead.pair / sets;
+            l.kvh = ahead.pair / sets;
             if (pos < rown[ahead.t]) {
                 const int col = pos / p.page_size;
-                l_off = pos - col * p.page_size;
-                l_page = p.table[rowreq[ahead.t] * p.table_stride + col];
+                l.off = pos - col * p.page_size;
+                l.page = p.table[rowreq[ahead.t] * p.table_stride + col];
             }
             advance(ahead);
         }
-        ++f_look;
+        return l;
     };
-    auto issue = [&](int stage) {
-        const bool ok = l_page >= 0 && l_page < p.pages;
-        const uint32_t row = ok ? (static_cast<uint32_t>(l_page) * p.kv_heads + l_kvh) * p.page_size + l_off : 0u;
+    auto issue = [&](int stage, const Look& l) {
+        const bool ok = l.page >= 0 && l.page < p.pages;
+        const uint32_t row = ok ? (static_cast<uint32_t>(l.page) * p.kv_heads + l.kvh) * p.page_size + l.off : 0u;
         const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
         if (lane == 0) mk[stage] = mask;
         const uint32_t dst = ring + static_cast<uint32_t>(stage) * (2 * S::kTileBytes);
-        if (f_look - 1 < f_end) {
+        if (l.on) {
 #pragma unroll
             for (int j = 0; j < S::kChunks / 2; ++j) {
                 const int i = j * 32 + lane, r = i / S::kChunks, c = i - r * S::kChunks;
@@ -215,60 +241,88 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    look();
-#pragma unroll 1
-    for (int s = 0; s < S::kStages - 1; ++s) {
-        issue(s);
-        look();
-    }
-
+    // the first tiles are looked up together, and the queries of the first pair requested, before anything is waited for
+    Look seen[S::kStages];
+#pragma unroll
+    for (int s = 0; s < S::kStages; ++s) seen[s] = look();
     uint32_t qa[KS][4];
     float acc[HD / 8][4], m = -INFINITY, l = 0.f;
-    Cursor cur = f < f_end ? locate(f) : c0;
+    const bool any = cur.at < f_end;
     bool fresh = true, from_start = false;
     int stage = 0, fill = S::kStages - 1;
     const int pair_heads = min(PA_HEADS, group);
     auto heads_of = [&](int pair) { return min(pair_heads, group - pair % sets * PA_HEADS); };
     auto first_head = [&](int pair) { return pair / sets * group + pair % sets * PA_HEADS; };
-    if (f >= f_end && !merged && lane < PA_HEADS) p.stat[(wid * 2) * PA_HEADS + lane] = make_float2(-INFINITY, 0.f);   // a warp without tiles
+    if (!any && !merged && lane < PA_HEADS) p.stat[(wid * 2) * PA_HEADS + lane] = make_float2(-INFINITY, 0.f);   // a warp without tiles
+    // Queries of a pair, heads by lanes (gid): dimensions d and d + HD / 2, d + 1 beside each, and the angles they are rotated by.
+    uint32_t raw[KS / 2][2][6];
+    auto ask = [&](const Cursor& c) {
+        const bool on = gid < heads_of(c.pair);
+        const __nv_bfloat16* qr = p.q + c.t * p.q_row + (first_head(c.pair) + (on ? gid : 0)) * p.q_head;
+        // two neighbours at once where every row begins at an even element
+        auto two = [&](const __nv_bfloat16* a) {
+            return p.pairs ? *reinterpret_cast<const uint32_t*>(a) : static_cast<uint32_t>(__bfloat16_as_ushort(a[0])) | static_cast<uint32_t>(__bfloat16_as_ushort(a[1])) << 16;
+        };
+#pragma unroll
+        for (int ks = 0; ks < KS / 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int d = ks * 16 + tig * 2 + i * 8;
+                uint32_t(&r)[6] = raw[ks][i];
+                r[0] = on ? two(qr + d) : 0u;
+                r[1] = on ? two(qr + d + HD / 2) : 0u;
+                if (p.cs) {
+                    const __nv_bfloat16 *cr = p.cs + c.t * p.cs_row + d, *sr = p.sn + c.t * p.cs_row + d;
+                    r[2] = two(cr);
+                    r[3] = two(cr + HD / 2);
+                    r[4] = two(sr);
+                    r[5] = two(sr + HD / 2);
+                }
+            }
+    };
+    auto rotate = [&] {                                                 // rotated, in two bfloat16 parts
+#pragma unroll
+        for (int ks = 0; ks < KS / 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t(&r)[6] = raw[ks][i];
+                float a0 = bf_lo(r[0]), a1 = bf_hi(r[0]), b0 = bf_lo(r[1]), b1 = bf_hi(r[1]);
+                if (p.cs) {
+                    const float x0 = a0, x1 = a1;
+                    a0 = x0 * bf_lo(r[2]) - b0 * bf_lo(r[4]);
+                    a1 = x1 * bf_hi(r[2]) - b1 * bf_hi(r[4]);
+                    b0 = b0 * bf_lo(r[3]) + x0 * bf_lo(r[5]);
+                    b1 = b1 * bf_hi(r[3]) + x1 * bf_hi(r[5]);
+                }
+                qa[ks][2 * i] = pa_split(a0, a1, qa[ks][2 * i + 1]);
+                qa[ks + KS / 2][2 * i] = pa_split(b0, b1, qa[ks + KS / 2][2 * i + 1]);
+            }
+    };
+    if (any) ask(cur);
+#pragma unroll
+    for (int s = 0; s < S::kStages - 1; ++s) issue(s, seen[s]);
+    Look next = seen[S::kStages - 1];
+    if (any) rotate();
+    bool have = true;
 #pragma unroll 1
-    for (; f < f_end; ++f) {
-        if (fresh) {                                                    // a new pair: its queries, rotated, in two bfloat16 parts
+    while (cur.at < f_end) {
+        if (fresh) {                                                    // a new pair
             fresh = false;
             from_start = cur.tile == 0;
             m = -INFINITY;
             l = 0.f;
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-            const bool on = gid < heads_of(cur.pair);
-            const __nv_bfloat16* qr = p.q + cur.t * p.q_row + (first_head(cur.pair) + (on ? gid : 0)) * p.q_head;
-            const __nv_bfloat16 *cr = p.cs + cur.t * p.cs_row, *sr = p.sn + cur.t * p.cs_row;
-            auto val = [](const __nv_bfloat16* a) { return __bfloat162float(*a); };
-#pragma unroll
-            for (int ks = 0; ks < KS / 2; ++ks) {
-                float a[4], b[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = ks * 16 + tig * 2 + (i & 1) + (i >> 1) * 8;
-                    const float x = on ? val(qr + d) : 0.f, y = on ? val(qr + d + HD / 2) : 0.f;
-                    a[i] = x;
-                    b[i] = y;
-                    if (p.cs) {
-                        a[i] = x * val(cr + d) - y * val(sr + d);
-                        b[i] = y * val(cr + d + HD / 2) + x * val(sr + d + HD / 2);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    qa[ks][2 * i] = pa_split(a[2 * i], a[2 * i + 1], qa[ks][2 * i + 1]);
-                    qa[ks + KS / 2][2 * i] = pa_split(b[2 * i], b[2 * i + 1], qa[ks + KS / 2][2 * i + 1]);
-                }
+            if (!have) {
+                ask(cur);
+                rotate();
             }
+            have = false;
         }
         pa_cp_wait<S::kStages - 2>();
         __syncwarp();                                                   // the tile is there, and the stage before it has been read by all lanes
-        issue(fill);
-        look();
+        issue(fill, next);
+        next = look();
         const uint32_t mask = mk[stage];
         if (mask) {
             const uint32_t kt = ring + static_cast<uint32_t>(stage) * (2 * S::kTileBytes), vt = kt + S::kTileBytes;
@@ -321,7 +375,7 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
         stage = stage + 1 == S::kStages ? 0 : stage + 1;
         fill = fill + 1 == S::kStages ? 0 : fill + 1;
         const bool pair_ends = cur.tile + 1 == cur.nt;
-        if (pair_ends || f + 1 == f_end) {
+        if (pair_ends || cur.at + 1 >= f_end) {
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
             l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
             const int heads = heads_of(cur.pair);
@@ -355,7 +409,6 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
         pa_cp_wait<0>();
         __syncwarp();
         float* mine_acc = reinterpret_cast<float*>(pa_smem) + static_cast<size_t>(warp) * (S::kStages * 2 * S::kTileBytes / 4);
-        const bool any = F0 + (F1 - F0) * warp / NW < f_end;
         const int heads = heads_of(c0.pair), h0 = first_head(c0.pair);
         if (any && gid < heads) {
 #pragma unroll
@@ -364,7 +417,7 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
         }
         if (tig == 0) mstat[warp * PA_HEADS + gid] = any ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         __syncthreads();
-        const bool whole = F0 == pair_begin(c0) && F1 == pair_begin(c0) + c0.nt, begins = F0 == pair_begin(c0);
+        const bool begins = F0 <= pair_begin(c0), whole = begins && F1 >= pair_begin(c0) + c0.nt;
         const int slot = cta * NW * 2 + (begins ? 1 : 0);
         for (int i = tid; i < heads * HD; i += NT) {
             const int h = i / HD, d = i - h * HD;

@@ -168,14 +168,21 @@ int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, con
     float* part = static_cast<float*>(work);
     float2* stat = reinterpret_cast<float2*>(part + kAttnWarps * 2 * ade::PA_HEADS * head_dim);
     int4* meta = reinterpret_cast<int4*>(stat + kAttnWarps * 2 * ade::PA_HEADS);
-    for (int t0 = 0; t0 < T; t0 += ade::PA_MAX_ROWS) {
+    const bool pairs = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) & 3) == 0 &&
+                       ((q_row_stride | q_head_stride | (cos_t ? cs_row_stride : 0)) & 1) == 0;
+    // rows of one launch: PA_MAX_ROWS, fewer where the places of that many full rows would not fit 31 bits
+    const long long heads = static_cast<long long>(kv_heads) * ((q_heads / kv_heads + ade::PA_HEADS - 1) / ade::PA_HEADS);
+    const long long fit = 0x7FFFFFFFll / (heads * (static_cast<long long>(width) * page_size / ade::PA_TILE + 1 + ade::PA_GAP));
+    if (fit < 1) return ADE_ERR_SHAPE;
+    const int chunk = fit < ade::PA_MAX_ROWS ? static_cast<int>(fit) : ade::PA_MAX_ROWS;
+    for (int t0 = 0; t0 < T; t0 += chunk) {
         const bf *cs = static_cast<const bf*>(cos_t), *sn = static_cast<const bf*>(sin_t);
         const long long o = t0;
         const ade::PagedAttnParams p = {static_cast<const bf*>(q) + o * q_row_stride, cs ? cs + o * cs_row_stride : nullptr,
                                         sn ? sn + o * cs_row_stride : nullptr, block_table, requests + o, positions + o, static_cast<const bf*>(k_pages),
                                         static_cast<const bf*>(v_pages), static_cast<bf*>(out) + o * q_heads * head_dim, part, stat, meta,
-                                        table_row_stride, q_row_stride, q_head_stride, cs_row_stride, T - t0 < ade::PA_MAX_ROWS ? T - t0 : ade::PA_MAX_ROWS, B,
-                                        width, pages, page_size, q_heads, kv_heads, scale * 1.44269504088896340736f};
+                                        table_row_stride, q_row_stride, q_head_stride, cs_row_stride, T - t0 < chunk ? T - t0 : chunk, B,
+                                        width, pages, page_size, q_heads, kv_heads, scale * 1.44269504088896340736f, pairs};
         const int rc_launch = launch_attn_dim(head_dim, p, sms, static_cast<cudaStream_t>(stream));
         if (rc_launch) return rc_launch;
     }
