@@ -22,7 +22,7 @@ constexpr int PA_MAX_CTAS = 160;           // one CTA per SM; bounds the workspa
 constexpr int PA_MAX_ROWS = 1024;          // rows of one launch (their prefix sums lie in shared memory); the places of a launch fit 31 bits
 constexpr int PA_HEADS = 8;                // query heads that share one pass over the keys and values
 constexpr int PA_TILE = 16;                // positions of a tile
-constexpr int PA_GAP = 5;                  // places of the line in front of a pair's tiles (1: 107 us, 2: 91, 4: 83, 6: 84, 9: 83 with 32 rows of 16 to 4000 positions)
+constexpr int PA_GAP = 3;                  // places of the line in front of a pair's tiles (0: 119 us, 2: 80.8, 3: 80.4, 5: 81.7 with 32 rows of 16 to 4000 positions)
 
 struct PagedAttnParams {
     const __nv_bfloat16 *q, *cs, *sn;          // q [T][q_heads][dim] by strides; cs, sn [T][dim] or nullptr: q is used as it is

@@ -48,12 +48,6 @@ int launch_early(void (*kernel)(Params...), int grid, int threads, size_t smem, 
 // Rows that one CTA of the page allocation still places itself.
 constexpr int kExtendOneCta = 2048;
 
-template <typename T>
-void launch_logprobs(const ade::LogprobParams& p, int sms, cudaStream_t st) {
-    if (p.rows <= sms) ade::logprob_kernel<T, 1024><<<p.rows, 1024, 0, st>>>(p);
-    else ade::logprob_kernel<T, 256><<<p.rows, 256, 0, st>>>(p);
-}
-
 constexpr size_t kAttnWarps = static_cast<size_t>(ade::PA_MAX_CTAS) * 8;
 
 // Both launches of the attention for up to PA_MAX_ROWS rows.  The second begins while the first runs and waits for its end.
@@ -229,9 +223,9 @@ int ade_b200_token_logprobs(const void* logits, int dtype, const long long* toke
     const ade::LogprobParams p = {logits, tokens, logprobs, entropy, top_logprobs, top_tokens, row_stride, rows, vocab, top};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case ADE_DTYPE_F32: launch_logprobs<float>(p, sms, st); break;
-        case ADE_DTYPE_BF16: launch_logprobs<__nv_bfloat16>(p, sms, st); break;
-        default: launch_logprobs<__half>(p, sms, st);
+        case ADE_DTYPE_F32: ade::logprob_kernel<float><<<rows, ade::LP_THREADS, 0, st>>>(p); break;
+        case ADE_DTYPE_BF16: ade::logprob_kernel<__nv_bfloat16><<<rows, ade::LP_THREADS, 0, st>>>(p); break;
+        default: ade::logprob_kernel<__half><<<rows, ade::LP_THREADS, 0, st>>>(p);
     }
     return launched();
 }

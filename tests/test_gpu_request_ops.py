@@ -479,6 +479,10 @@ def test_infinities_and_nan():
     x[7, 5], x[7, 9] = nan, nan
     tokens = torch.tensor([3, 0, 300, 4, 0, 9, 2, -5, V], device=DEV)
     _check_logprobs(x, tokens, 8)
+    for dtype in (torch.bfloat16, torch.float16):                     # the lowest value of each type beside -inf
+        y = x.clamp(min=torch.finfo(dtype).min).to(dtype)
+        y[6, 20:] = -inf
+        _check_logprobs(y, tokens, 8)
     logp, entropy, _, tt = token_logprobs(x, tokens, 2)
     assert entropy[1] == 0 and logp[1] == 0 and logp[4] == -inf and logp[7] == 0 and bool(torch.isnan(logp[8]))
     assert tt[0].tolist() == [0, 1] and tt[7].tolist() == [5, 9]
