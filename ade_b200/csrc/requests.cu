@@ -75,6 +75,9 @@ int launch_attn_dim(int head_dim, const ade::PagedAttnParams& p, int sms, cudaSt
     }
 }
 
+// Rows of a cache layer (page, head, offset) are counted in 32 bits; a cache with more of them would not fit a device.
+bool rows_fit(int pages, int kv_heads, int page_size) { return static_cast<unsigned long long>(pages) * kv_heads <= 0xFFFFFFFFull / page_size; }
+
 }  // namespace
 
 extern "C" {
@@ -120,20 +123,30 @@ int ade_b200_paged_write(const void* k, const void* v, const void* cos_t, const 
     if (!k || !v || !slots || !k_pages || !v_pages || !cos_t != !sin_t) return ADE_ERR_NULL;
     if (T < 1 || kv_heads < 1 || !dim_ok(head_dim) || pages < 1 || page_size < 1) return ADE_ERR_SHAPE;
     if (k_row_stride < 0 || k_head_stride < 0 || v_row_stride < 0 || v_head_stride < 0 || cs_row_stride < 0) return ADE_ERR_SHAPE;
+    if (!rows_fit(pages, kv_heads, page_size)) return ADE_ERR_SHAPE;
     if (!aligned16(k_pages) || !aligned16(v_pages)) return ADE_ERR_ALIGN;
     int sms = 0;
     const int rc = ade_host::sm_count(&sms);
     if (rc) return rc;
     using bf = __nv_bfloat16;
-    ade::WriteParams p = {static_cast<const bf*>(k), static_cast<const bf*>(v), static_cast<const bf*>(cos_t), static_cast<const bf*>(sin_t), slots,
-                          static_cast<bf*>(k_pages), static_cast<bf*>(v_pages), static_cast<long long>(pages) * page_size, k_row_stride, k_head_stride,
-                          v_row_stride, v_head_stride, cs_row_stride, T, kv_heads, head_dim, page_size};
     const bool vec = aligned16(k) && aligned16(v) && (!cos_t || (aligned16(cos_t) && aligned16(sin_t))) &&
                      ((k_row_stride | k_head_stride | v_row_stride | v_head_stride | (cos_t ? cs_row_stride : 0)) & 7) == 0;
-    const long long work = static_cast<long long>(T) * kv_heads * (head_dim / 2 / (vec ? 8 : 1)), want = (work + 255) / 256;
-    const int grid = static_cast<int>(want < 16ll * sms ? want : 16ll * sms);
-    (vec ? ade::paged_write_kernel<true> : ade::paged_write_kernel<false>)<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    return launched();
+    // pieces are counted in 31 bits, with room for a step of the grid behind them
+    const long long per = static_cast<long long>(kv_heads) * (head_dim / 2 / (vec ? 8 : 1)), most = 0x70000000ll / per;
+    if (most < 1) return ADE_ERR_SHAPE;
+    for (long long t0 = 0; t0 < T; t0 += most) {
+        const int rows = static_cast<int>(T - t0 < most ? T - t0 : most);
+        const bf *cs = static_cast<const bf*>(cos_t), *sn = static_cast<const bf*>(sin_t);
+        const ade::WriteParams p = {static_cast<const bf*>(k) + t0 * k_row_stride, static_cast<const bf*>(v) + t0 * v_row_stride,
+                                    cs ? cs + t0 * cs_row_stride : nullptr, sn ? sn + t0 * cs_row_stride : nullptr, slots + t0,
+                                    static_cast<bf*>(k_pages), static_cast<bf*>(v_pages), k_row_stride, k_head_stride, v_row_stride, v_head_stride,
+                                    cs_row_stride, static_cast<uint32_t>(pages) * static_cast<uint32_t>(page_size), rows, kv_heads, head_dim, page_size};
+        const long long want = (rows * per + ade::PW_THREADS - 1) / ade::PW_THREADS;
+        const int grid = static_cast<int>(want < 16ll * sms ? want : 16ll * sms);
+        (vec ? ade::paged_write_kernel<true> : ade::paged_write_kernel<false>)<<<grid, ade::PW_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
+    }
+    return ADE_OK;
 }
 
 size_t ade_b200_paged_attn_workspace_bytes(int T, int q_heads, int kv_heads, int head_dim) {
@@ -152,9 +165,7 @@ int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, con
     if (!work) return ADE_ERR_NULL;
     if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(work)) return ADE_ERR_ALIGN;
     if (work_bytes < ade_b200_paged_attn_workspace_bytes(T, q_heads, kv_heads, head_dim)) return ADE_ERR_SCRATCH;
-    // positions count in 31 bits, rows of the cache in 32
-    if (static_cast<long long>(width) * page_size > 0x7FFFFFFFll || static_cast<unsigned long long>(pages) * kv_heads > 0xFFFFFFFFull / page_size)
-        return ADE_ERR_SHAPE;
+    if (static_cast<long long>(width) * page_size > 0x7FFFFFFFll || !rows_fit(pages, kv_heads, page_size)) return ADE_ERR_SHAPE;
     int sms = 0;
     const int rc = ade_host::sm_count(&sms);
     if (rc) return rc;
