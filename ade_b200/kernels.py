@@ -430,14 +430,16 @@ def bank_deltas(stored_forms) -> dict:
     """Bank of the deltas that several fine-tuned models have on one module, for `multi_delta_forward`.
 
     Parameters:
-        stored_forms: one ``pack_int4`` result per model, all of the same d_o and d_i on one CUDA device; ranks may differ.
+        stored_forms: for each model its ``pack_int4`` result, all of the same d_o and d_i on one device (ranks may differ), or None where
+            a model has no delta on this module.
 
     Returns:
         dict of the tensors of ``struct ade_delta_bank``: the models' rank groups one behind the other, each group's codes of U^
         and of V^^T in one piece (``uq`` (groups, d_o, 64), ``vt`` (groups, 128, d_i / 2)), scales and zero-points beside them,
         ``start`` (models + 1) int32 with the first group of each model, and the ints ``M``, ``N``.  The bank holds copies.
     """
-    forms = list(stored_forms)
+    each = list(stored_forms)
+    forms = [f for f in each if f is not None]
     if not forms:
         raise ValueError("bank_deltas: no deltas given")
     M, N, dev = int(forms[0]["M"]), int(forms[0]["N"]), forms[0]["uq"].device
@@ -446,11 +448,11 @@ def bank_deltas(stored_forms) -> dict:
             raise ValueError("bank_deltas: the deltas must have the same d_o and d_i and be on one device")
         if not GROUP <= int(f["r"]) <= 2048 or int(f["r"]) % GROUP:
             raise ValueError(f"bank_deltas: rank {f['r']} must be a multiple of {GROUP} up to 2048")
-    ng = [int(f["r"]) // GROUP for f in forms]
-    columns = lambda key, *tail: torch.cat([f[key].reshape(M, n, *tail).transpose(0, 1) for f, n in zip(forms, ng)]).contiguous()
-    start = torch.tensor([sum(ng[:i]) for i in range(len(ng) + 1)], dtype=torch.int32)
+    groups = [0 if f is None else int(f["r"]) // GROUP for f in each]
+    columns = lambda key, *tail: torch.cat([f[key].reshape(M, int(f["r"]) // GROUP, *tail).transpose(0, 1) for f in forms]).contiguous()
+    start = torch.tensor([sum(groups[:i]) for i in range(len(groups) + 1)], dtype=torch.int32)
     return {"uq": columns("uq", GROUP // 2), "us": columns("us"), "uz": columns("uz"),
-            "vt": torch.cat([f["vt"].reshape(n, GROUP, N // 2) for f, n in zip(forms, ng)]), "vs": torch.cat([f["vs"] for f in forms]),
+            "vt": torch.cat([f["vt"].reshape(-1, GROUP, N // 2) for f in forms]), "vs": torch.cat([f["vs"] for f in forms]),
             "vz": torch.cat([f["vz"] for f in forms]), "start": start.to(dev), "M": M, "N": N}
 
 

@@ -1,0 +1,217 @@
+"""Many requests at once: modules with a delta for every row's own fine-tuned model, and the decoder on a paged cache, against one
+model per fine-tune run by transformers."""
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from ade_b200 import kernels, synth
+from ade_b200._lib import AdeKernelError
+from ade_b200.batch_serving import BatchDecoder, DeltaRoute, MultiDeltaLinear, attach_multi_deltas
+from ade_b200.serving import LINEAR_MODULE_NAMES, attach_kernel_linears
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+VOCAB = 320
+
+
+def _llama(kv_heads=2):
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    cfg = LlamaConfig(hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=kv_heads, vocab_size=VOCAB,
+                      max_position_embeddings=512)
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(cfg).to(torch.bfloat16).eval()
+    with torch.no_grad():
+        model.lm_head.weight.mul_(20.0)                  # logits that tell tokens apart
+    return model
+
+
+def _deltas(sd, seed, skip=()):
+    per = {}
+    for li in range(2):
+        for i, n in enumerate(LINEAR_MODULE_NAMES):
+            if (li, n) in skip:
+                continue
+            d_o, d_i = sd[f"model.layers.{li}.{n}.weight"].shape
+            p = synth.random_packed(d_o, d_i, 128 * (1 + (i + seed) % 2), seed=100 * seed + 10 * li + i)
+            for k in ("U_scale", "Vt_scale"):
+                p[k] = p[k] * 4.0                         # fine-tunes that differ visibly from the base
+            per[f"model.layers.{li}.{n}"] = p
+    return per
+
+
+@pytest.fixture(scope="module")
+def served():
+    """(base model, [one model per fine-tune], the model that serves all of them)."""
+    base = _llama()
+    sd = {k: v.clone() for k, v in base.state_dict().items()}
+    # the second fine-tune has no delta on two modules, the third none but on one
+    every = [(li, n) for li in range(2) for n in LINEAR_MODULE_NAMES]
+    deltas = [_deltas(sd, 1), _deltas(sd, 2, skip=every[3:5]), _deltas(sd, 3, skip=every[1:])]
+    single = []
+    for per in deltas:
+        m = copy.deepcopy(base)
+        attach_kernel_linears(m, sd, per, device=DEV)
+        single.append(m.to(DEV))
+    many = copy.deepcopy(base)
+    n = attach_multi_deltas(many, sd, deltas, device=DEV)
+    assert n == 14
+    return base.to(DEV), single, many.to(DEV)
+
+
+def test_modules_route_rows_to_their_models():
+    forms = [kernels.pack_int4(synth.random_packed(192, 256, r, seed=r, device=DEV)) for r in (128, 256)]
+    W = synth.base_weight(192, 256, 1).to(DEV)
+    route = DeltaRoute(3)
+    lin = MultiDeltaLinear(W, [forms[0], None, forms[1]], route)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for T in (1, 5, 128, 129, 300):                       # above 128 rows in several launches
+        x = torch.randn(T, 256, generator=g, device=DEV).to(torch.bfloat16)
+        route.ids = None
+        y = lin(x)
+        assert torch.equal(y, F.linear(x, W))
+        ids = torch.randint(-1, 3, (T,), generator=g, device=DEV, dtype=torch.int32)
+        route.ids = ids
+        got = lin(x.view(1, T, 256))
+        assert got.shape == (1, T, 192)
+        for lo in range(0, T, 128):
+            part = slice(lo, min(T, lo + 128))
+            want = kernels.multi_delta_forward(x[part], y[part], lin.bank(), ids[part])
+            assert torch.equal(got[0, part], want)
+        rows = (ids < 0) | (ids == 1)
+        assert torch.equal(got[0][rows], y[rows])
+        route.ids = ids[:-1]
+        if T > 1:
+            with pytest.raises(ValueError, match="route"):
+                lin(x)
+    assert lin(x[:0]).shape == (0, 192)
+    with pytest.raises(ValueError):
+        MultiDeltaLinear(W[:64], forms, route)
+
+
+# Each of the about thirteen tensors that a layer rounds to bfloat16 (projections, rotated queries and keys, attention, products, sums, norms) is off
+# by 2^-8 of its values at most on either side; two layers, the final norm and the logits: 2 * 28 * 2^-8 = 0.22 of the logits' own scale if all
+# errors pointed the same way.  They do not: as a random walk sqrt(2 * 28) * 2^-8 / sqrt(3) = 0.017.  Four times that is asked for.
+WALK = 4 * 0.017
+
+
+def _check_answer(model, tokens, logprobs, prompt_len):
+    """The answer's log probabilities are the model's, and every token is the model's likeliest to within that."""
+    with torch.no_grad():
+        logits = model(input_ids=tokens[None]).logits[0].float()
+    ref = torch.log_softmax(logits, -1)[prompt_len - 1:-1]
+    chosen = ref.gather(1, tokens[prompt_len:, None])[:, 0]
+    tol = WALK * float(logits.std())
+    assert logprobs.shape == chosen.shape
+    assert float((chosen - logprobs).abs().max()) <= 2 * tol, float((chosen - logprobs).abs().max())
+    assert bool((ref.amax(-1) - chosen <= 2 * tol).all())
+
+
+def test_a_ragged_batch_of_many_models_answers_as_each_model_alone(served):
+    base, single, many = served
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (5, 1, 64, 130, 17, 33)]
+    models = [0, 1, 2, 0, -1, 1]
+    dec = BatchDecoder(many, max_requests=8, max_len=160, page_size=16)
+    free = int(dec.free_count)
+    answers = dec.generate(prompts, 20, models)
+    assert int(dec.free_count) == free and int(dec.lengths.abs().sum()) == 0
+    for (tokens, logprobs), p, d in zip(answers, prompts, models):
+        assert torch.equal(tokens[:p.numel()].cpu(), p) and tokens.numel() == p.numel() + 20
+        _check_answer(base if d < 0 else single[d], tokens, logprobs, p.numel())
+    again = dec.generate(prompts, 20, models)             # the captured step, pages and histories are used again
+    for a, b in zip(answers, again):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    # the same requests in another order and company: what a request gets does not depend on the others
+    order = [3, 0, 5, 1]
+    other = dec.generate([prompts[i] for i in order], 20, [models[i] for i in order])
+    for i, (tokens, _) in zip(order, other):
+        _check_answer(base if models[i] < 0 else single[models[i]], tokens, other[order.index(i)][1], prompts[i].numel())
+    # the serving model itself still runs as its base
+    ids = prompts[2][None].to(DEV)
+    with torch.no_grad():
+        assert torch.equal(many(input_ids=ids).logits, base(input_ids=ids).logits)
+
+
+def test_requests_enter_and_leave_between_steps(served):
+    base, single, many = served
+    g = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (9, 30, 3)]
+    dec = BatchDecoder(many, max_requests=2, max_len=64, page_size=8)
+    a = dec.add(prompts[0], 0)
+    for _ in range(5):
+        dec.step()
+    b = dec.add(prompts[1], 1)
+    for _ in range(7):
+        dec.step()
+    assert (a, b) == (0, 1) and dec.lengths.tolist() == [9 + 12, 30 + 7]
+    _check_answer(single[0], dec.tokens[a, :22].clone(), dec.logprobs[a, 9:22].clone(), 9)
+    dec.finish(a)
+    c = dec.add(prompts[2], 2)
+    assert c == a
+    for _ in range(10):
+        dec.step()
+    _check_answer(single[1], dec.tokens[b, :48].clone(), dec.logprobs[b, 30:48].clone(), 30)
+    _check_answer(single[2], dec.tokens[c, :14].clone(), dec.logprobs[c, 3:14].clone(), 3)
+    dec.check_status()
+    dec.finish(b)
+    dec.finish(c)
+    assert int(dec.free_count) == 2 * 8
+    for bad in (lambda: dec.finish(c), lambda: dec.finish(7), lambda: dec.add(prompts[0], 3), lambda: dec.add(torch.zeros(64, dtype=torch.long)),
+                lambda: dec.add(torch.zeros(0, dtype=torch.long)), lambda: dec.generate(prompts, 4), lambda: dec.generate(prompts[:1], 60),
+                lambda: dec.generate(prompts[:2], 3, [0])):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_a_request_that_cannot_grow_is_reported_and_hurts_no_other(served):
+    _, single, many = served
+    g = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (15, 14, 40)]
+    dec = BatchDecoder(many, max_requests=3, max_len=64, pages=3, page_size=16)
+    a, b = dec.add(prompts[0], 0), dec.add(prompts[1], 1)
+    with pytest.raises(AdeKernelError, match="NO_PAGE"):  # 40 tokens on one free page
+        dec.add(prompts[2], 2)
+    for _ in range(8):                                    # one of the two gets the third page, the other waits at 16 tokens
+        dec.step()
+    with pytest.raises(AdeKernelError, match="NO_PAGE"):
+        dec.check_status()
+    first, second = (a, b) if int(dec.lengths[a]) > 16 else (b, a)
+    assert int(dec.lengths[second]) == 16
+    n = 15 if first == a else 14
+    _check_answer(single[0 if first == a else 1], dec.tokens[first, :n + 9].clone(), dec.logprobs[first, n:n + 9].clone(), n)
+    dec.finish(first)                                     # its pages let the other go on
+    for _ in range(6):
+        dec.step()
+    m = 15 if second == a else 14
+    _check_answer(single[0 if second == a else 1], dec.tokens[second, :23].clone(), dec.logprobs[second, m:23].clone(), m)
+
+
+def test_an_end_token_stops_its_request_alone(served):
+    _, _, many = served
+    g = torch.Generator().manual_seed(7)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (6, 11, 4)]
+    dec = BatchDecoder(many, max_requests=3, max_len=64)
+    plain = dec.generate(prompts, 12, [0, 1, 2])
+    eos = int(plain[1][0][11 + 4])
+    stopped = dec.generate(prompts, 12, [0, 1, 2], eos_token_id=eos)
+    for (t, lp), (s, sp), p in zip(plain, stopped, prompts):
+        answer = t[p.numel():].tolist()
+        n = answer.index(eos) + 1 if eos in answer else 12
+        assert s.tolist() == t[:p.numel() + n].tolist() and torch.equal(sp, lp[:n])
+
+
+def test_plain_and_single_delta_models_are_served_too(served):
+    base, single, _ = served
+    g = torch.Generator().manual_seed(8)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (7, 21)]
+    for model in (base, single[0]):
+        for tokens, logprobs in BatchDecoder(model, 4, 48, page_size=32).generate(prompts, 9):
+            _check_answer(model, tokens, logprobs, tokens.numel() - 9)
+    for bad in (lambda: BatchDecoder(torch.nn.Linear(2, 2), 1, 8), lambda: BatchDecoder(_llama(), 1, 8), lambda: BatchDecoder(base, 0, 8), lambda: BatchDecoder(base, 5000, 8)):
+        with pytest.raises(ValueError):
+            bad()
