@@ -197,6 +197,17 @@ __device__ __forceinline__ int md_share(int n, int b) {
     return each * b + min(b, more);
 }
 
+// How many of the ascending sums, times `by`, do not exceed `value`; by the whole warp.
+__device__ __forceinline__ int md_count(const int* sums, int n, int by, int value) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < MD_MAX_ROWS; i += 32) {
+        const int k = i + static_cast<int>(threadIdx.x & 31);
+        c += k < n && sums[k] * by <= value;
+    }
+    return __reduce_add_sync(0xFFFFFFFFu, c);
+}
+
 // ------------------------------------------------------------------ h = V^T x
 // An item is one rank group of one entry over MD_COLS columns: a warp multiplies the group's 128 ranks with 128 columns, eight tiles of 16
 // ranks one behind the other, and the warps' sums are added through shared memory.  Items go entry by entry, slice by slice, group by group, and a
@@ -206,12 +217,7 @@ struct MdVItem {
 };
 
 __device__ __forceinline__ MdVItem md_v_item(const MdEntries& e, int item, int slices) {
-    int lo = 0, hi = e.n - 1;              // first entry with groups_end * slices > item
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (e.groups_end[mid] * slices > item) hi = mid;
-        else lo = mid + 1;
-    }
+    const int lo = md_count(e.groups_end, e.n, slices, item);             // the entry with groups_end * slices > item
     const int rest = item - (e.groups_end[lo] - e.ng[lo]) * slices;
     return {lo, rest / e.ng[lo], rest % e.ng[lo]};
 }
@@ -303,21 +309,35 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
     }
     __syncwarp();                                                     // every lane has read the scales and zero-points
     next.sides(lane);
+    constexpr int PAIR = 2 / NT;                                      // tiles of 16 ranks at a time: two chains of products in flight
 #pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-        md_wait<8>();
-        const uint4 r0 = lds16(next.fifo + (mt * 2) * MD_THREADS * 16), r1 = lds16(next.fifo + (mt * 2 + 1) * MD_THREADS * 16);
-        const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
-        int d[NT][4];
+    for (int m0 = 0; m0 < 8; m0 += PAIR) {
+        md_wait<8 - (PAIR - 1)>();
+        uint4 r0[PAIR], r1[PAIR];
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k) {
+            r0[k] = lds16(next.fifo + ((m0 + k) * 2) * MD_THREADS * 16);
+            r1[k] = lds16(next.fifo + ((m0 + k) * 2 + 1) * MD_THREADS * 16);
+        }
+        int d[PAIR][NT][4];
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) md_mma_word(d[n], w0[w], w1[w], xs[n][2 * w], xs[n][2 * w + 1], w == 0 ? base[n] : d[n]);
-        next.tile(mt);                                                // into the pieces just used
+            for (int k = 0; k < PAIR; ++k) {
+                const uint32_t w0 = w == 0 ? r0[k].x : w == 1 ? r0[k].y : w == 2 ? r0[k].z : r0[k].w;
+                const uint32_t w1 = w == 0 ? r1[k].x : w == 1 ? r1[k].y : w == 2 ? r1[k].z : r1[k].w;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) md_mma_word(d[k][n], w0, w1, xs[n][2 * w], xs[n][2 * w + 1], w == 0 ? base[n] : d[k][n]);
+            }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) part[(n * 4 + tig) * MD_PART + mt * 16 + gid + i * 8] = md_join(d[n][2 * i], d[n][2 * i + 1], weight[n]);
+        for (int k = 0; k < PAIR; ++k) next.tile(m0 + k);             // into the pieces just used
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    part[(n * 4 + tig) * MD_PART + (m0 + k) * 16 + gid + i * 8] = md_join(d[k][n][2 * i], d[k][n][2 * i + 1], weight[n]);
     }
 }
 
@@ -470,12 +490,7 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_u_kernel(const Mult
     };
     // first tile that begins at or behind `cost`
     auto place = [&](int cost) {
-        int lo = 0, hi = e.n;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (e.cost_end[mid] * tiles > cost) hi = mid;
-            else lo = mid + 1;
-        }
+        const int lo = md_count(e.cost_end, e.n, tiles, cost);                   // the entry that ends behind `cost`
         if (lo == e.n) return Place{lo, 0};
         const int before = lo ? e.cost_end[lo - 1] : 0, per = e.cost_end[lo] - before, tile = (cost - before * tiles + per - 1) / per;
         return tile < tiles ? Place{lo, tile} : Place{lo + 1, 0};

@@ -221,7 +221,11 @@ int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_ban
     const int slices = ade::md_slices(d.N);
     ade::multi_delta_v_kernel<<<2 * sms, ade::MD_THREADS, ade::md_v_smem(), st>>>(p, slices);
     if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
-    return launch_early(ade::multi_delta_u_kernel, 2 * sms, ade::MD_THREADS, ade::md_u_smem(), st, p, slices);
+    // One CTA per SM for the second launch where that gives a warp two tiles at most: it is set up beside the first one's CTAs then, instead of behind
+    // them (4096 x 4096, 16 rows of 12 deltas: 14.0 us with two).
+    const long long entries = T < d.deltas + 1 + T / ade::MD_ENTRY ? T : d.deltas + 1 + T / ade::MD_ENTRY;
+    const bool few = entries * ((d.M + ade::MD_TILE - 1) / ade::MD_TILE) <= 2ll * sms * (ade::MD_THREADS / 32);
+    return launch_early(ade::multi_delta_u_kernel, few ? sms : 2 * sms, ade::MD_THREADS, ade::md_u_smem(), st, p, slices);
 }
 
 int ade_b200_token_logprobs(const void* logits, int dtype, const long long* tokens, float* logprobs, float* entropy, float* top_logprobs,
