@@ -40,8 +40,7 @@ constexpr int MD_TILE = 64;                       // rows of U that a warp takes
 constexpr int MD_UDEPTH = 2;                      // steps in the queue of the second launch
 constexpr int MD_STAGE = 36;                      // row pitch of half a tile's results, in floats
 constexpr int MD_SIDE = 224;                      // bytes of a step's scales (nine pieces) and zero-points (five)
-constexpr float kMdMagic = 12582912.f;            // 1.5 * 2^23: an integer below 2^22 added to its bits is added to its value
-constexpr int kMdMagicBits = 0x4B400000;
+constexpr float kMdMagic = 12582912.f;            // 1.5 * 2^23: what is added to it is rounded to an integer, in the lower bits of the sum
 
 struct MultiDeltaParams {
     const __nv_bfloat16 *x, *y;           // [T][N], [T][M]
@@ -105,11 +104,8 @@ __device__ __forceinline__ float md_max(float a, float b) {              // NaN 
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// What the integers of upper and lower bytes, given as the bits of kMdMagic plus each, come to; `unit` is a power of two, so only the sum is rounded.
-__device__ __forceinline__ float md_join(int up, int lo, float unit) {
-    const float u = unit * 256.f;
-    return fmaf(__int_as_float(up), u, -kMdMagic * u) + fmaf(__int_as_float(lo), unit, -kMdMagic * unit);
-}
+// What the sums of upper and lower bytes come to: their integer is exact, below 2^26, and rounded once.
+__device__ __forceinline__ float md_join(int up, int lo, float unit) { return static_cast<float>(up * 256 + lo) * unit; }
 // Fixed point for values of magnitude up to m: v * scale is at most 32637, so its upper and lower eight bits are signed bytes; `unit` = 1 / scale, a
 // power of two (infinite or NaN where m is, so that results show it).
 struct MdFixed {
@@ -270,7 +266,7 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
     // x vs of row gid / 2 at this lane's 32 columns: the largest of the row's 128, then the upper (gid even) or lower bytes of the fixed-point values
     uint32_t xs[NT][8];
     float weight[NT];                                                 // what an integer of lower bytes counts for row tig
-    int base[NT][4];                                                  // the float bits of an integer, less the zero-points' part
+    int base[NT][4];                                                  // what the sums begin with: the zero-points' part off
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         float m = 0.f;
@@ -305,7 +301,7 @@ __device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const Md
 #pragma unroll
         for (int i = 0; i < 4; ++i) md_mma(zero, z[2 * i], z[2 * i], z[2 * i + 1], z[2 * i + 1], xs[n][2 * i], xs[n][2 * i + 1], zero);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) base[n][i] = kMdMagicBits - zero[i];
+        for (int i = 0; i < 4; ++i) base[n][i] = -zero[i];
     }
     __syncwarp();                                                     // every lane has read the scales and zero-points
     next.sides(lane);
@@ -421,7 +417,7 @@ template <int NT, typename Refill>
 __device__ __forceinline__ void md_u_step(uint32_t codes, const uint8_t* hcol, const float2* hsum, int j, const float (&us)[2], const float (&usz)[2],
                                           float (&acc)[NT][8], Refill refill) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-    int base[4] = {kMdMagicBits, kMdMagicBits, kMdMagicBits, kMdMagicBits};
+    int base[4] = {0, 0, 0, 0};
     uint4 b[NT][2];
     float2 s[NT];
 #pragma unroll
