@@ -241,17 +241,22 @@ struct MdVCopy {
     }
 };
 
-template <int NT>
-__device__ __forceinline__ void md_v_compute(const MultiDeltaParams& p, const MdEntries& e, const MdVItem& it, int cb, float* part, const MdVCopy& next) {
+// x of the entry's rows gid / 2 and gid / 2 + 4 at this lane's 32 columns, asked for an item ahead
+__device__ __forceinline__ void md_v_x(const MultiDeltaParams& p, const MdEntries& e, const MdVItem& it, int cb, uint4 (&xv)[2][4]) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-    uint4 xv[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < 2; ++n) {
         const int r = n * 4 + (gid >> 1);
-        const uint4* xp = reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(e.row[it.e][r < e.rows[it.e] ? r : 0]) * p.N + cb * 128 + tig * 32);
+        const bool on = r < e.rows[it.e];
+        const uint4* xp = reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(e.row[it.e][on ? r : 0]) * p.N + cb * 128 + tig * 32);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[n][i] = r < e.rows[it.e] ? ldg16(xp + i) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 4; ++i) xv[n][i] = on ? ldg16(xp + i) : make_uint4(0u, 0u, 0u, 0u);
     }
+}
+
+template <int NT>
+__device__ __forceinline__ void md_v_compute(const uint4 (&xv)[2][4], float* part, const MdVCopy& next) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     md_wait<8>();                                                     // the scales and zero-points are there; the tiles may be under way
     __syncwarp();
     uint32_t z[8];                                                    // zero-points in the order of the codes' bytes
@@ -361,11 +366,13 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_v_kernel(const Mult
         return c;
     };
     MdVItem it = md_v_item(e, item, slices);
+    uint4 xv[2][4];
     {
         const MdVCopy c = copy(it, true);
         c.sides(lane);
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) c.tile(mt);
+        if (c.codes) md_v_x(p, e, it, it.slice * (MD_COLS / 128) + warp, xv);
     }
     while (true) {
         MdVItem nx = it;
@@ -383,19 +390,21 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_v_kernel(const Mult
         const int cb = it.slice * (MD_COLS / 128) + warp, rows = e.rows[it.e];
         if (cb < blocks) {
             float* mine = part + warp * (MD_ENTRY * MD_PART);
-            if (rows <= 4) md_v_compute<1>(p, e, it, cb, mine, next);
-            else md_v_compute<2>(p, e, it, cb, mine, next);
+            if (rows <= 4) md_v_compute<1>(xv, mine, next);
+            else md_v_compute<2>(xv, mine, next);
         } else {
             next.sides(lane);
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) next.tile(mt);
         }
+        if (next.codes) md_v_x(p, e, nx, nx.slice * (MD_COLS / 128) + warp, xv);
         __syncthreads();
         const int warps = min(8, blocks - it.slice * (MD_COLS / 128));
         for (int i = tid; i < rows * 128; i += MD_THREADS) {
             const int r = i >> 7, k = i & 127;
             float s = 0.f;
-            for (int w = 0; w < warps; ++w) s += part[(w * MD_ENTRY + r) * MD_PART + k];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) s += w < warps ? part[(w * MD_ENTRY + r) * MD_PART + k] : 0.f;
             p.h[(static_cast<size_t>(it.slice) * p.T + e.row[it.e][r]) * MD_H + it.j * 128 + k] = s;
         }
         if (!go_on) return;

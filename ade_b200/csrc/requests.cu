@@ -203,7 +203,9 @@ int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_ban
     if (!x || !y_dense || !bank || !ids || !out) return ADE_ERR_NULL;
     const ade_delta_bank_t& d = *bank;
     if (!d.uq || !d.us || !d.uz || !d.vt || !d.vs || !d.vz || !d.start) return ADE_ERR_NULL;
-    if (T < 1 || T > ADE_B200_MAX_TOKENS || d.M < 1 || d.M > (1 << 21) || d.N < 128 || d.N % 128 || d.groups < 1 || d.deltas < 1) return ADE_ERR_SHAPE;
+    if (T < 1 || T > ADE_B200_MAX_TOKENS || d.M < 1 || d.M > (1 << 21) || d.N < 128 || d.N > (1 << 21) || d.N % 128 || d.groups < 1 || d.deltas < 1)
+        return ADE_ERR_SHAPE;
+    if (static_cast<unsigned long long>(d.groups) * d.M > 0xFFFFFFFFull) return ADE_ERR_SHAPE;          // rows of U are counted in 32 bits
     if (!work) return ADE_ERR_NULL;
     const void* all[] = {x, y_dense, out, work, d.uq, d.us, d.uz, d.vt, d.vs, d.vz};
     for (const void* a : all)

@@ -319,8 +319,11 @@ def test_attention_takes_strided_queries():
 
 # ------------------------------------------------------------------------------------ multi_delta_forward
 def _delta64(x, y, packed, ids):
-    """y + U (V x) in float64 from the unpacked codes, and the magnitudes that roundings on the way are relative to."""
-    out, mag = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64, device=DEV)
+    """y + U (V x) in float64 from the unpacked codes, and how far off the operands' fixed point may put it.
+
+    x vs is held, for each row, rank group and 128 columns, to half a unit of a grid with at least 2^14 units to the largest of the 128 (less
+    0.4 %): off by 1.004 2^-15 of it.  h is held the same way for each row and group of 128 ranks.  A code less its zero-point is at most 15."""
+    out, off, mag = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64, device=DEV), torch.zeros(y.shape, dtype=torch.float64, device=DEV)
     for t, d in enumerate(ids):
         if not 0 <= d < len(packed):
             continue
@@ -328,11 +331,13 @@ def _delta64(x, y, packed, ids):
         U = (p["U_codes"] - p["U_zero"].repeat_interleave(128, 1)) * p["U_scale"].repeat_interleave(128, 1)
         V = (p["Vt_codes"] - p["Vt_zero"].repeat_interleave(128, 0)) * p["Vt_scale"].repeat_interleave(128, 0)
         h = V @ x[t].double()
-        # codes without their zero-point, up to 15, stand for what is added before the zero-points' part is taken off again
-        habs = (15 * p["Vt_scale"].repeat_interleave(128, 0)) @ x[t].double().abs()
         out[t] += U @ h
-        mag[t] = (15 * p["U_scale"].repeat_interleave(128, 1)) @ habs
-    return out, mag
+        largest = (x[t].double() * p["Vt_scale"]).abs().view(p["Vt_scale"].shape[0], -1, 128).amax(-1)      # (rank group, 128 columns)
+        habs = 15 * 128 * largest.sum(-1)                                                                 # of any rank of the group
+        hmax = h.abs().view(-1, 128).amax(-1)
+        off[t] = 1.004 * 2.0 ** -15 * (15 * 128 * p["U_scale"]) @ (habs + hmax)
+        mag[t] = (15 * 128 * p["U_scale"]) @ habs
+    return out, off, mag
 
 
 def _check_delta(M, N, ranks, ids, seed):
@@ -344,9 +349,9 @@ def _check_delta(M, N, ranks, ids, seed):
     y = torch.randn(T, M, generator=g, device=DEV).to(torch.bfloat16)
     y *= 0.02                                                          # the delta is a visible part of the result
     got = multi_delta_forward(x, y, bank, _i32(ids))
-    want, mag = _delta64(x, y, packed, ids)
-    # Products are formed from operands held to 2^-16 (two bfloat16 parts) or exactly, sums are float32 (N, then rank terms), one rounding at the end.
-    e = mag * (2 * 2.0 ** -16 + (N + max(ranks)) * 2.0 ** -24)
+    want, off, mag = _delta64(x, y, packed, ids)
+    # integers are exact; what they come to is added in float32 (N / 128 terms and the rank groups', none more than mag), one rounding at the end
+    e = off + mag * (N / 128 + 16) * 2.0 ** -24
     off = (got.double() - want).abs()
     assert bool((off <= 2.0 ** -8 * (want.abs() + e) + e).all()), float((off / (2.0 ** -8 * want.abs() + e).clamp(min=1e-30)).max())
     # the typical error is that of the last rounding alone: a uniform error of half a step has a root mean square of 2^-8 / sqrt(3) of a value
@@ -380,6 +385,36 @@ def test_rows_of_one_delta_match_the_single_delta_path():
         rows = torch.tensor([t for t, i in enumerate(ids) if i == d], device=DEV)
         want = kernels.decode_forward_packed(x[rows].contiguous(), y[rows].contiguous(), f)
         assert float((got[rows].float() - want.float()).norm() / want.float().norm()) < 1e-2
+
+
+def test_values_that_are_no_numbers_stay_in_their_row():
+    """NaN, infinities, zeros and tiny values in rows of one delta: each row gives what it gives alone."""
+    forms = [kernels.pack_int4(synth.random_packed(200, 384, 256, seed=5, device=DEV))]
+    bank = bank_deltas(forms)
+    g = _gen(4)
+    x = torch.randn(9, 384, generator=g, device=DEV).to(torch.bfloat16)
+    y = torch.zeros(9, 200, dtype=torch.bfloat16, device=DEV)
+    x[1, 7], x[3, 300], x[4, 1], x[5], x[6] = float("nan"), float("inf"), float("-inf"), 0.0, 1e-30
+    got = multi_delta_forward(x, y, bank, _i32([0] * 9))
+    for t in range(9):
+        alone = multi_delta_forward(x[t:t + 1].contiguous(), y[:1], bank, _i32([0]))
+        assert torch.equal(got[t].nan_to_num(7.0), alone[0].nan_to_num(7.0)) and torch.equal(torch.isnan(got[t]), torch.isnan(alone[0]))
+    assert not bool(torch.isfinite(got[[1, 3, 4]]).any()) and bool((got[5] == 0).all()) and bool(torch.isfinite(got[[0, 2, 5, 6, 7, 8]]).all())
+
+
+def test_the_output_may_be_the_shared_term_itself():
+    import ctypes
+
+    from ade_b200 import _lib
+
+    x, y, bank, want = _check_delta(129, 256, [256, 128], [0, 1, -1, 0], seed=31)
+    lib, ids = _lib.load(), _i32([0, 1, -1, 0])
+    b = _lib.AdeDeltaBank(*[bank[k].data_ptr() for k in kernels.BANK_KEYS], 129, 256, bank["uq"].shape[0], 2)
+    work = torch.empty(lib.ade_b200_multi_delta_workspace_bytes(4, 256), dtype=torch.uint8, device=DEV)
+    out = y.clone()
+    assert lib.ade_b200_multi_delta(x.data_ptr(), out.data_ptr(), ctypes.byref(b), ids.data_ptr(), out.data_ptr(), work.data_ptr(), work.numel(), 4,
+                                    torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, want)
 
 
 def test_delta_ids_are_read_when_the_graph_runs():

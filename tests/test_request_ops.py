@@ -62,7 +62,8 @@ def _logprobs(**kw):
     (lambda: _attn(hq=3), SHAPE), (lambda: _attn(hk=0), SHAPE), (lambda: _attn(dim=100), SHAPE), (lambda: _attn(stride=3), SHAPE),
     (lambda: _attn(kp=P + 8), ALIGN), (lambda: _attn(out=P + 2), ALIGN), (lambda: _attn(work_bytes=0), SCRATCH),
     (lambda: _delta(x=None), NULL), (lambda: _delta(_bank(vt=None)), NULL), (lambda: _delta(T=0), SHAPE), (lambda: _delta(T=129), SHAPE),
-    (lambda: _delta(_bank(N=192)), SHAPE), (lambda: _delta(_bank(groups=0)), SHAPE), (lambda: _delta(_bank(deltas=0)), SHAPE),
+    (lambda: _delta(_bank(N=192)), SHAPE), (lambda: _delta(_bank(M=(1 << 21) + 1)), SHAPE), (lambda: _delta(_bank(N=1 << 22)), SHAPE),
+    (lambda: _delta(_bank(M=1 << 21, groups=1 << 12)), SHAPE), (lambda: _delta(_bank(groups=0)), SHAPE), (lambda: _delta(_bank(deltas=0)), SHAPE),
     (lambda: _delta(_bank(uq=P + 4)), ALIGN), (lambda: _delta(y=P + 2), ALIGN), (lambda: _delta(work_bytes=16), SCRATCH),
     (lambda: _logprobs(x=None), NULL), (lambda: _logprobs(logp=None), NULL), (lambda: _logprobs(tokens=None), NULL), (lambda: _logprobs(top_tok=None), NULL),
     (lambda: _logprobs(rows=0), SHAPE), (lambda: _logprobs(vocab=0), SHAPE), (lambda: _logprobs(top=33), SHAPE), (lambda: _logprobs(top=-1), SHAPE),
