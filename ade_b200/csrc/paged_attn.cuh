@@ -37,6 +37,7 @@ struct PagedAttnParams {
     long long table_stride, q_row, q_head, cs_row;
     int T, B, width, pages, page_size, q_heads, kv_heads;
     float scale2;                              // scale * log2(e)
+    uint32_t page_mul, page_shift;             // n / page_size = (mulhi(n, page_mul) + n) >> page_shift for n below 2^31
     bool pairs;                                // q, cs and sn begin every row and head at an even element of 4-byte aligned memory
 };
 
@@ -213,9 +214,9 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
         Look l = {ahead.at < f_end, -1, 0, 0};
         if (l.on) {
             const int pos = ahead.tile * PA_TILE + (lane & 15);
-            l.kvh = ahead.pair / sets;
+            l.kvh = sets == 1 ? ahead.pair : ahead.pair / sets;
             if (pos < rown[ahead.t]) {
-                const int col = pos / p.page_size;
+                const int col = static_cast<int>((__umulhi(static_cast<uint32_t>(pos), p.page_mul) + static_cast<uint32_t>(pos)) >> p.page_shift);
                 l.off = pos - col * p.page_size;
                 l.page = p.table[rowreq[ahead.t] * p.table_stride + col];
             }
@@ -251,8 +252,8 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
     bool fresh = true, from_start = false;
     int stage = 0, fill = S::kStages - 1;
     const int pair_heads = min(PA_HEADS, group);
-    auto heads_of = [&](int pair) { return min(pair_heads, group - pair % sets * PA_HEADS); };
-    auto first_head = [&](int pair) { return pair / sets * group + pair % sets * PA_HEADS; };
+    auto heads_of = [&](int pair) { return sets == 1 ? group : min(pair_heads, group - pair % sets * PA_HEADS); };
+    auto first_head = [&](int pair) { return sets == 1 ? pair * group : pair / sets * group + pair % sets * PA_HEADS; };
     if (!any && !merged && lane < PA_HEADS) p.stat[(wid * 2) * PA_HEADS + lane] = make_float2(-INFINITY, 0.f);   // a warp without tiles
     // Queries of a pair, heads by lanes (gid): dimensions d and d + HD / 2, d + 1 beside each, and the angles they are rotated by.
     uint32_t raw[KS / 2][2][6];
@@ -475,26 +476,39 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const PagedAttnPar
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (h < heads) {
+        // the largest maximum, and a part's sum relative to it; the weighted sums do not wait for either.  A part of no positions (its maximum is
+        // -inf) has no weighted sum: what is read there is not used.
         float mm = -INFINITY;
         for (int i = lane; i < n; i += 32) mm = fmaxf(mm, p.stat[slot(i) * PA_HEADS + h].x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
-#pragma unroll 8
-        for (int i = part; i < n; i += share) {
-            const int s = slot(i);
-            const float2 st = p.stat[s * PA_HEADS + h];
-            const bool on = st.x != -INFINITY;
-            const float fac = on ? exp2f(st.x - mm) : 0.f;
-            den += on ? fac * st.y : 0.f;
+        constexpr int U = V == 1 ? 8 : 4;
+        for (int i0 = part; i0 < n; i0 += U * share) {
+            float2 st[U];
+            float4 a[U][V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int d = lane * 4 + v * 128;
-                if (d < HD && on) {
-                    const float4 a = *reinterpret_cast<const float4*>(p.part + (static_cast<size_t>(s) * PA_HEADS + h) * HD + d);
-                    acc[v].x += fac * a.x;
-                    acc[v].y += fac * a.y;
-                    acc[v].z += fac * a.z;
-                    acc[v].w += fac * a.w;
+            for (int u = 0; u < U; ++u) {
+                st[u] = make_float2(-INFINITY, 0.f);
+                if (i0 + u * share < n) {
+                    const int s = slot(i0 + u * share);
+                    st[u] = p.stat[s * PA_HEADS + h];
+#pragma unroll
+                    for (int v = 0; v < V; ++v)
+                        if (lane * 4 + v * 128 < HD)
+                            a[u][v] = *reinterpret_cast<const float4*>(p.part + (static_cast<size_t>(s) * PA_HEADS + h) * HD + lane * 4 + v * 128);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (st[u].x == -INFINITY) continue;
+                const float fac = exp2f(st[u].x - mm);
+                den += fac * st[u].y;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    acc[v].x += fac * a[u][v].x;
+                    acc[v].y += fac * a[u][v].y;
+                    acc[v].z += fac * a[u][v].z;
+                    acc[v].w += fac * a[u][v].w;
                 }
             }
         }

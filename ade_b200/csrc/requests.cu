@@ -175,6 +175,10 @@ int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, con
     int4* meta = reinterpret_cast<int4*>(stat + kAttnWarps * 2 * ade::PA_HEADS);
     const bool pairs = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cos_t) | reinterpret_cast<uintptr_t>(sin_t)) & 3) == 0 &&
                        ((q_row_stride | q_head_stride | (cos_t ? cs_row_stride : 0)) & 1) == 0;
+    // division by page_size as a multiplication: the shift is its logarithm rounded up, the factor 2^32 (2^shift - page_size) / page_size + 1
+    uint32_t page_shift = 0;
+    while ((1ull << page_shift) < static_cast<unsigned long long>(page_size)) ++page_shift;
+    const uint32_t page_mul = static_cast<uint32_t>((((1ull << page_shift) - page_size) << 32) / page_size + 1);
     // rows of one launch: PA_MAX_ROWS, fewer where the places of that many full rows would not fit 31 bits
     const long long heads = static_cast<long long>(kv_heads) * ((q_heads / kv_heads + ade::PA_HEADS - 1) / ade::PA_HEADS);
     const long long fit = 0x7FFFFFFFll / (heads * (static_cast<long long>(width) * page_size / ade::PA_TILE + 1 + ade::PA_GAP));
@@ -187,7 +191,7 @@ int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, con
                                         sn ? sn + o * cs_row_stride : nullptr, block_table, requests + o, positions + o, static_cast<const bf*>(k_pages),
                                         static_cast<const bf*>(v_pages), static_cast<bf*>(out) + o * q_heads * head_dim, part, stat, meta,
                                         table_row_stride, q_row_stride, q_head_stride, cs_row_stride, T - t0 < chunk ? T - t0 : chunk, B,
-                                        width, pages, page_size, q_heads, kv_heads, scale * 1.44269504088896340736f, pairs};
+                                        width, pages, page_size, q_heads, kv_heads, scale * 1.44269504088896340736f, page_mul, page_shift, pairs};
         const int rc_launch = launch_attn_dim(head_dim, p, sms, static_cast<cudaStream_t>(stream));
         if (rc_launch) return rc_launch;
     }
