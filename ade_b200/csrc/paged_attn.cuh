@@ -7,7 +7,7 @@
 // rounding left over, so queries and probabilities enter with 16 bits of mantissa at no cost (one to eight heads leave those rows
 // free) and the two halves of a result are added in float32.  The running maximum and sum of the softmax stay in registers.
 //
-// The cache is cut into tiles of 16 positions; the tiles of all pairs, one pair behind the other, are shared out evenly over the
+// The cache is cut into tiles of 16 positions (32 up to 64 dimensions); the tiles of all pairs, one pair behind the other, are shared out evenly over the
 // CTAs and there over the warps, whatever the lengths.  On that line of tiles every pair has PA_GAP places more in front of its tiles, for what
 // a pair costs besides them (its queries, its result): without them the warps that meet the short pairs of a ragged batch end last.  A warp streams its tiles through cp.async stages of its own and never waits
 // for another; what it has of a pair that others share goes to the workspace as (maximum, sum, weighted sum), and a second
@@ -21,7 +21,6 @@ namespace ade {
 constexpr int PA_MAX_CTAS = 160;           // one CTA per SM; bounds the workspace
 constexpr int PA_MAX_ROWS = 1024;          // rows of one launch (their prefix sums lie in shared memory); the places of a launch fit 31 bits
 constexpr int PA_HEADS = 8;                // query heads that share one pass over the keys and values
-constexpr int PA_TILE = 16;                // positions of a tile
 constexpr int PA_GAP = 3;                  // places of the line in front of a pair's tiles (0: 119 us, 2: 80.8, 3: 80.4, 5: 81.7 with 32 rows of 16 to 4000 positions)
 
 struct PagedAttnParams {
@@ -44,8 +43,9 @@ struct PagedAttnParams {
 template <int HD>
 struct PaShape {
     static constexpr int kWarps = HD <= 128 ? 8 : 4;
+    static constexpr int kTile = HD <= 64 ? 32 : 16;                     // positions of a tile, 8 KB of a cache of 64 or 128 dimensions
     static constexpr int kChunks = HD / 8;                               // 16-byte pieces of a row
-    static constexpr int kTileBytes = PA_TILE * HD * 2;
+    static constexpr int kTileBytes = kTile * HD * 2;
     static constexpr int kStages = 192 * 1024 / (kWarps * 2 * kTileBytes) < 8 ? 192 * 1024 / (kWarps * 2 * kTileBytes) : 8;
     static constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * 2 * kTileBytes;
     // where piece c of row r lies in a tile: the eight rows that a matrix load reads at one piece are spread over the banks
@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t pa_split(float a, float b, uint32_t& rest) {
 template <int HD>
 __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel(const PagedAttnParams p) {
     using S = PaShape<HD>;
-    constexpr int KS = HD / 16, NW = S::kWarps, NT = NW * 32;
+    constexpr int KS = HD / 16, NW = S::kWarps, NT = NW * 32, TILE = S::kTile;
     extern __shared__ __align__(128) uint8_t pa_smem[];
     float2* mstat = reinterpret_cast<float2*>(pa_smem + S::kRing);                 // [NW][PA_HEADS]
     uint32_t* masks = reinterpret_cast<uint32_t*>(mstat + NW * PA_HEADS);          // [NW][stages] positions of a tile that count
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
     const int group = p.q_heads / p.kv_heads, sets = (group + PA_HEADS - 1) / PA_HEADS, H = p.kv_heads * sets;
 
     // places of every row, summed, the longest row and the rows that have any
-    auto places = [](int n) { return n ? (n + PA_TILE - 1) / PA_TILE + PA_GAP : 0; };              // of one pair
+    auto places = [](int n) { return n ? (n + TILE - 1) / TILE + PA_GAP : 0; };              // of one pair
     const int per = (p.T + NT - 1) / NT, ta = min(tid * per, p.T), tb = min(ta + per, p.T);
     int mine = 0, longest = 0, live = 0;
     for (int t = ta; t < tb; ++t) {
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
     auto look = [&] {
         Look l = {ahead.at < f_end, -1, 0, 0};
         if (l.on) {
-            const int pos = ahead.tile * PA_TILE + (lane & 15);
+            const int pos = ahead.tile * TILE + (lane & (TILE - 1));
             l.kvh = sets == 1 ? ahead.pair : ahead.pair / sets;
             if (pos < rown[ahead.t]) {
                 const int col = static_cast<int>((__umulhi(static_cast<uint32_t>(pos), p.page_mul) + static_cast<uint32_t>(pos)) >> p.page_shift);
@@ -227,12 +227,12 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
     auto issue = [&](int stage, const Look& l) {
         const bool ok = l.page >= 0 && l.page < p.pages;
         const uint32_t row = ok ? (static_cast<uint32_t>(l.page) * p.kv_heads + l.kvh) * p.page_size + l.off : 0u;
-        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok) & 0xFFFFu;
+        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok) & (TILE == 32 ? 0xFFFFFFFFu : 0xFFFFu);
         if (lane == 0) mk[stage] = mask;
         const uint32_t dst = ring + static_cast<uint32_t>(stage) * (2 * S::kTileBytes);
         if (l.on) {
 #pragma unroll
-            for (int j = 0; j < S::kChunks / 2; ++j) {
+            for (int j = 0; j < S::kChunks * TILE / 32; ++j) {
                 const int i = j * 32 + lane, r = i / S::kChunks, c = i - r * S::kChunks;
                 const size_t at = static_cast<size_t>(__shfl_sync(0xFFFFFFFFu, row, r)) * HD + c * 8;
                 const bool live = mask >> r & 1u;
@@ -255,9 +255,9 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
     auto heads_of = [&](int pair) { return sets == 1 ? group : min(pair_heads, group - pair % sets * PA_HEADS); };
     auto first_head = [&](int pair) { return sets == 1 ? pair * group : pair / sets * group + pair % sets * PA_HEADS; };
     if (!any && !merged && lane < PA_HEADS) p.stat[(wid * 2) * PA_HEADS + lane] = make_float2(-INFINITY, 0.f);   // a warp without tiles
-    // Queries of a pair, heads by lanes (gid): dimensions d and d + HD / 2, d + 1 beside each, and the angles they are rotated by.
-    uint32_t raw[KS / 2][2][6];
-    auto ask = [&](const Cursor& c) {
+    // Queries of a pair, heads by lanes (gid): dimensions d and d + HD / 2, d + 1 beside each, and the angles they are rotated by, for step ks of
+    // the first half.
+    auto ask = [&](const Cursor& c, int ks, uint32_t (&raw)[2][6]) {
         const bool on = gid < heads_of(c.pair);
         const __nv_bfloat16* qr = p.q + c.t * p.q_row + (first_head(c.pair) + (on ? gid : 0)) * p.q_head;
         // two neighbours at once where every row begins at an even element
@@ -265,45 +265,65 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
             return p.pairs ? *reinterpret_cast<const uint32_t*>(a) : static_cast<uint32_t>(__bfloat16_as_ushort(a[0])) | static_cast<uint32_t>(__bfloat16_as_ushort(a[1])) << 16;
         };
 #pragma unroll
-        for (int ks = 0; ks < KS / 2; ++ks)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int d = ks * 16 + tig * 2 + i * 8;
-                uint32_t(&r)[6] = raw[ks][i];
-                r[0] = on ? two(qr + d) : 0u;
-                r[1] = on ? two(qr + d + HD / 2) : 0u;
-                if (p.cs) {
-                    const __nv_bfloat16 *cr = p.cs + c.t * p.cs_row + d, *sr = p.sn + c.t * p.cs_row + d;
-                    r[2] = two(cr);
-                    r[3] = two(cr + HD / 2);
-                    r[4] = two(sr);
-                    r[5] = two(sr + HD / 2);
-                }
+        for (int i = 0; i < 2; ++i) {
+            const int d = ks * 16 + tig * 2 + i * 8;
+            uint32_t(&r)[6] = raw[i];
+            r[0] = on ? two(qr + d) : 0u;
+            r[1] = on ? two(qr + d + HD / 2) : 0u;
+            if (p.cs) {
+                const __nv_bfloat16 *cr = p.cs + c.t * p.cs_row + d, *sr = p.sn + c.t * p.cs_row + d;
+                r[2] = two(cr);
+                r[3] = two(cr + HD / 2);
+                r[4] = two(sr);
+                r[5] = two(sr + HD / 2);
             }
+        }
     };
-    auto rotate = [&] {                                                 // rotated, in two bfloat16 parts
+    auto rotate = [&](int ks, const uint32_t (&raw)[2][6]) {            // rotated, in two bfloat16 parts
 #pragma unroll
-        for (int ks = 0; ks < KS / 2; ++ks)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t(&r)[6] = raw[ks][i];
-                float a0 = bf_lo(r[0]), a1 = bf_hi(r[0]), b0 = bf_lo(r[1]), b1 = bf_hi(r[1]);
-                if (p.cs) {
-                    const float x0 = a0, x1 = a1;
-                    a0 = x0 * bf_lo(r[2]) - b0 * bf_lo(r[4]);
-                    a1 = x1 * bf_hi(r[2]) - b1 * bf_hi(r[4]);
-                    b0 = b0 * bf_lo(r[3]) + x0 * bf_lo(r[5]);
-                    b1 = b1 * bf_hi(r[3]) + x1 * bf_hi(r[5]);
-                }
-                qa[ks][2 * i] = pa_split(a0, a1, qa[ks][2 * i + 1]);
-                qa[ks + KS / 2][2 * i] = pa_split(b0, b1, qa[ks + KS / 2][2 * i + 1]);
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t(&r)[6] = raw[i];
+            float a0 = bf_lo(r[0]), a1 = bf_hi(r[0]), b0 = bf_lo(r[1]), b1 = bf_hi(r[1]);
+            if (p.cs) {
+                const float x0 = a0, x1 = a1;
+                a0 = x0 * bf_lo(r[2]) - b0 * bf_lo(r[4]);
+                a1 = x1 * bf_hi(r[2]) - b1 * bf_hi(r[4]);
+                b0 = b0 * bf_lo(r[3]) + x0 * bf_lo(r[5]);
+                b1 = b1 * bf_hi(r[3]) + x1 * bf_hi(r[5]);
             }
+            qa[ks][2 * i] = pa_split(a0, a1, qa[ks][2 * i + 1]);
+            qa[ks + KS / 2][2 * i] = pa_split(b0, b1, qa[ks + KS / 2][2 * i + 1]);
+        }
     };
-    if (any) ask(cur);
+    auto queries = [&](const Cursor& c) {
+        constexpr int B = KS / 2 < 4 ? KS / 2 : 4;                      // steps under way at once, as registers allow
 #pragma unroll
-    for (int s = 0; s < S::kStages - 1; ++s) issue(s, seen[s]);
+        for (int k0 = 0; k0 < KS / 2; k0 += B) {
+            uint32_t raw[B][2][6];
+#pragma unroll
+            for (int k = 0; k < B; ++k)
+                if (k0 + k < KS / 2) ask(c, k0 + k, raw[k]);
+#pragma unroll
+            for (int k = 0; k < B; ++k)
+                if (k0 + k < KS / 2) rotate(k0 + k, raw[k]);
+        }
+    };
+    if constexpr (HD <= 128) {                                          // asked for in front of the first tiles
+        uint32_t raw[KS / 2][2][6];
+        if (any)
+#pragma unroll
+            for (int ks = 0; ks < KS / 2; ++ks) ask(cur, ks, raw[ks]);
+#pragma unroll
+        for (int s = 0; s < S::kStages - 1; ++s) issue(s, seen[s]);
+        if (any)
+#pragma unroll
+            for (int ks = 0; ks < KS / 2; ++ks) rotate(ks, raw[ks]);
+    } else {
+#pragma unroll
+        for (int s = 0; s < S::kStages - 1; ++s) issue(s, seen[s]);
+        if (any) queries(cur);
+    }
     Look next = seen[S::kStages - 1];
-    if (any) rotate();
     bool have = true;
 #pragma unroll 1
     while (cur.at < f_end) {
@@ -314,10 +334,7 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
             l = 0.f;
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-            if (!have) {
-                ask(cur);
-                rotate();
-            }
+            if (!have) queries(cur);
             have = false;
         }
         pa_cp_wait<S::kStages - 2>();
@@ -327,21 +344,25 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
         const uint32_t mask = mk[stage];
         if (mask) {
             const uint32_t kt = ring + static_cast<uint32_t>(stage) * (2 * S::kTileBytes), vt = kt + S::kTileBytes;
-            float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint32_t b[4];
-                pa_ldm4(kt + S::at((lane >> 4) * 8 + (lane & 7), 2 * ks + (lane >> 3 & 1)), b);
-                mma_bf16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
-                mma_bf16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
-            }
-            // head gid at positions 2 tig, 2 tig + 1 and the same + 8
-            float w[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+            // head gid at positions 8 j + 2 tig and the one behind it, j = 0 .. TILE / 8 - 1
+            float w[TILE / 4];
             float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = mask >> (tig * 2 + (i & 1) + (i >> 1) * 8) & 1u ? w[i] * p.scale2 : -INFINITY;
-                mx = fmaxf(mx, w[i]);
+            for (int t = 0; t < TILE / 16; ++t) {
+                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    uint32_t b[4];
+                    pa_ldm4(kt + S::at(t * 16 + (lane >> 4) * 8 + (lane & 7), 2 * ks + (lane >> 3 & 1)), b);
+                    mma_bf16(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
+                    mma_bf16(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
+                }
+                const float v[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[t * 4 + i] = mask >> (t * 16 + tig * 2 + (i & 1) + (i >> 1) * 8) & 1u ? v[i] * p.scale2 : -INFINITY;
+                    mx = fmaxf(mx, w[t * 4 + i]);
+                }
             }
             mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
@@ -358,19 +379,22 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < TILE / 4; ++i) {
                 w[i] = exp2f(w[i] - m);
                 l += w[i];
             }
-            uint32_t pa[4];
-            pa[0] = pa_split(w[0], w[1], pa[1]);
-            pa[2] = pa_split(w[2], w[3], pa[3]);
 #pragma unroll
-            for (int j = 0; j < HD / 16; ++j) {
-                uint32_t b[4];
-                pa_ldm4t(vt + S::at((lane >> 3 & 1) * 8 + (lane & 7), 2 * j + (lane >> 4)), b);
-                mma_bf16(acc[2 * j], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
-                mma_bf16(acc[2 * j + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+            for (int t = 0; t < TILE / 16; ++t) {
+                uint32_t pa[4];
+                pa[0] = pa_split(w[t * 4], w[t * 4 + 1], pa[1]);
+                pa[2] = pa_split(w[t * 4 + 2], w[t * 4 + 3], pa[3]);
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) {
+                    uint32_t b[4];
+                    pa_ldm4t(vt + S::at(t * 16 + (lane >> 3 & 1) * 8 + (lane & 7), 2 * j + (lane >> 4)), b);
+                    mma_bf16(acc[2 * j], pa[0], pa[1], pa[2], pa[3], b[0], b[1]);
+                    mma_bf16(acc[2 * j + 1], pa[0], pa[1], pa[2], pa[3], b[2], b[3]);
+                }
             }
         }
         stage = stage + 1 == S::kStages ? 0 : stage + 1;

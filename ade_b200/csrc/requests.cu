@@ -181,7 +181,7 @@ int ade_b200_paged_attn(const void* q, const void* cos_t, const void* sin_t, con
     const uint32_t page_mul = static_cast<uint32_t>((((1ull << page_shift) - page_size) << 32) / page_size + 1);
     // rows of one launch: PA_MAX_ROWS, fewer where the places of that many full rows would not fit 31 bits
     const long long heads = static_cast<long long>(kv_heads) * ((q_heads / kv_heads + ade::PA_HEADS - 1) / ade::PA_HEADS);
-    const long long fit = 0x7FFFFFFFll / (heads * (static_cast<long long>(width) * page_size / ade::PA_TILE + 1 + ade::PA_GAP));
+    const long long fit = 0x7FFFFFFFll / (heads * (static_cast<long long>(width) * page_size / 16 + 1 + ade::PA_GAP));
     if (fit < 1) return ADE_ERR_SHAPE;
     const int chunk = fit < ade::PA_MAX_ROWS ? static_cast<int>(fit) : ade::PA_MAX_ROWS;
     for (int t0 = 0; t0 < T; t0 += chunk) {
