@@ -59,7 +59,7 @@ int launch_attn(ade::PagedAttnParams p, int sms, cudaStream_t st) {
     if (!allow_smem<ade::paged_attn_kernel<HD>>(ade::pa_smem_bytes(S::kRing, S::kWarps, S::kStages, ade::PA_MAX_ROWS))) return ADE_ERR_CUDA;
     ade::paged_attn_kernel<HD><<<ctas, S::kWarps * 32, smem, st>>>(p);
     if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
-    return launch_early(ade::paged_attn_join_kernel<HD>, ctas * S::kWarps, 256, 0, st, p);
+    return launch_early(ade::paged_attn_join_kernel<HD>, ctas * S::kWarps / ade::PA_JOIN, 256, 0, st, p);
 }
 
 int launch_attn_dim(int head_dim, const ade::PagedAttnParams& p, int sms, cudaStream_t st) {
