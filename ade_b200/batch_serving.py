@@ -15,7 +15,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .decode_ops import add_rmsnorm, rmsnorm, silu_mul, token_logprobs
+from .decode_ops import SILU_TYPES, add_rmsnorm, rmsnorm, silu_mul, token_logprobs
 from .kernels import BANK_KEYS, bank_deltas, multi_delta_forward, pack_int4
 from .paged import MAX_REQUESTS, paged_attn_decode, paged_extend, paged_write
 from .serving import LINEAR_MODULE_NAMES, _decoder_layers
@@ -101,14 +101,15 @@ class BatchDecoder:
 
     Linear modules may be MultiDeltaLinear (each request then has a model of its own), ADEKernelLinear or plain.  Device state of a
     request: its length, its row of the block table, its last token, and its history: `tokens` (max_requests, max_len) and `logprobs`, the
-    log probability each generated token had.
+    log probability each generated token had.  The step is captured at the first call of ``step``: the model's modules and weights stay as they are
+    from then on.
     """
 
     def __init__(self, model, max_requests: int, max_len: int, pages: int | None = None, page_size: int = 64):
         """
         Parameters:
             max_requests: requests at a time, up to 4096.
-            max_len: tokens of a request, prompt and answer.
+            max_len: tokens of a request, prompt and answer; rounded up to whole pages for requests that are stepped one by one.
             pages: pages of the cache; default: enough for every request at its full length.
             page_size: tokens per page.
         """
@@ -116,6 +117,10 @@ class BatchDecoder:
 
         if not isinstance(model, ml.LlamaForCausalLM):
             raise ValueError("BatchDecoder: a LLaMA causal LM is expected")
+        if any(type(layer.mlp.act_fn).__name__ not in SILU_TYPES for layer in model.model.layers):
+            raise ValueError("BatchDecoder: MLPs with SiLU are expected")
+        if model.model.rotary_emb.rope_type in ("dynamic", "longrope"):
+            raise ValueError("BatchDecoder: rotary angles that change with the length would need the keys of a request anew")
         if not 1 <= max_requests <= MAX_REQUESTS or max_len < 1 or page_size < 1:
             raise ValueError(f"BatchDecoder: 1 to {MAX_REQUESTS} requests, max_len and page_size of at least 1")
         w = model.model.embed_tokens.weight
@@ -266,7 +271,7 @@ class BatchDecoder:
             raise ValueError(f"request {request} is not running")
         with torch.cuda.device(self.device):
             self._extend(request, -1, 0)
-            self.new_tokens[request] = 0
+            self.new_tokens[request] = self.status[request] = 0
             self._model_of[request] = -1
         self._free_slots.append(request)
 

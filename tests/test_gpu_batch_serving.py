@@ -215,3 +215,14 @@ def test_plain_and_single_delta_models_are_served_too(served):
     for bad in (lambda: BatchDecoder(torch.nn.Linear(2, 2), 1, 8), lambda: BatchDecoder(_llama(), 1, 8), lambda: BatchDecoder(base, 0, 8), lambda: BatchDecoder(base, 5000, 8)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_a_finished_request_leaves_no_report_behind(served):
+    _, single, many = served
+    g = torch.Generator().manual_seed(9)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (16, 16, 5)]
+    dec = BatchDecoder(many, max_requests=3, max_len=64, pages=3, page_size=16)
+    with pytest.raises(AdeKernelError, match="NO_PAGE"):  # three pages hold the prompts, none is left to grow
+        dec.generate(prompts, 4, [0, 1, 2])
+    (tokens, logprobs), = dec.generate(prompts[2:], 6, [2])
+    _check_answer(single[2], tokens, logprobs, 5)

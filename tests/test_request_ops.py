@@ -123,3 +123,15 @@ def test_status_table_follows_the_header():
     codes = {int(v): k for k, v in re.findall(r"#define (ADE_PAGED_\w+) (\d+)", header) if int(v)}
     assert set(codes) == set(_lib.PAGED_STATUS) and all(_lib.PAGED_STATUS[c].startswith(n + ":") for c, n in codes.items())
     assert f"ADE_B200_MAX_REQUESTS {paged.MAX_REQUESTS}" in header
+
+
+@pytest.mark.parametrize("change, why", [({"hidden_act": "gelu"}, "SiLU"),
+                                         ({"rope_parameters": {"rope_type": "dynamic", "factor": 2.0, "rope_theta": 10000.0}}, "rotary")])
+def test_models_that_a_step_would_answer_differently_are_refused(change, why):
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from ade_b200.batch_serving import BatchDecoder
+
+    cfg = LlamaConfig(hidden_size=64, intermediate_size=64, num_hidden_layers=1, num_attention_heads=2, vocab_size=50, **change)
+    with pytest.raises(ValueError, match=why):
+        BatchDecoder(LlamaForCausalLM(cfg).to(torch.bfloat16), 2, 16)
