@@ -39,6 +39,9 @@ struct ExtendParams {
 
 enum { PX_OK = 0, PX_NO_PAGE = 1, PX_TABLE_FULL = 2, PX_NO_ROW = 3, PX_BAD_LENGTH = 4 };
 
+// pages of n tokens; n + page_size may pass 31 bits
+__device__ __forceinline__ int px_pages(int n, int page_size) { return static_cast<int>((static_cast<uint32_t>(n) + page_size - 1u) / page_size); }
+
 // What the requests come to, in shared memory: inclusive sums over the requests of the rows of the packed batch, the pages handed back and
 // the pages taken, and each request's old length (-1: it has no rows).
 struct PxSums {
@@ -102,7 +105,7 @@ __device__ __forceinline__ PxSums px_sum(const ExtendParams& p, int* smem) {
             if (len[i] < 0 || len[i] > p.width * p.page_size) {
                 st[i] = PX_BAD_LENGTH;
             } else {
-                have[i] = (len[i] + p.page_size - 1) / p.page_size;
+                have[i] = px_pages(len[i], p.page_size);
                 rel[i] = f < 0;
                 grow[i] = max(f, 0);
                 const long long end = (static_cast<long long>(len[i]) + grow[i] + p.page_size - 1) / p.page_size;
@@ -167,7 +170,7 @@ __device__ __forceinline__ void px_place(const ExtendParams& p, const PxSums& r,
     // the i-th page of all that are taken comes from the i-th place below the top
     for (int i = at; i < r.used; i += threads) {
         const int b = px_find(r.need_end, p.B, i);
-        const int col = (r.len[b] + p.page_size - 1) / p.page_size + i - (b ? r.need_end[b - 1] : 0);
+        const int col = px_pages(r.len[b], p.page_size) + i - (b ? r.need_end[b - 1] : 0);
         p.table[b * p.table_stride + col] = stack(r.available - 1 - i);
     }
     for (int row = at; row < p.total; row += threads) {
@@ -176,7 +179,7 @@ __device__ __forceinline__ void px_place(const ExtendParams& p, const PxSums& r,
         const int b = px_find(r.row_end, p.B, row);
         if (b < p.B && r.len[b] >= 0) {
             const int len = r.len[b], to = len + row - (b ? r.row_end[b - 1] : 0), col = to / p.page_size;
-            const int have = (len + p.page_size - 1) / p.page_size;
+            const int have = px_pages(len, p.page_size);
             const int page = col < have ? p.table[b * p.table_stride + col] : stack(r.available - 1 - ((b ? r.need_end[b - 1] : 0) + col - have));
             if (page >= 0 && page < p.pages) {
                 slot = static_cast<long long>(page) * p.page_size + to - col * p.page_size;
@@ -190,6 +193,8 @@ __device__ __forceinline__ void px_place(const ExtendParams& p, const PxSums& r,
     }
 }
 
+// The reads depend on one another (lengths, sums, table, stack), a launch long and little else: 3.8 us for 64 requests on one CTA, and 11.8
+// for 45 000 rows of 1001 requests, whose 2 MB would take 0.3; with one CTA for all of them it took 105.
 // One CTA for all of it (a decode step), or, with `split`, for the sums alone, which paged_place_kernel takes from `work`.
 template <int NT, int ITEMS>
 __global__ void __launch_bounds__(NT) paged_extend_kernel(const ExtendParams p, bool split) {

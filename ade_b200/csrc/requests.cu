@@ -45,8 +45,18 @@ int launch_early(void (*kernel)(Params...), int grid, int threads, size_t smem, 
     return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, args...)) ? ADE_OK : ADE_ERR_CUDA;
 }
 
-// Rows that one CTA of the page allocation still places itself.
-constexpr int kExtendOneCta = 2048;
+// Threads of the page allocation's CTA: few, for short sums, as long as a thread has two requests at most (64 requests with a row each: 3.7 us, 7.6 with
+// 1024 threads; 512 requests: 5.4, 6.8 with 1024; 1000 requests: 6.8 either way).  It places up to four rows a thread itself (64 requests: 64 rows 3.7 us,
+// 5.8 with a second launch; 512 rows 6.4, 6.1; 1024 rows 9.5, 6.0; 1000 requests, 2048 rows: 8.9 either way).
+int extend_threads(int B) { return B <= 128 ? 128 : B <= 1024 ? 512 : 1024; }
+bool extend_split(int B, int total) { return total > 4 * extend_threads(B); }
+
+template <int NT, int ITEMS>
+int launch_extend(const ade::ExtendParams& p, bool split, cudaStream_t st) {
+    if (!allow_smem<ade::paged_extend_kernel<NT, ITEMS>>(ade::px_smem_bytes(NT * ITEMS))) return ADE_ERR_CUDA;
+    ade::paged_extend_kernel<NT, ITEMS><<<1, NT, ade::px_smem_bytes(p.B), st>>>(p, split);
+    return launched();
+}
 
 constexpr size_t kAttnWarps = static_cast<size_t>(ade::PA_MAX_CTAS) * 8;
 
@@ -83,7 +93,7 @@ bool rows_fit(int pages, int kv_heads, int page_size) { return static_cast<unsig
 extern "C" {
 
 size_t ade_b200_paged_extend_workspace_bytes(int B, int total) {
-    return B < 1 || B > ADE_B200_MAX_REQUESTS || total <= kExtendOneCta ? 0 : 16 + ade::px_smem_bytes(B);
+    return B < 1 || B > ADE_B200_MAX_REQUESTS || !extend_split(B, total) ? 0 : 16 + ade::px_smem_bytes(B);
 }
 
 int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int32_t* block_table, int32_t* free_pages, const int32_t* free_count,
@@ -94,7 +104,7 @@ int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int
     if (total > 0 && (!slots || !positions || !requests)) return ADE_ERR_NULL;
     if (B < 1 || B > ADE_B200_MAX_REQUESTS || width < 1 || table_row_stride < width || pages < 1 || page_size < 1 || total < 0) return ADE_ERR_SHAPE;
     if (static_cast<long long>(width) * page_size > 0x7FFFFFFFll || total > (1 << 30)) return ADE_ERR_SHAPE;
-    const bool split = total > kExtendOneCta;
+    const bool split = extend_split(B, total);
     if (split && !work) return ADE_ERR_NULL;
     if (!aligned16(work)) return ADE_ERR_ALIGN;
     if (work_bytes < ade_b200_paged_extend_workspace_bytes(B, total)) return ADE_ERR_SCRATCH;
@@ -104,17 +114,12 @@ int ade_b200_paged_extend(const int32_t* lengths, const int32_t* new_tokens, int
     const ade::ExtendParams p = {lengths, new_tokens, block_table, free_pages, free_count, lengths_out, free_count_out, status, slots, positions,
                                  requests, static_cast<int*>(work), B, width, pages, page_size, total, table_row_stride};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const size_t smem = ade::px_smem_bytes(B);
-    if (B <= 128 && !split) {
-        ade::paged_extend_kernel<128, 1><<<1, 128, smem, st>>>(p, false);
-        return launched();
-    }
-    const size_t most = ade::px_smem_bytes(ADE_B200_MAX_REQUESTS);
-    if (!allow_smem<ade::paged_extend_kernel<1024, 4>>(most) || !allow_smem<ade::paged_place_kernel>(most)) return ADE_ERR_CUDA;
-    ade::paged_extend_kernel<1024, 4><<<1, 1024, smem, st>>>(p, split);
-    if (!split || !cuda_ok(cudaGetLastError())) return launched();
+    const int threads = extend_threads(B);
+    const int rc_launch = threads == 128 ? launch_extend<128, 1>(p, split, st) : threads == 512 ? launch_extend<512, 2>(p, split, st) : launch_extend<1024, 4>(p, split, st);
+    if (rc_launch || !split) return rc_launch;
+    if (!allow_smem<ade::paged_place_kernel>(ade::px_smem_bytes(ADE_B200_MAX_REQUESTS))) return ADE_ERR_CUDA;
     const int ctas = (total + 511) / 512;
-    return launch_early(ade::paged_place_kernel, ctas < 2 * sms ? ctas : 2 * sms, 256, smem, st, p);
+    return launch_early(ade::paged_place_kernel, ctas < 2 * sms ? ctas : 2 * sms, 256, ade::px_smem_bytes(B), st, p);
 }
 
 int ade_b200_paged_write(const void* k, const void* v, const void* cos_t, const void* sin_t, const long long* slots, void* k_pages, void* v_pages,
@@ -227,10 +232,10 @@ int ade_b200_multi_delta(const void* x, const void* y_dense, const ade_delta_ban
     const int slices = ade::md_slices(d.N);
     ade::multi_delta_v_kernel<<<2 * sms, ade::MD_THREADS, ade::md_v_smem(), st>>>(p, slices);
     if (!cuda_ok(cudaGetLastError())) return ADE_ERR_CUDA;
-    // One CTA per SM for the second launch where that gives a warp two tiles at most: it is set up beside the first one's CTAs then, instead of behind
-    // them (4096 x 4096, 16 rows of 12 deltas: 14.0 us with two).
+    // One CTA per SM for the second launch where that gives a warp one tile at most: it is set up beside the first one's CTAs then, instead of behind
+    // them.  4096 x 4096: 13.2 us for 16 rows of 12 deltas, 13.7 with two CTAs; 19.3 for 40 rows of 30 deltas (two tiles), 17.2 with two.
     const long long entries = T < d.deltas + 1 + T / ade::MD_ENTRY ? T : d.deltas + 1 + T / ade::MD_ENTRY;
-    const bool few = entries * ((d.M + ade::MD_TILE - 1) / ade::MD_TILE) <= 2ll * sms * (ade::MD_THREADS / 32);
+    const bool few = entries * ((d.M + ade::MD_TILE - 1) / ade::MD_TILE) <= 1ll * sms * (ade::MD_THREADS / 32);
     return launch_early(ade::multi_delta_u_kernel, few ? sms : 2 * sms, ade::MD_THREADS, ade::md_u_smem(), st, p, slices);
 }
 

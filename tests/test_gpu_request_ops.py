@@ -94,7 +94,7 @@ def _check_extend(lengths, new, table, free, count, total, ps, in_place=False):
     return new_len.tolist(), t.tolist(), f.tolist(), new_count.item()
 
 
-@pytest.mark.parametrize("B, width, ps, pages, seed", [(1, 3, 4, 3, 0), (5, 4, 1, 12, 1), (33, 6, 16, 90, 2), (64, 5, 24, 400, 3), (1025, 3, 8, 1500, 4),
+@pytest.mark.parametrize("B, width, ps, pages, seed", [(1, 3, 4, 3, 0), (5, 4, 1, 12, 1), (33, 6, 16, 90, 2), (64, 5, 24, 400, 3), (1025, 3, 8, 1500, 4), (300, 4, 16, 700, 7),
                                                        (4096, 2, 64, 8192, 5), (7, 9, 3, 20, 6)])
 def test_extend_follows_the_rules_step_by_step(B, width, ps, pages, seed):
     """Requests enter, grow, rest, end and fail (no page, a full table, no row) over ten steps; no page is ever owned twice."""
@@ -124,6 +124,21 @@ def test_extend_takes_bad_states_for_what_they_are():
     t, f = _i32([[-1]]), _i32([0, 1])
     assert paged_extend(_i32([0]), _i32([1]), t, f, _i32([7]), 1, 4)[4].item() == 1 and t.item() == 1
     assert paged_extend(_i32([0]), _i32([1]), t, f, _i32([-3]), 1, 4)[5].item() == 1
+
+
+def test_extend_counts_pages_of_any_size():
+    big = 2 ** 31 - 1
+    _check_extend([2 ** 30, 5, big, 0, big, 1], [3, -1, -1, 1, 1, big - 1], [[4], [3], [5], [-1], [1], [0]], [7, 6, 2, -1, -1, -1, -1, -1], 3, 5, big)
+
+
+def test_extend_places_rows_by_one_launch_or_two():
+    """Around the sizes at which a second launch begins, for few requests and for many."""
+    for B, sums in ((3, (511, 512, 513)), (128, (513,)), (129, (2047, 2048, 2049)), (1024, (2049,)), (1025, (4096, 4097))):
+        for total in sums:
+            new = [total // B + (b < total % B) for b in range(B)]
+            width = max(new) // 16 + 3
+            _check_extend([b % 33 for b in range(B)], new, [[b * width + c for c in range(width)] for b in range(B)],
+                          list(range(B * width, 2 * B * width)) + [-1] * (B * width), B * width, total, 16)
 
 
 def test_extend_reads_a_table_that_is_a_slice():
