@@ -8,6 +8,8 @@
 // counting.  A row whose list would not fit (hundreds of equal logits at the bound) or that holds a NaN is walked once for every
 // alternative instead.  256 threads whatever the row: 1024 of them took 6.6 us instead of 5.3 for 8 rows of 32000, 12.7 instead of 12.6 for 8 of
 // 152064, and 512 took 49 instead of 37 for 2048 rows of 32000.
+// 2048 rows of 50257 float32 logits with twenty alternatives take 82 us (0.41 GB, 5.0 TB/s; 69 without alternatives, whose small dependent steps end each
+// row); in bfloat16, 2048 rows of 32000, 37 us (3.5 TB/s): there exponentials and sums bound it, two bytes a logit.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

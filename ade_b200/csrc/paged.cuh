@@ -193,7 +193,7 @@ __device__ __forceinline__ void px_place(const ExtendParams& p, const PxSums& r,
     }
 }
 
-// The reads depend on one another (lengths, sums, table, stack), a launch long and little else: 3.8 us for 64 requests on one CTA, and 11.8
+// The reads depend on one another (lengths, sums, table, stack), a launch long and little else: 3.7 us for 64 requests on one CTA, and 10.8
 // for 45 000 rows of 1001 requests, whose 2 MB would take 0.3; with one CTA for all of them it took 105.
 // One CTA for all of it (a decode step), or, with `split`, for the sums alone, which paged_place_kernel takes from `work`.
 template <int NT, int ITEMS>

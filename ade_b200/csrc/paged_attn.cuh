@@ -12,6 +12,10 @@
 // a pair costs besides them (its queries, its result): without them the warps that meet the short pairs of a ragged batch end last.  A warp streams its tiles through cp.async stages of its own and never waits
 // for another; what it has of a pair that others share goes to the workspace as (maximum, sum, weighted sum), and a second
 // launch joins those parts in the order of the tiles.  A CTA whose tiles all belong to one pair joins its warps' parts itself.
+//
+// Long rows are bound by memory: 32 rows of 16 to 4000 positions, 32 heads of 128 (0.41 GB) take 81 us, 3 rows of up to 60 000 positions on 8 heads for 32
+// queries (0.47 GB) 87 us, 5.0 and 5.3 TB/s, of which 4 us are set-up and 3 the join.  Short ones are bound by two launches and what depends on
+// what in them: lengths, table, keys, parts.
 #pragma once
 #include "paged.cuh"
 #include "ptx.cuh"
@@ -43,7 +47,9 @@ struct PagedAttnParams {
 template <int HD>
 struct PaShape {
     static constexpr int kWarps = HD <= 128 ? 8 : 4;
-    static constexpr int kTile = HD <= 64 ? 32 : 16;                     // positions of a tile, 8 KB of a cache of 64 or 128 dimensions
+    // positions of a tile: 32 up to 64 dimensions (32 rows of 100 to 2000 positions, 8 heads of 64: 19.2 us, 21.0 with 16), 16 where 32 would leave a warp
+    // fewer than three stages
+    static constexpr int kTile = HD <= 64 ? 32 : 16;
     static constexpr int kChunks = HD / 8;                               // 16-byte pieces of a row
     static constexpr int kTileBytes = kTile * HD * 2;
     static constexpr int kStages = 192 * 1024 / (kWarps * 2 * kTileBytes) < 8 ? 192 * 1024 / (kWarps * 2 * kTileBytes) : 8;
@@ -143,11 +149,12 @@ __global__ void __launch_bounds__(PaShape<HD>::kWarps * 32, 1) paged_attn_kernel
             for (int i = tid; i < p.q_heads * HD / 8; i += NT)
                 reinterpret_cast<uint4*>(p.out + static_cast<long long>(t) * p.q_heads * HD)[i] = make_uint4(0u, 0u, 0u, 0u);
 
-    // This warp's places f .. f_end - 1 of all, and whether its whole CTA works on one pair.  Where every warp would have two tiles at most, a pair
-    // gets as many CTAs of its own as it takes: for short rows one, which then needs nobody else.
+    // This warp's places f .. f_end - 1 of all, and whether its whole CTA works on one pair.  Where every warp would have two tiles at most and the pairs
+    // are of one length, a pair gets as many CTAs of its own as it takes: for short rows one, which then needs nobody else (100 positions, 32 heads of
+    // 128: 8.4 us, 10.1 with all CTAs; 4 rows of 20 to 200 positions: 11.6 so, 11.1 with all CTAs, since the cuts do not fall between the pairs).
     const int total = prefix[p.T], cta = blockIdx.x, pairs = live * H;
     int most = gridDim.x;
-    if (total <= most * NW * 2 && pairs > 0 && pairs <= most) most = pairs * min(most / pairs, (longest + 2 * NW - 1) / (2 * NW));
+    if (total <= most * NW * 2 && pairs > 0 && pairs <= most && total == pairs * longest) most = pairs * min(most / pairs, (longest + 2 * NW - 1) / (2 * NW));
     const int ctas = min(most, total), each = ctas ? total / ctas : 0, more = total - each * ctas;
     auto cta_begin = [&](int c) { return each * c + min(c, more); };
     const int wid = cta * NW + warp;
