@@ -568,43 +568,69 @@ __global__ void __launch_bounds__(MD_THREADS, 2) multi_delta_u_kernel(const Mult
     }
     int slot = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // the columns of h of some entries, from rank group `at` in shared memory on: one (row, rank group) per warp and round, four ranks per lane; the
-    // slices' sums in fixed point, bytes in the order of the codes' (0 4 1 5 and 2 6 3 7 of eight, which two lanes share)
+    // the columns of h of some entries, from rank group `at` in shared memory on: two (row, rank group) per warp and round, side by side since each is a
+    // chain of waits, four ranks per lane; the slices' sums in fixed point, bytes in the order of the codes' (0 4 1 5 and 2 6 3 7 of eight, which two
+    // lanes share).  Magnitudes are compared as integers: NaN lies behind infinity.
     auto bring = [&](int en, int at) {
-        const int ng = e.ng[en];
-        for (int i = warp; i < e.rows[en] * ng; i += MD_THREADS / 32) {
-            const int r = i / ng, jr = i - r * ng, j = at + jr;
-            const float* from = p.h + static_cast<size_t>(e.row[en][r]) * MD_H + jr * 128 + lane * 4;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int W = MD_THREADS / 32;
+        const int ng = e.ng[en], n = e.rows[en] * ng;
+        for (int i0 = warp; i0 < n; i0 += 2 * W) {
+            const int i[2] = {i0, i0 + W < n ? i0 + W : i0};                     // the last one twice where the number is odd
+            int r[2], j[2];
+            float v[2][4] = {};
+            const float* from[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                r[k] = i[k] / ng;
+                j[k] = i[k] - r[k] * ng;
+                from[k] = p.h + static_cast<size_t>(e.row[en][r[k]]) * MD_H + j[k] * 128 + lane * 4;
+            }
 #pragma unroll 4
-            for (int s = 0; s < slices; ++s) {
-                const float4 a = *reinterpret_cast<const float4*>(from + static_cast<size_t>(s) * p.T * MD_H);
-                v.x += a.x;
-                v.y += a.y;
-                v.z += a.z;
-                v.w += a.w;
-            }
-            float m = md_max(md_max(fabsf(v.x), fabsf(v.y)), md_max(fabsf(v.z), fabsf(v.w)));
+            for (int s = 0; s < slices; ++s)
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = md_max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            const MdFixed fx = md_fixed(m);
-            const float w[4] = {v.x, v.y, v.z, v.w};
-            uint32_t q[4], q8[4];
+                for (int k = 0; k < 2; ++k) {
+                    const float4 a = *reinterpret_cast<const float4*>(from[k] + static_cast<size_t>(s) * p.T * MD_H);
+                    v[k][0] += a.x;
+                    v[k][1] += a.y;
+                    v[k][2] += a.z;
+                    v[k][3] += a.w;
+                }
+            uint32_t m[2], up[2], lo[2], up2[2], lo2[2];
+            MdFixed fx[2];
+            int su[2], sl[2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                q[k] = __float_as_uint(fmaf(w[k], fx.scale, kMdMagic));
-                q8[k] = q[k] + 128u;                                             // the upper byte is the one of v + 128
+            for (int k = 0; k < 2; ++k)
+                m[k] = max(max(__float_as_uint(v[k][0]) & 0x7FFFFFFFu, __float_as_uint(v[k][1]) & 0x7FFFFFFFu),
+                           max(__float_as_uint(v[k][2]) & 0x7FFFFFFFu, __float_as_uint(v[k][3]) & 0x7FFFFFFFu));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) m[k] = __reduce_max_sync(0xFFFFFFFFu, m[k]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                fx[k] = md_fixed(__uint_as_float(m[k]));
+                uint32_t q[4], q8[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    q[x] = __float_as_uint(fmaf(v[k][x], fx[k].scale, kMdMagic));
+                    q8[x] = q[x] + 128u;                                         // the upper byte is the one of v + 128
+                }
+                up[k] = __byte_perm(__byte_perm(q8[0], q8[1], 0x51), __byte_perm(q8[2], q8[3], 0x51), 0x5410);
+                lo[k] = __byte_perm(__byte_perm(q[0], q[1], 0x40), __byte_perm(q[2], q[3], 0x40), 0x5410);
             }
-            const uint32_t up = __byte_perm(__byte_perm(q8[0], q8[1], 0x51), __byte_perm(q8[2], q8[3], 0x51), 0x5410);
-            const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x40), __byte_perm(q[2], q[3], 0x40), 0x5410);
-            const uint32_t up2 = __shfl_xor_sync(0xFFFFFFFFu, up, 1), lo2 = __shfl_xor_sync(0xFFFFFFFFu, lo, 1);
-            const int c = r * 2;                                                 // column of the upper bytes; the lower stand behind it
-            uint8_t* to = hcol + c * MD_HCOL + j * 128 + (lane >> 2 & 1) * 64 + (lane >> 3) * 16 + (lane >> 1 & 1) * 8 + (lane & 1) * 4;
-            *reinterpret_cast<uint32_t*>(to) = lane & 1 ? __byte_perm(up2, up, 0x7362) : __byte_perm(up, up2, 0x5140);
-            *reinterpret_cast<uint32_t*>(to + MD_HCOL) = lane & 1 ? __byte_perm(lo2, lo, 0x7362) : __byte_perm(lo, lo2, 0x5140);
-            const int su = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(up), 0x01010101, 0));
-            const int sl = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(lo), 0x01010101, 0));
-            if (lane == 0) hsum[j * 8 + r] = make_float2(fx.unit, fx.unit * (256.f * su + sl));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                up2[k] = __shfl_xor_sync(0xFFFFFFFFu, up[k], 1);
+                lo2[k] = __shfl_xor_sync(0xFFFFFFFFu, lo[k], 1);
+                su[k] = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(up[k]), 0x01010101, 0));
+                sl[k] = __reduce_add_sync(0xFFFFFFFFu, __dp4a(static_cast<int>(lo[k]), 0x01010101, 0));
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int c = r[k] * 2;                                          // column of the upper bytes; the lower stand behind it
+                uint8_t* to = hcol + c * MD_HCOL + (at + j[k]) * 128 + (lane >> 2 & 1) * 64 + (lane >> 3) * 16 + (lane >> 1 & 1) * 8 + (lane & 1) * 4;
+                *reinterpret_cast<uint32_t*>(to) = lane & 1 ? __byte_perm(up2[k], up[k], 0x7362) : __byte_perm(up[k], up2[k], 0x5140);
+                *reinterpret_cast<uint32_t*>(to + MD_HCOL) = lane & 1 ? __byte_perm(lo2[k], lo[k], 0x7362) : __byte_perm(lo[k], lo2[k], 0x5140);
+                if (lane == 0) hsum[(at + j[k]) * 8 + r[k]] = make_float2(fx[k].unit, fx[k].unit * (256.f * su[k] + sl[k]));
+            }
         }
     };
     const bool vec = (p.M & 3) == 0;                                             // four outputs are an aligned piece of 8 bytes

@@ -490,7 +490,8 @@ def _check_logprobs(x, tokens, top):
 
 @pytest.mark.parametrize("rows, V, dtype, top", [(1, 1, torch.float32, 1), (3, 5, torch.bfloat16, 5), (2, 31, torch.float16, 31), (1, 32, torch.float32, 32),
                                                  (4, 255, torch.bfloat16, 7), (5, 256, torch.float32, 0), (7, 1003, torch.float16, 32), (64, 32000, torch.bfloat16, 5),
-                                                 (3, 50257, torch.float32, 20), (2, 152064, torch.bfloat16, 32), (1, 257001, torch.float32, 1), (300, 2048, torch.bfloat16, 3)])
+                                                 (3, 50257, torch.float32, 20), (2, 152064, torch.bfloat16, 32), (1, 257001, torch.float32, 1), (300, 2048, torch.bfloat16, 3),
+                                                 (10, 532, torch.bfloat16, 20), (9, 517, torch.float32, 32), (5, 1025, torch.float16, 32)])
 def test_log_probabilities(rows, V, dtype, top):
     g = _gen(rows + V)
     x = (torch.randn(rows, V, generator=g, device=DEV) * 3).to(dtype)
