@@ -21,9 +21,9 @@
 // Every thread copies the 16-byte pieces of codes that it will use itself with cp.async into a queue of its own, so the
 // stream runs through the barriers of an item and into the next one.  Sums have a fixed order; there are no floating-point atomics.
 //
-// Measured: 50.6 us for 128 rows of 48 deltas, 11008 x 4096 (178 MB, 3.5 TB/s): about 24 us for the first launch, which has a quarter of the bytes and is
-// bound by bringing the activations to fixed point and by the latency of its short items, the rest for the second, at 5 TB/s.  13.0 us for 16 rows
-// of 12 deltas, 4096 x 4096, and 9.1 for 3 rows, 1000 x 2048: launches, and what depends on what in them.
+// Measured: 50.4 us for 128 rows of 48 deltas, 11008 x 4096 (178 MB, 3.5 TB/s): alone, 19 us for the first launch, which has a quarter of the bytes and is
+// bound by bringing the activations to fixed point and by the latency of its short items, and 39 for the second; no pipe of either is above 40 %.
+// 13.0 us for 16 rows of 12 deltas, 4096 x 4096, and 9.1 for 3 rows, 1000 x 2048: launches, and what depends on what in them.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
