@@ -60,7 +60,8 @@ def paged_attn_decode(q: torch.Tensor, block_table: torch.Tensor, requests: torc
     """softmax(q K^T scale) V of single token rows over the cached positions 0 .. positions[t] of request requests[t].
 
     q is a (rows, q_heads, head_dim) bfloat16 view with a contiguous last dimension, rotated with cos and sin where they are given; the
-    heads of a key-value head are consecutive.  Rows without a request (requests[t] = -1) are zero.  Returns
-    (rows, q_heads * head_dim) bfloat16; scores, probabilities and sums are float32.
+    heads of a key-value head are consecutive.  Rows without a request (requests[t] = -1) are zero.  Positions whose table entry is no page
+    are left out.  What a row sees of keys, values and scores has to be finite; where it is not, that row (and no other) may be NaN.  What
+    stands behind positions[t] is not read.  Returns (rows, q_heads * head_dim) bfloat16; scores, probabilities and sums are float32.
     """
     return _call("paged_attn", q, block_table, requests, positions, k_pages, v_pages, scale, cos, sin)

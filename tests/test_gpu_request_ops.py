@@ -320,6 +320,19 @@ def test_attention_does_not_look_behind_the_row():
     assert torch.equal(paged_attn_decode(**c), clean)
 
 
+@pytest.mark.parametrize("lengths", [[40, 33, 70, 5], [900, 2000, 64, 1500]], ids=str)
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_row_that_sees_no_number_leaves_the_others_alone(lengths, value):
+    c = _attn_case(4, 8, 2, 64, 16, lengths, seed=5)
+    clean = paged_attn_decode(**c)
+    page = int(c["block_table"][int(c["requests"][1]), 1])
+    c["k_pages"][page, :, 3], c["v_pages"][page, :, 4] = value, value
+    got = paged_attn_decode(**c)
+    assert bool(torch.isnan(got[1]).any())
+    for t in (0, 2, 3):
+        assert torch.equal(got[t], clean[t])
+
+
 def test_attention_takes_strided_queries():
     c = _attn_case(5, 4, 4, 64, 16, [30, 1, 64, 7, 19], seed=4)
     want = paged_attn_decode(**c)
