@@ -33,17 +33,18 @@ class DeltaRoute:
 
 
 class MultiDeltaLinear(nn.Module):
-    """W_b x + U_d^ (V_d^^T x) with the delta d of each row's own fine-tuned model (bfloat16, inference): the library GEMM for the
+    """W_b x + b + U_d^ (V_d^^T x) with the delta d of each row's own fine-tuned model (bfloat16, inference): the library GEMM for the
     shared term, as the reference's module has it above its own launch (src/serving.py:106-111), and one
     ``multi_delta_forward`` for every 128 rows."""
 
-    def __init__(self, W_b: torch.Tensor, stored_forms, route: DeltaRoute):
+    def __init__(self, W_b: torch.Tensor, stored_forms, route: DeltaRoute, bias: torch.Tensor | None = None):
         """
         Parameters:
             W_b: base weight (d_o, d_i).
             stored_forms: for each fine-tuned model its ``pack_int4`` result for this module on the CUDA device, or None where the
                 model has no delta here.
             route: the rows' models.
+            bias: the base's bias (d_o,), which all of the models share, or None.
         """
         super().__init__()
         self.out_features, self.in_features = W_b.shape
@@ -51,6 +52,9 @@ class MultiDeltaLinear(nn.Module):
         if (bank["M"], bank["N"]) != tuple(W_b.shape):
             raise ValueError(f"deltas are {bank['M']} x {bank['N']}, base weight {tuple(W_b.shape)}")
         self.register_buffer("weight", W_b.detach().to(device=bank["start"].device, dtype=torch.bfloat16).contiguous())
+        if bias is not None and bias.shape != W_b.shape[:1]:
+            raise ValueError(f"base weight is {tuple(W_b.shape)}, bias {tuple(bias.shape)}")
+        self.register_buffer("bias", None if bias is None else bias.detach().to(device=self.weight.device, dtype=torch.bfloat16).contiguous())
         for k in BANK_KEYS:
             self.register_buffer(f"bank_{k}", bank[k])
         self.route = route
@@ -61,7 +65,7 @@ class MultiDeltaLinear(nn.Module):
     def forward(self, x):
         """x (..., d_i) -> (..., d_o) in bfloat16; the route names as many rows as x has."""
         x2 = x.reshape(-1, x.shape[-1]).to(torch.bfloat16).contiguous()
-        y = F.linear(x2, self.weight)
+        y = F.linear(x2, self.weight, self.bias)
         ids = self.route.ids
         if ids is not None and x2.shape[0]:
             if ids.shape[0] != x2.shape[0]:
@@ -77,6 +81,7 @@ def attach_multi_deltas(model, base_state_dict: dict, per_model, device="cuda") 
 
     `per_model` is a sequence with one mapping per fine-tuned model from ``model.layers.<i>.<name>`` to the packed fields
     (what ``attach_kernel_linears`` takes for one); `base_state_dict` maps ``model.layers.<i>.<name>.weight`` to the base weight.
+    A module with a bias keeps it: ``model.layers.<i>.<name>.bias`` of `base_state_dict`, or where that has none the module's own.
     The model's route (``model._ade_route``) says which row uses which; it starts at the base model.  Returns the number of
     modules replaced.
     """
@@ -91,7 +96,11 @@ def attach_multi_deltas(model, base_state_dict: dict, per_model, device="cuda") 
             if all(f is None for f in forms):
                 continue
             owner_path, _, leaf = sub.rpartition(".")
-            setattr(layer.get_submodule(owner_path), leaf, MultiDeltaLinear(base_state_dict[prefix + ".weight"], forms, route))
+            owner = layer.get_submodule(owner_path)
+            bias = getattr(getattr(owner, leaf), "bias", None)
+            if bias is not None and prefix + ".bias" in base_state_dict:
+                bias = base_state_dict[prefix + ".bias"]
+            setattr(owner, leaf, MultiDeltaLinear(base_state_dict[prefix + ".weight"], forms, route, bias))
             swapped += 1
     return swapped
 

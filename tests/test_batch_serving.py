@@ -1,0 +1,53 @@
+"""Modules and decoder for many requests: what needs no GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from ade_b200 import kernels, synth
+from ade_b200.batch_serving import DeltaRoute, MultiDeltaLinear, attach_multi_deltas
+from ade_b200.serving import LINEAR_MODULE_NAMES
+
+
+def _llama(**change):
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    torch.manual_seed(0)
+    cfg = LlamaConfig(**{**dict(hidden_size=128, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2, vocab_size=50), **change})
+    return LlamaForCausalLM(cfg).to(torch.bfloat16).eval()
+
+
+def _deltas(sd, seed, skip=()):
+    return {f"model.layers.{li}.{n}": synth.random_packed(*sd[f"model.layers.{li}.{n}.weight"].shape, 128, seed=seed + 10 * li + i)
+            for li in range(2) for i, n in enumerate(LINEAR_MODULE_NAMES) if n not in skip}
+
+
+@pytest.mark.parametrize("change", [{"attention_bias": True}, {"mlp_bias": True}, {"attention_bias": True, "mlp_bias": True}, {}], ids=str)
+def test_biases_of_the_base_stay(change):
+    """Rows of the base model are answered by the same operations as before: the same bits.  With the biases in the mapping and without."""
+    model = _llama(**change)
+    g = torch.Generator().manual_seed(1)
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if n.endswith(".bias"):
+                p.copy_(torch.randn(p.shape, generator=g) * 0.5)
+    sd = {k: v.clone() for k, v in model.state_dict().items()}
+    weights = {k: v for k, v in sd.items() if not k.endswith(".bias")}
+    ids = torch.arange(7)[None]
+    with torch.no_grad():
+        want = model(input_ids=ids).logits
+        for given in (sd, weights, sd):               # the third time in place of the modules of the second
+            assert attach_multi_deltas(model, given, [_deltas(sd, 1), _deltas(sd, 2, skip=LINEAR_MODULE_NAMES[1:3])], device="cpu") == 14
+            assert torch.equal(model(input_ids=ids).logits, want)
+        assert len([n for n, _ in model.named_buffers() if n.endswith("proj.bias")]) == sum(k.endswith(".bias") for k in sd)
+        # the mapping's bias goes before the module's
+        moved = {k: v + 1 if k.endswith(".bias") else v for k, v in sd.items()}
+        attach_multi_deltas(model, moved, [_deltas(sd, 1)], device="cpu")
+        assert torch.equal(model(input_ids=ids).logits, want) != bool(change)
+
+
+def test_a_bias_of_another_size_is_refused():
+    form = kernels.pack_int4(synth.random_packed(32, 128, 128, 1))
+    for bias in (torch.zeros(128), torch.zeros(1), torch.zeros(32, 1)):
+        with pytest.raises(ValueError, match="bias"):
+            MultiDeltaLinear(torch.zeros(32, 128), [form], DeltaRoute(1), bias)
