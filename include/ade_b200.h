@@ -319,9 +319,9 @@ int ade_b200_attn_decode(const void* q, const void* k, const void* v, const void
  *                  request b did not grow (its length then stays): ADE_PAGED_NO_PAGE (the stack does not reach to it),
  *                  ADE_PAGED_TABLE_FULL (width * page_size), ADE_PAGED_NO_ROW (its rows do not end within `total`),
  *                  ADE_PAGED_BAD_LENGTH (negative, or beyond its row of the table; nothing is handed back either).  lengths_out
- *                  and free_count_out may be lengths and free_count; work: 16-byte aligned, ade_b200_paged_extend_workspace_bytes
- *                  (0 up to 2048 rows: work may be NULL), contents of no meaning before and after the call.  B <= ADE_B200_MAX_REQUESTS, width * page_size < 2^31,
- *                  total <= 2^30.
+ *                  and free_count_out may be lengths and free_count; work: 16-byte aligned, ade_b200_paged_extend_workspace_bytes(B, total)
+ *                  bytes, contents of no meaning before and after the call; it may be NULL where that function returns 0, which depends
+ *                  on both numbers.  B <= ADE_B200_MAX_REQUESTS, width * page_size < 2^31, total <= 2^30.
  *   ade_b200_paged_write   k [T][kv_heads][head_dim] (rotated with cos / sin [T][head_dim] in float32 and rounded once; both NULL:
  *                  as it is) and v into the slots of their rows; slots outside 0 .. pages * page_size - 1 are left out.  Of two rows
  *                  with the same slot either may stay.  head_dim a multiple of 32 up to 256, here and below.

@@ -135,3 +135,17 @@ def test_models_that_a_step_would_answer_differently_are_refused(change, why):
     cfg = LlamaConfig(hidden_size=64, intermediate_size=64, num_hidden_layers=1, num_attention_heads=2, vocab_size=50, **change)
     with pytest.raises(ValueError, match=why):
         BatchDecoder(LlamaForCausalLM(cfg).to(torch.bfloat16), 2, 16)
+
+
+@pytest.mark.parametrize("B, most", [(1, 512), (4, 512), (128, 512), (129, 2048), (1024, 2048), (1025, 4096), (4096, 4096)])
+def test_page_allocation_needs_a_workspace_where_it_says_so(B, most):
+    """The header names the function and no number of rows: the number depends on the requests."""
+    import os
+
+    size = _lib.load().ade_b200_paged_extend_workspace_bytes
+    assert size(B, 0) == size(B, most) == 0 and size(B, most + 1) >= 16 * B
+    assert _extend(B=B, total=most + 1, work=None, work_bytes=0) == NULL
+    assert _extend(B=B, total=most + 1, work_bytes=size(B, most + 1) - 1) == SCRATCH
+    assert size(0, 5000) == size(4097, 5000) == 0
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "ade_b200.h")).read()
+    assert "may be NULL where that function returns 0" in header and "rows: work may be NULL" not in header
