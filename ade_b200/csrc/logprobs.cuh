@@ -113,7 +113,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprob_kernel(const LogprobPar
     const int head = min(V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
     const int pieces = (V - head) / P::N, tail = head + pieces * P::N;
     const uint4* body = reinterpret_cast<const uint4*>(x + head);
-    const int edge = tid < head ? tid : tail + tid - head;                   // this thread's logit outside the pieces, if below V
+    // this thread's logit outside the pieces, if below V; behind the last of them it may pass 31 bits
+    const uint32_t edge = tid < head ? tid : static_cast<uint32_t>(tail) + tid - head, end = V;
     if (tid == 0) listed = found = 0;
     float given = 0.f;                                                       // the given token's logit, under way from the start
     if (tid == 0 && p.tokens) {
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprob_kernel(const LogprobPar
     }
 
     LpSums a = {-INFINITY, 0.f, 0.f};
-    if (edge < V) {
+    if (edge < end) {
         const float v = lp_float(x[edge]);
         a.m = fmaxf(a.m, v);
         a.add(v, a.base());
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprob_kernel(const LogprobPar
             const int n = atomicAdd(&listed, 1);
             if (n < LP_LIST) list[n] = lp_key(v, at);
         };
-        if (edge < V) list_it(lp_float(x[edge]), edge);
+        if (edge < end) list_it(lp_float(x[edge]), edge);
         if (mine >= bound)
             for (int r = 0; r * length < batches; ++r)
                 if (rmax[r][tid] >= bound) runs[atomicAdd(&found, 1)] = static_cast<unsigned short>(r * THREADS + tid);
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprob_kernel(const LogprobPar
             const unsigned long long key = lp_key(v, at);
             if ((j == 0 || key < below) && key > best) best = key;
         };
-        if (edge < V) look(lp_float(x[edge]), edge);
+        if (edge < end) look(lp_float(x[edge]), edge);
         for (int k = tid; k < pieces; k += THREADS) {
             float v[P::N];
             P::get(__ldg(body + k), v);

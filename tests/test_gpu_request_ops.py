@@ -564,6 +564,20 @@ def test_logits_with_strides_and_without_tokens():
     assert token_logprobs(big[:0], tokens[:0], 3)[2].shape == (0, 3)
 
 
+def test_a_row_of_all_31_bits():
+    """The places behind the row's last whole piece, and the threads that have none there, are counted beyond 31 bits."""
+    V = 2 ** 31 - 1
+    x = torch.zeros(1, V, dtype=torch.bfloat16, device=DEV)
+    x[0, V - 1], x[0, V - 2], x[0, 0] = 3.0, 2.0, 1.0
+    logp, entropy, tl, tt = token_logprobs(x, torch.tensor([V - 1], device=DEV), 3)
+    assert tt.tolist() == [[V - 1, V - 2, 0]]
+    # a thread adds V / 256 terms in float32, each sum off by 2^-24 of it at most: e^(+-tol) of the sum of exp
+    tol = 2.0 ** -24 * (113 + V / 256)
+    want = 3.0 - math.log(math.exp(3.0) + math.exp(2.0) + math.exp(1.0) + V - 3)
+    assert abs(logp.item() - want) <= tol and (tl[0] - tl[0, 0]).tolist() == pytest.approx([0.0, -1.0, -2.0], abs=2.0 ** -19)
+    assert tl[0, 0] == logp[0] and bool(torch.isfinite(entropy).all())
+
+
 # ------------------------------------------------------------------------------------ refusals, streams, graphs
 def test_arguments_are_refused_with_a_reason():
     g = _gen(0)
