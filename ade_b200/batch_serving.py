@@ -153,7 +153,7 @@ class BatchDecoder:
         self._model_of = i32(R + 1, -1)
         self._tokens = torch.zeros(R + 1, width * page_size + 1, dtype=torch.long, device=dev)
         self._logprobs = torch.zeros(R + 1, width * page_size + 1, dtype=torch.float32, device=dev)
-        self._eos = torch.full((1,), -1, dtype=torch.long, device=dev)
+        self._eos = torch.full((R + 1,), -1, dtype=torch.long, device=dev)       # each request's own end token, -1: none
         self._route = getattr(model, "_ade_route", None)
         self._rows = i32(R, -1)                     # the route of a step's rows
         self._free_slots = list(range(R - 1, -1, -1))
@@ -199,7 +199,7 @@ class BatchDecoder:
         nxt = self._record(row, positions + 1, m.lm_head(h))
         # a request that has produced the end token rests
         stop = torch.cat((self.new_tokens, self.new_tokens[:1]))
-        stop[row] = (nxt != self._eos).int()
+        stop[row] = (nxt != self._eos[row]).int()
         self.new_tokens.copy_(torch.minimum(self.new_tokens, stop[:R]))
 
     @torch.no_grad()
@@ -238,9 +238,10 @@ class BatchDecoder:
         return paged_extend(self.lengths, grow, self.block_table, self.free_pages, self.free_count, rows, self.page_size, in_place=True)
 
     @torch.no_grad()
-    def add(self, prompt: torch.Tensor, model_id: int = -1) -> int:
+    def add(self, prompt: torch.Tensor, model_id: int = -1, eos_token_id: int | None = None) -> int:
         """Enter a request: run its prompt (token ids, at least one) through fine-tuned model `model_id` (-1: the base model), keep its keys
-        and values, and choose its first token.  Returns the request's number; raises when no request or page is free.  Synchronises."""
+        and values, and choose its first token.  With `eos_token_id` the request rests once it has produced that token.  Returns the
+        request's number; raises when no request or page is free.  Synchronises."""
         T = int(prompt.numel())
         if not 1 <= T < self.max_len:
             raise ValueError(f"a prompt has 1 to {self.max_len - 1} tokens")
@@ -268,9 +269,10 @@ class BatchDecoder:
                 paged_write(layer.keys[0].transpose(0, 1), layer.values[0].transpose(0, 1), slots, kp, vp)
             self.status[b] = 0
             self._model_of[b] = model_id
+            self._eos[b] = -1 if eos_token_id is None else eos_token_id
             self._tokens[b, :T], self._logprobs[b] = ids[0], 0.0
             self._record(torch.tensor([b], device=dev), T, out.logits[:, -1])
-            self.new_tokens[b] = (self._tok[b] != self._eos[0]).int()
+            self.new_tokens[b] = (self._tok[b] != self._eos[b]).int()
         return b
 
     @torch.no_grad()
@@ -303,11 +305,10 @@ class BatchDecoder:
             raise ValueError(f"prompt and answer have at most {self.max_len} tokens")
         if len(prompts) > len(self._free_slots):
             raise ValueError(f"{len(prompts)} prompts for {len(self._free_slots)} free requests")
-        self._eos.fill_(-1 if eos_token_id is None else eos_token_id)
         running = []
         try:
             for p, d in zip(prompts, models):
-                running.append(self.add(p, d))
+                running.append(self.add(p, d, eos_token_id))
             for _ in range(max_new_tokens - 1):
                 self.step()
             self.check_status()
@@ -320,4 +321,3 @@ class BatchDecoder:
         finally:
             for b in running:
                 self.finish(b)
-            self._eos.fill_(-1)

@@ -226,3 +226,35 @@ def test_a_finished_request_leaves_no_report_behind(served):
         dec.generate(prompts, 4, [0, 1, 2])
     (tokens, logprobs), = dec.generate(prompts[2:], 6, [2])
     _check_answer(single[2], tokens, logprobs, 5)
+
+
+def test_each_request_has_its_own_end_token(served):
+    """A request beside an answer with an end token goes on through that token, and one entered with an end token stops there."""
+    _, _, many = served
+    g = torch.Generator().manual_seed(10)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (12, 8)]
+
+    def run(eos):
+        dec = BatchDecoder(many, max_requests=3, max_len=64)
+        a, b = dec.add(prompts[0], 0), dec.add(prompts[0], 0, eos_token_id=eos)
+        dec.generate(prompts[1:], 8, [1], eos_token_id=eos)
+        for _ in range(10):
+            dec.step()
+        return dec, a, b, dec.tokens[a, 12:int(dec.lengths[a]) + 1].tolist()
+
+    plain = run(None)[3]
+    eos = next(t for i, t in enumerate(plain) if 3 <= i < 9 and t not in plain[:i])
+    dec, a, b, through = run(eos)
+    assert len(through) == len(plain) and int(dec.new_tokens[a]) == 1
+    stopped = dec.tokens[b, 12:int(dec.lengths[b]) + 1].tolist()
+    assert stopped == plain[:plain.index(eos) + 1] and int(dec.new_tokens[b]) == 0
+    dec.check_status()
+    # a number's former end token is forgotten; an answer's first token may be its last
+    dec.finish(b)
+    c = dec.add(prompts[1], 1)
+    begin = int(dec.tokens[c, 8])
+    assert c == b and int(dec._eos[c]) == -1
+    dec.finish(c)
+    c = dec.add(prompts[1], 1, eos_token_id=begin)
+    dec.step()
+    assert int(dec.new_tokens[c]) == 0 and int(dec.lengths[c]) == 8
