@@ -288,7 +288,11 @@ class BatchDecoder:
 
     def check_status(self) -> None:
         """Raise if a request could not grow: no page was left, or it reached max_len.  Synchronises."""
-        bad = [(b, s) for b, s in enumerate(self.status.tolist()) if s]
+        self._report(range(self.max_requests))
+
+    def _report(self, requests) -> None:
+        state = self.status.tolist()
+        bad = [(b, state[b]) for b in requests if state[b]]
         if bad:
             raise _lib.AdeKernelError("; ".join(f"request {b}: {_lib.PAGED_STATUS[s]}" for b, s in bad))
 
@@ -296,7 +300,8 @@ class BatchDecoder:
         """Answers of `max_new_tokens` tokens to a list of prompts, each by its own fine-tuned model (default: the base model), all at once.
 
         Returns a list of (token ids of prompt and answer, log probabilities of the answer's tokens).  With `eos_token_id` an answer ends
-        with that token.
+        with that token.  Requests that are running already rest meanwhile and go on with the next ``step``; whether they could grow
+        plays no part here.
         """
         models = [-1] * len(prompts) if models is None else list(models)
         if len(models) != len(prompts) or max_new_tokens < 1:
@@ -305,13 +310,14 @@ class BatchDecoder:
             raise ValueError(f"prompt and answer have at most {self.max_len} tokens")
         if len(prompts) > len(self._free_slots):
             raise ValueError(f"{len(prompts)} prompts for {len(self._free_slots)} free requests")
-        running = []
+        running, others = [], self.new_tokens.clone()
         try:
+            self.new_tokens.zero_()
             for p, d in zip(prompts, models):
                 running.append(self.add(p, d, eos_token_id))
             for _ in range(max_new_tokens - 1):
                 self.step()
-            self.check_status()
+            self._report(running)
             out = []
             for b, p in zip(running, prompts):
                 T = int(p.numel())
@@ -321,3 +327,4 @@ class BatchDecoder:
         finally:
             for b in running:
                 self.finish(b)
+            self.new_tokens.copy_(others)

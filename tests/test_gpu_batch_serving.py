@@ -258,3 +258,50 @@ def test_each_request_has_its_own_end_token(served):
     c = dec.add(prompts[1], 1, eos_token_id=begin)
     dec.step()
     assert int(dec.new_tokens[c]) == 0 and int(dec.lengths[c]) == 8
+
+
+def test_requests_that_run_already_rest_while_an_answer_is_generated(served):
+    """Lengths, histories and reports of requests that were entered before are what they would be without the answer, in the same company."""
+    base, single, many = served
+    g = torch.Generator().manual_seed(11)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (10, 16, 6)]
+
+    def run(answer):
+        dec = BatchDecoder(many, max_requests=4, max_len=48, pages=5, page_size=16)
+        a, b = dec.add(prompts[0], 0), dec.add(prompts[1], 1)
+        for _ in range(3):
+            dec.step()
+        if answer:
+            (tokens, logprobs), = dec.generate(prompts[2:], 9, [2], eos_token_id=int(dec.tokens[a, 12]))
+            assert tokens.numel() <= 15
+            _check_answer(single[2], tokens, logprobs, 6)
+        assert dec.lengths[:2].tolist() == [13, 19]
+        for _ in range(3):
+            dec.step()
+        assert dec.lengths[:2].tolist() == [16, 22]
+        return [t[[a, b]][:, 6:23].clone() for t in (dec.tokens, dec.logprobs)]
+
+    for without, beside in zip(run(False), run(True)):
+        assert torch.equal(without[0, :11], beside[0, :11]) and torch.equal(without[1], beside[1])
+    # a request that waits for a page does not spoil the answers of others, and is still reported afterwards
+    dec = BatchDecoder(many, max_requests=4, max_len=64, pages=3, page_size=16)
+    a, b = dec.add(prompts[1], 0), dec.add(prompts[1], 1)
+    for _ in range(17):
+        dec.step()                                        # one has the third page and has filled it by now
+    dec.finish(a if int(dec.lengths[a]) == 16 else b)
+    waits = b if a in dec._free_slots else a
+    assert int(dec.lengths[waits]) == 32
+    dec.add(prompts[2], -1)                               # takes the page that was handed back
+    dec.step()
+    with pytest.raises(AdeKernelError, match="NO_PAGE"):
+        dec.check_status()
+    c = next(r for r in range(4) if r not in dec._free_slots and r != waits)
+    dec.finish(c)
+    (tokens, logprobs), = dec.generate(prompts[2:], 5)
+    _check_answer(base, tokens, logprobs, 6)
+    with pytest.raises(AdeKernelError, match="NO_PAGE"):
+        dec.check_status()
+    # an answer that fails leaves the others as they were
+    with pytest.raises(AdeKernelError, match="NO_PAGE"):
+        dec.generate([torch.cat(prompts)[:30]], 5)
+    assert int(dec.new_tokens[waits]) == 1 and int(dec.new_tokens.sum()) == 1 and sorted(dec._free_slots) == [r for r in range(4) if r != waits]
