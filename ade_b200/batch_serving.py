@@ -182,7 +182,7 @@ class BatchDecoder:
         R, m, lm = self.max_requests, self.model, self.model.model
         slots, positions, requests, _, _, status = paged_extend(self.lengths, self.new_tokens, self.block_table, self.free_pages, self.free_count, R,
                                                                 self.page_size, in_place=True)
-        torch.maximum(self.status, status, out=self.status)
+        self.status.copy_(torch.where(self.new_tokens > 0, status, self.status))      # a request that found its page is well again
         row = torch.where(requests < 0, R, requests).long()
         self._rows.copy_(self._model_of[row])
         x = lm.embed_tokens(self._tok[row])
@@ -287,7 +287,7 @@ class BatchDecoder:
         self._free_slots.append(request)
 
     def check_status(self) -> None:
-        """Raise if a request could not grow: no page was left, or it reached max_len.  Synchronises."""
+        """Raise if a request could not grow when it last was to: no page was left, or it reached max_len.  Synchronises."""
         self._report(range(self.max_requests))
 
     def _report(self, requests) -> None:

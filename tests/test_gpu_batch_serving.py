@@ -305,3 +305,28 @@ def test_requests_that_run_already_rest_while_an_answer_is_generated(served):
     with pytest.raises(AdeKernelError, match="NO_PAGE"):
         dec.generate([torch.cat(prompts)[:30]], 5)
     assert int(dec.new_tokens[waits]) == 1 and int(dec.new_tokens.sum()) == 1 and sorted(dec._free_slots) == [r for r in range(4) if r != waits]
+
+
+def test_a_request_that_found_its_page_after_all_is_well(served):
+    _, single, many = served
+    g = torch.Generator().manual_seed(12)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (16, 16, 4)]
+    dec = BatchDecoder(many, max_requests=3, max_len=64, pages=3, page_size=16)
+    a, b = dec.add(prompts[0], 0), dec.add(prompts[1], 1)
+    for _ in range(3):
+        dec.step()
+    with pytest.raises(AdeKernelError, match="NO_PAGE"):
+        dec.check_status()
+    first, second = (a, b) if int(dec.lengths[a]) > 16 else (b, a)
+    dec.finish(first)
+    dec.new_tokens[second] = 0                            # resting: its last attempt failed, and that stays
+    dec.step()
+    with pytest.raises(AdeKernelError, match=f"request {second}: ADE_PAGED_NO_PAGE"):
+        dec.check_status()
+    dec.new_tokens[second] = 1
+    dec.step()
+    dec.check_status()
+    (tokens, logprobs), = dec.generate(prompts[2:], 5, [2])
+    _check_answer(single[2], tokens, logprobs, 4)
+    dec.check_status()
+    assert int(dec.lengths[second]) == 17
