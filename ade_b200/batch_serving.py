@@ -252,28 +252,37 @@ class BatchDecoder:
         dev, route = self.device, self._route
         with torch.cuda.device(dev):
             ids = prompt.reshape(1, T).to(device=dev, dtype=torch.long)
-            if route is not None:
-                before, route.ids = route.ids, None if model_id < 0 else torch.full((T,), model_id, dtype=torch.int32, device=dev)
-            try:
-                out = self.model(input_ids=ids, use_cache=True, logits_to_keep=1)
-            finally:
-                if route is not None:
-                    route.ids = before
             b = self._free_slots[-1]
             slots, _, _, _, _, status = self._extend(b, T, T)
             state = int(status[b])
             if state:
                 raise _lib.AdeKernelError(f"request {b}: {_lib.PAGED_STATUS[state]}")
-            self._free_slots.pop()
-            for layer, kp, vp in zip(out.past_key_values.layers, self.k_pages, self.v_pages):
-                paged_write(layer.keys[0].transpose(0, 1), layer.values[0].transpose(0, 1), slots, kp, vp)
-            self.status[b] = 0
-            self._model_of[b] = model_id
-            self._eos[b] = -1 if eos_token_id is None else eos_token_id
-            self._tokens[b, :T], self._logprobs[b] = ids[0], 0.0
-            self._record(torch.tensor([b], device=dev), T, out.logits[:, -1])
-            self.new_tokens[b] = (self._tok[b] != self._eos[b]).int()
+            try:
+                if route is not None:
+                    before, route.ids = route.ids, None if model_id < 0 else torch.full((T,), model_id, dtype=torch.int32, device=dev)
+                try:
+                    out = self.model(input_ids=ids, use_cache=True, logits_to_keep=1)
+                finally:
+                    if route is not None:
+                        route.ids = before
+                for layer, kp, vp in zip(out.past_key_values.layers, self.k_pages, self.v_pages):
+                    paged_write(layer.keys[0].transpose(0, 1), layer.values[0].transpose(0, 1), slots, kp, vp)
+                self._model_of[b] = model_id
+                self._eos[b] = -1 if eos_token_id is None else eos_token_id
+                self._tokens[b, :T], self._logprobs[b] = ids[0], 0.0
+                self._record(torch.tensor([b], device=dev), T, out.logits[:, -1])
+                self.new_tokens[b] = (self._tok[b] != self._eos[b]).int()
+            except BaseException:
+                self._release(b)
+                raise
+        self._free_slots.pop()
         return b
+
+    def _release(self, request: int) -> None:
+        """Hand a request's pages back and leave nothing of it behind."""
+        self._extend(request, -1, 0)
+        self.new_tokens[request] = self.status[request] = 0
+        self._model_of[request] = -1
 
     @torch.no_grad()
     def finish(self, request: int) -> None:
@@ -281,9 +290,7 @@ class BatchDecoder:
         if request in self._free_slots or not 0 <= request < self.max_requests:
             raise ValueError(f"request {request} is not running")
         with torch.cuda.device(self.device):
-            self._extend(request, -1, 0)
-            self.new_tokens[request] = self.status[request] = 0
-            self._model_of[request] = -1
+            self._release(request)
         self._free_slots.append(request)
 
     def check_status(self) -> None:

@@ -8,7 +8,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from ade_b200 import kernels, synth
+from ade_b200 import batch_serving, kernels, synth
 from ade_b200._lib import AdeKernelError
 from ade_b200.batch_serving import BatchDecoder, DeltaRoute, MultiDeltaLinear, attach_multi_deltas
 from ade_b200.serving import LINEAR_MODULE_NAMES, attach_kernel_linears
@@ -330,3 +330,36 @@ def test_a_request_that_found_its_page_after_all_is_well(served):
     _check_answer(single[2], tokens, logprobs, 4)
     dec.check_status()
     assert int(dec.lengths[second]) == 17
+
+
+@pytest.mark.parametrize("fails", ["paged_write", "token_logprobs", "model"])
+def test_a_request_that_fails_on_its_way_in_leaves_nothing_behind(served, monkeypatch, fails):
+    """Whatever raises behind the allocation of its pages: number, pages, length and the rows' models are as before."""
+    _, single, many = served
+    g = torch.Generator().manual_seed(13)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (20, 7)]
+    dec = BatchDecoder(many, max_requests=2, max_len=64, page_size=8)
+    a = dec.add(prompts[1], 0)
+    before = [t.clone() for t in (dec.lengths, dec.new_tokens, dec.status, dec.free_count, dec._model_of)]
+    taken = sorted(dec.free_pages[:int(dec.free_count)].tolist())
+
+    def broken(*args, **kw):
+        raise RuntimeError("planted")
+
+    with monkeypatch.context() as m:
+        if fails == "model":
+            m.setattr(many, "forward", broken)
+        else:
+            m.setattr(batch_serving, fails, broken)
+        for _ in range(3):
+            with pytest.raises(RuntimeError, match="planted"):
+                dec.add(prompts[0], 1)
+    assert many._ade_route.ids is None and dec._free_slots == [1]
+    for t, kept in zip((dec.lengths, dec.new_tokens, dec.status, dec.free_count, dec._model_of), before):
+        assert torch.equal(t, kept)
+    assert sorted(dec.free_pages[:int(dec.free_count)].tolist()) == taken
+    b = dec.add(prompts[0], 1)
+    for _ in range(6):
+        dec.step()
+    _check_answer(single[0], dec.tokens[a, :14].clone(), dec.logprobs[a, 7:14].clone(), 7)
+    _check_answer(single[1], dec.tokens[b, :27].clone(), dec.logprobs[b, 20:27].clone(), 20)
