@@ -132,13 +132,16 @@ class BatchDecoder:
             raise ValueError("BatchDecoder: rotary angles that change with the length would need the keys of a request anew")
         if not 1 <= max_requests <= MAX_REQUESTS or max_len < 1 or page_size < 1:
             raise ValueError(f"BatchDecoder: 1 to {MAX_REQUESTS} requests, max_len and page_size of at least 1")
+        cfg = model.config
+        head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+        if head_dim % 32 or not 32 <= head_dim <= 256:
+            raise ValueError(f"BatchDecoder: head dimensions that are a multiple of 32 up to 256 are expected; the model has {head_dim}")
         w = model.model.embed_tokens.weight
         if w.dtype != torch.bfloat16 or not w.is_cuda:
             raise ValueError("BatchDecoder: the model must be in bfloat16 on a CUDA device")
-        cfg, dev, R = model.config, w.device, max_requests
+        dev, R = w.device, max_requests
         self.model, self.max_requests, self.max_len, self.page_size, self.device = model, R, max_len, page_size, dev
-        self.heads, self.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
-        self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+        self.heads, self.kv_heads, self.head_dim = cfg.num_attention_heads, cfg.num_key_value_heads, head_dim
         width = -(-max_len // page_size)
         pages = R * width if pages is None else int(pages)
         shape = (pages, self.kv_heads, page_size, self.head_dim)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from ade_b200 import kernels, synth
-from ade_b200.batch_serving import DeltaRoute, MultiDeltaLinear, attach_multi_deltas
+from ade_b200.batch_serving import BatchDecoder, DeltaRoute, MultiDeltaLinear, attach_multi_deltas
 from ade_b200.serving import LINEAR_MODULE_NAMES
 
 
@@ -51,3 +51,13 @@ def test_a_bias_of_another_size_is_refused():
     for bias in (torch.zeros(128), torch.zeros(1), torch.zeros(32, 1)):
         with pytest.raises(ValueError, match="bias"):
             MultiDeltaLinear(torch.zeros(32, 128), [form], DeltaRoute(1), bias)
+
+
+@pytest.mark.parametrize("dim", [16, 48, 80, 100, 288])
+def test_head_dimensions_without_a_kernel_are_refused(dim):
+    with pytest.raises(ValueError, match=f"multiple of 32 up to 256.* {dim}"):
+        BatchDecoder(_llama(head_dim=dim), 2, 16)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        BatchDecoder(_llama(hidden_size=2 * dim), 2, 16)
+    with pytest.raises(ValueError, match="CUDA device"):             # the only thing wrong with this one
+        BatchDecoder(_llama(head_dim=96), 2, 16)
