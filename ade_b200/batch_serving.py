@@ -105,13 +105,27 @@ def attach_multi_deltas(model, base_state_dict: dict, per_model, device="cuda") 
     return swapped
 
 
+def _unheard(mod) -> bool:
+    """Nobody would notice that `mod` is not called for a step: no forward hooks of its own or for all modules, and the forward it came with or
+    ``enable_fused_decode_ops`` gave it.  The hooks with which transformers collects hidden states, once it was asked for them, stay on the
+    modules and do nothing in other calls."""
+    m = torch.nn.modules.module
+    hooks = [h for d in (mod._forward_hooks, mod._forward_pre_hooks, m._global_forward_hooks, m._global_forward_pre_hooks) for h in d.values()]
+    own = mod.__dict__
+    stock = lambda f: f is None or (getattr(f, "__func__", None) is type(mod).forward and f.__self__ is mod)
+    forward = own.get("forward")
+    return (all(getattr(h, "__module__", None) == "transformers.utils.output_capturing" for h in hooks)
+            and (stock(own.get("_ade_orig_forward")) if forward is own.get("_ade_forward") else stock(forward)))
+
+
 class BatchDecoder:
     """Greedy decoding of many requests of a transformers LLaMA causal LM in bfloat16 on a CUDA device.
 
     Linear modules may be MultiDeltaLinear (each request then has a model of its own), ADEKernelLinear or plain.  Device state of a
     request: its length, its row of the block table, its last token, and its history: `tokens` (max_requests, max_len) and `logprobs`, the
     log probability each generated token had.  The step is captured at the first call of ``step``: the model's modules and weights stay as they are
-    from then on.
+    from then on.  A step calls the embedding, the rotary embedding, the linear modules and the head, whose hooks run when it is captured and
+    not when it is replayed; it does the work of the other modules itself, so those have to be transformers' own and without hooks.
     """
 
     def __init__(self, model, max_requests: int, max_len: int, pages: int | None = None, page_size: int = 64):
@@ -126,8 +140,8 @@ class BatchDecoder:
 
         if not isinstance(model, ml.LlamaForCausalLM):
             raise ValueError("BatchDecoder: a LLaMA causal LM is expected")
-        if any(type(layer.mlp.act_fn).__name__ not in SILU_TYPES for layer in model.model.layers):
-            raise ValueError("BatchDecoder: MLPs with SiLU are expected")
+        self.model = model
+        self._check_modules()
         if model.model.rotary_emb.rope_type in ("dynamic", "longrope"):
             raise ValueError("BatchDecoder: rotary angles that change with the length would need the keys of a request anew")
         if not 1 <= max_requests <= MAX_REQUESTS or max_len < 1 or page_size < 1:
@@ -140,7 +154,7 @@ class BatchDecoder:
         if w.dtype != torch.bfloat16 or not w.is_cuda:
             raise ValueError("BatchDecoder: the model must be in bfloat16 on a CUDA device")
         dev, R = w.device, max_requests
-        self.model, self.max_requests, self.max_len, self.page_size, self.device = model, R, max_len, page_size, dev
+        self.max_requests, self.max_len, self.page_size, self.device = R, max_len, page_size, dev
         self.heads, self.kv_heads, self.head_dim = cfg.num_attention_heads, cfg.num_key_value_heads, head_dim
         width = -(-max_len // page_size)
         pages = R * width if pages is None else int(pages)
@@ -161,6 +175,21 @@ class BatchDecoder:
         self._rows = i32(R, -1)                     # the route of a step's rows
         self._free_slots = list(range(R - 1, -1, -1))
         self._graph = None
+
+    def _check_modules(self) -> None:
+        """Refuse a model whose modules do something that a step, which does not call them, would not do."""
+        from transformers.models.llama import modeling_llama as ml
+
+        passed_by = [("the model", self.model, ml.LlamaForCausalLM), ("model", self.model.model, ml.LlamaModel), ("model.norm", self.model.model.norm, ml.LlamaRMSNorm)]
+        for i, layer in enumerate(self.model.model.layers):
+            passed_by.append((f"model.layers.{i}", layer, ml.LlamaDecoderLayer))
+            passed_by += [(f"model.layers.{i}.{n}", getattr(layer, n, None), cls) for n, cls in
+                          (("self_attn", ml.LlamaAttention), ("mlp", ml.LlamaMLP), ("input_layernorm", ml.LlamaRMSNorm), ("post_attention_layernorm", ml.LlamaRMSNorm))]
+        for name, mod, cls in passed_by:
+            if not isinstance(mod, cls) or type(mod).forward is not cls.forward or not _unheard(mod):
+                raise ValueError(f"BatchDecoder: {name} has hooks or a forward of its own, which a step would not call")
+            if cls is ml.LlamaMLP and not (type(mod.act_fn).__name__ in SILU_TYPES and _unheard(mod.act_fn)):
+                raise ValueError(f"BatchDecoder: MLPs with SiLU are expected, without hooks; {name} has {type(mod.act_fn).__name__}")
 
     @property
     def tokens(self) -> torch.Tensor:
@@ -214,6 +243,7 @@ class BatchDecoder:
             self._graph.replay()
 
     def _capture(self):
+        self._check_modules()
         keep = self.new_tokens.clone()
         self.new_tokens.zero_()                     # warm-up and capture run without requests
         ids, route = None, self._route

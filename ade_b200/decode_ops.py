@@ -236,7 +236,7 @@ def enable_fused_decode_ops(model) -> int:
                 return mod._ade_orig_forward(hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
                                              past_key_values=past_key_values, **kw)
 
-            mod.forward = attn_forward
+            mod.forward = mod._ade_forward = attn_forward
             n += 1
         elif isinstance(mod, ml.LlamaRMSNorm) and not hasattr(mod, "_ade_orig_forward"):
             mod._ade_orig_forward = mod.forward
@@ -268,7 +268,7 @@ def enable_fused_decode_ops(model) -> int:
                     return mod.down_proj(mod.act_fn(g) * u)
                 return mod._ade_orig_forward(x)
 
-            mod.forward = mlp_forward
+            mod.forward = mod._ade_forward = mlp_forward
             n += 1
     # Residual connections: a decoder layer adds the attention output and the MLP output to its input, each time right in
     # front of an RMSNorm (its own post-attention norm; the next layer's input norm, or the model's final norm).  A
@@ -309,6 +309,6 @@ def enable_fused_decode_ops(model) -> int:
                 nxt._ade_pre = (s2, s2._version, h3)
                 return s2
 
-            layer.forward = layer_forward
+            layer.forward = layer._ade_forward = layer_forward
             n += 1
     return n

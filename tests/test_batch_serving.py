@@ -61,3 +61,87 @@ def test_head_dimensions_without_a_kernel_are_refused(dim):
         BatchDecoder(_llama(hidden_size=2 * dim), 2, 16)
     with pytest.raises(ValueError, match="CUDA device"):             # the only thing wrong with this one
         BatchDecoder(_llama(head_dim=96), 2, 16)
+
+
+def _hook(where, kind="register_forward_hook"):
+    return lambda m: getattr(m.get_submodule(where) if where else m, kind)(lambda *a: None)
+
+
+def _replace(where, change):
+    """`change`d copy of the module at `where` in its place."""
+    def edit(m):
+        owner, _, leaf = where.rpartition(".")
+        owner = m.get_submodule(owner)
+        setattr(owner, leaf, change(getattr(owner, leaf)))
+    return edit
+
+
+def _other_forward(where):
+    def edit(m):
+        mod = m.get_submodule(where) if where else m
+        forward = mod.forward
+        mod.forward = lambda *a, **kw: forward(*a, **kw)
+    return edit
+
+
+def _subclass(where):
+    def edit(m):
+        mod = m.get_submodule(where) if where else m
+        base = type(mod)
+        mod.__class__ = type("Own" + base.__name__, (base,), {"forward": lambda self, *a, **kw: base.forward(self, *a, **kw)})
+    return edit
+
+
+class _Wrapped(torch.nn.Module):
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, *a, **kw):
+        return self.inner(*a, **kw)
+
+
+PASSED_BY = ["", "model", "model.norm", "model.layers.1", "model.layers.0.self_attn", "model.layers.1.mlp", "model.layers.0.input_layernorm", "model.layers.1.post_attention_layernorm"]
+
+
+@pytest.mark.parametrize("where, change", [(w, c) for w in PASSED_BY for c in (_hook(w), _hook(w, "register_forward_pre_hook"), _other_forward(w), _subclass(w))]
+                         + [(w, _replace(w, _Wrapped)) for w in PASSED_BY[2:]] + [("model.layers.1.mlp", c("model.layers.1.mlp.act_fn")) for c in (_hook, _other_forward)])
+@pytest.mark.parametrize("fused", ["no", "before", "behind"])
+def test_modules_that_a_step_passes_by_have_to_be_the_stock_ones(where, change, fused):
+    """A step does the work of these modules itself: a hook, another forward, a subclass or a wrapper in their place would act on prompts alone."""
+    from ade_b200.decode_ops import enable_fused_decode_ops
+
+    model = _llama()
+    if fused == "before":
+        enable_fused_decode_ops(model)
+    change(model)
+    if fused == "behind" and not isinstance(model.model.layers[1], _Wrapped):      # which asks every layer for its norms
+        enable_fused_decode_ops(model)
+    with pytest.raises(ValueError, match=f"{where or 'the model'} has") as e:
+        BatchDecoder(model, 2, 16)
+    assert "CUDA" not in str(e.value)
+
+
+def test_hooks_for_all_modules_are_seen():
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+    try:
+        with pytest.raises(ValueError, match="hooks"):
+            BatchDecoder(_llama(), 2, 16)
+    finally:
+        handle.remove()
+
+
+@pytest.mark.parametrize("change", [
+    lambda m: None, lambda m: m(input_ids=torch.arange(3)[None], output_hidden_states=True), _hook("model.layers.0.self_attn.q_proj"), _hook("lm_head"), _hook("model.embed_tokens"),
+    _replace("lm_head", _Wrapped), _replace("model.layers.0.mlp.up_proj", _Wrapped)])
+@pytest.mark.parametrize("fused", [False, True])
+def test_what_a_step_calls_may_be_anything(change, fused):
+    """Nothing is wrong with these but where they are: linear modules, head and embedding are called; transformers' own hooks collect nothing."""
+    from ade_b200.decode_ops import enable_fused_decode_ops
+
+    model = _llama()
+    if fused:
+        enable_fused_decode_ops(model)
+    change(model)
+    with pytest.raises(ValueError, match="CUDA device"):
+        BatchDecoder(model, 2, 16)

@@ -11,6 +11,7 @@ import torch.nn.functional as F
 from ade_b200 import batch_serving, kernels, synth
 from ade_b200._lib import AdeKernelError
 from ade_b200.batch_serving import BatchDecoder, DeltaRoute, MultiDeltaLinear, attach_multi_deltas
+from ade_b200.decode_ops import enable_fused_decode_ops
 from ade_b200.serving import LINEAR_MODULE_NAMES, attach_kernel_linears
 
 pytestmark = pytest.mark.gpu
@@ -363,3 +364,28 @@ def test_a_request_that_fails_on_its_way_in_leaves_nothing_behind(served, monkey
         dec.step()
     _check_answer(single[0], dec.tokens[a, :14].clone(), dec.logprobs[a, 7:14].clone(), 7)
     _check_answer(single[1], dec.tokens[b, :27].clone(), dec.logprobs[b, 20:27].clone(), 20)
+
+
+def test_hooks_are_looked_for_again_before_the_step_is_captured(served):
+    """A hook on a module that a step does not call is refused, whenever it came; the framework's and transformers' own changes are not."""
+    base, _, _ = served
+    g = torch.Generator().manual_seed(14)
+    prompt = torch.randint(0, VOCAB, (9,), generator=g)
+    model = copy.deepcopy(base)
+    dec = BatchDecoder(model, 2, 48)
+    a = dec.add(prompt)
+    handle = model.model.layers[1].register_forward_hook(lambda mod, args, out: out * 2)
+    for _ in range(2):
+        with pytest.raises(ValueError, match=r"model\.layers\.1 has hooks"):
+            dec.step()
+    assert int(dec.lengths[a]) == 9 and int(dec.new_tokens[a]) == 1
+    handle.remove()
+    enable_fused_decode_ops(model)
+    with torch.no_grad():
+        assert len(model(input_ids=prompt[None].to(DEV), output_hidden_states=True).hidden_states) == 3
+    for _ in range(5):
+        dec.step()
+    _check_answer(base, dec.tokens[a, :15].clone(), dec.logprobs[a, 9:15].clone(), 9)
+    dec.finish(a)
+    for tokens, logprobs in BatchDecoder(model, 2, 48).generate([prompt, prompt[:3]], 7):
+        _check_answer(base, tokens, logprobs, tokens.numel() - 7)
