@@ -185,9 +185,12 @@ class BatchDecoder:
             passed_by.append((f"model.layers.{i}", layer, ml.LlamaDecoderLayer))
             passed_by += [(f"model.layers.{i}.{n}", getattr(layer, n, None), cls) for n, cls in
                           (("self_attn", ml.LlamaAttention), ("mlp", ml.LlamaMLP), ("input_layernorm", ml.LlamaRMSNorm), ("post_attention_layernorm", ml.LlamaRMSNorm))]
+        dev = self.model.model.embed_tokens.weight.device
         for name, mod, cls in passed_by:
             if not isinstance(mod, cls) or type(mod).forward is not cls.forward or not _unheard(mod):
                 raise ValueError(f"BatchDecoder: {name} has hooks or a forward of its own, which a step would not call")
+            if cls is ml.LlamaRMSNorm and (mod.weight.dtype != torch.bfloat16 or mod.weight.device != dev or not mod.weight.is_contiguous()):
+                raise ValueError(f"BatchDecoder: {name} must be in bfloat16 on {dev}, not {mod.weight.dtype} on {mod.weight.device}")
             if cls is ml.LlamaMLP and not (type(mod.act_fn).__name__ in SILU_TYPES and _unheard(mod.act_fn)):
                 raise ValueError(f"BatchDecoder: MLPs with SiLU are expected, without hooks; {name} has {type(mod.act_fn).__name__}")
 
@@ -210,6 +213,13 @@ class BatchDecoder:
         self._logprobs[row, at] = logp
         return nxt
 
+    def _plain(self, *tensors):
+        """What a module returned, if the launches, which take it by its address, can read it."""
+        for t in tensors:
+            if t.dtype != torch.bfloat16 or t.device != self.device or t.stride(-1) != 1:
+                raise ValueError(f"BatchDecoder: modules that return bfloat16 on {self.device} are expected; one returned {t.dtype} on {t.device}")
+        return tensors if len(tensors) > 1 else tensors[0]
+
     def _forward_step(self):
         R, m, lm = self.max_requests, self.model, self.model.model
         slots, positions, requests, _, _, status = paged_extend(self.lengths, self.new_tokens, self.block_table, self.free_pages, self.free_count, R,
@@ -217,7 +227,7 @@ class BatchDecoder:
         self.status.copy_(torch.where(self.new_tokens > 0, status, self.status))      # a request that found its page is well again
         row = torch.where(requests < 0, R, requests).long()
         self._rows.copy_(self._model_of[row])
-        x = lm.embed_tokens(self._tok[row])
+        x = self._plain(lm.embed_tokens(self._tok[row]))
         cos, sin = (t[0].contiguous() for t in lm.rotary_emb(x[None], positions[None]))
         norms = [layer.input_layernorm for layer in lm.layers[1:]] + [lm.norm]
         h = rmsnorm(x, lm.layers[0].input_layernorm.weight, lm.layers[0].input_layernorm.variance_epsilon)
@@ -226,8 +236,9 @@ class BatchDecoder:
             q, k, v = (p(h).view(R, -1, self.head_dim) for p in (a.q_proj, a.k_proj, a.v_proj))
             paged_write(k, v, slots, kp, vp, cos, sin)
             ctx = paged_attn_decode(q, self.block_table, requests, positions, kp, vp, a.scaling, cos, sin)
-            x, h = add_rmsnorm(a.o_proj(ctx), x, post.weight, post.variance_epsilon)
-            x, h = add_rmsnorm(layer.mlp.down_proj(silu_mul(layer.mlp.gate_proj(h), layer.mlp.up_proj(h))), x, nxt.weight, nxt.variance_epsilon)
+            x, h = add_rmsnorm(self._plain(a.o_proj(ctx)), x, post.weight, post.variance_epsilon)
+            act = silu_mul(*self._plain(layer.mlp.gate_proj(h), layer.mlp.up_proj(h)))
+            x, h = add_rmsnorm(self._plain(layer.mlp.down_proj(act)), x, nxt.weight, nxt.variance_epsilon)
         nxt = self._record(row, positions + 1, m.lm_head(h))
         # a request that has produced the end token rests
         stop = torch.cat((self.new_tokens, self.new_tokens[:1]))

@@ -145,3 +145,13 @@ def test_what_a_step_calls_may_be_anything(change, fused):
     change(model)
     with pytest.raises(ValueError, match="CUDA device"):
         BatchDecoder(model, 2, 16)
+
+
+@pytest.mark.parametrize("where", ["model.norm", "model.layers.0.input_layernorm", "model.layers.1.post_attention_layernorm"])
+@pytest.mark.parametrize("change", [torch.float32, torch.float16, "meta"])
+def test_norms_of_another_type_or_device_are_refused(where, change):
+    """Their launches read the weights as bfloat16 of the model's device, by their address."""
+    model = _llama()
+    model.get_submodule(where).to(change)
+    with pytest.raises(ValueError, match=f"{where} must be in bfloat16"):
+        BatchDecoder(model, 2, 16)

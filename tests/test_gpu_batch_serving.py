@@ -389,3 +389,15 @@ def test_hooks_are_looked_for_again_before_the_step_is_captured(served):
     dec.finish(a)
     for tokens, logprobs in BatchDecoder(model, 2, 48).generate([prompt, prompt[:3]], 7):
         _check_answer(base, tokens, logprobs, tokens.numel() - 7)
+
+
+@pytest.mark.parametrize("where", ["model.layers.0.self_attn.o_proj", "model.layers.1.mlp.gate_proj", "model.layers.1.mlp.up_proj", "model.layers.0.mlp.down_proj", "model.embed_tokens"])
+def test_modules_that_return_another_type_are_refused(served, where):
+    """The launches of a step take what modules return by its address; a type that they do not have is refused before the first of them."""
+    _, _, many = served
+    model = copy.deepcopy(many)
+    model.get_submodule(where).register_forward_hook(lambda mod, args, out: out.float())
+    dec = BatchDecoder(model, 2, 48)
+    with pytest.raises(ValueError, match="return bfloat16"):
+        dec.step()
+    assert dec._graph is None and int(dec.lengths.sum()) == 0
