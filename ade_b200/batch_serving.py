@@ -159,8 +159,9 @@ class BatchDecoder:
         width = -(-max_len // page_size)
         pages = R * width if pages is None else int(pages)
         shape = (pages, self.kv_heads, page_size, self.head_dim)
-        self.k_pages = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(cfg.num_hidden_layers)]
-        self.v_pages = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(cfg.num_hidden_layers)]
+        layers = min(cfg.num_hidden_layers, len(model.model.layers))            # the model runs the first num_hidden_layers of its layers
+        self.k_pages = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(layers)]
+        self.v_pages = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(layers)]
         i32 = lambda n, v=0: torch.full((n,), v, dtype=torch.int32, device=dev)
         self.block_table = torch.full((R, width), -1, dtype=torch.int32, device=dev)
         self.free_pages, self.free_count = torch.arange(pages, dtype=torch.int32, device=dev), i32(1, pages)
@@ -229,9 +230,10 @@ class BatchDecoder:
         self._rows.copy_(self._model_of[row])
         x = self._plain(lm.embed_tokens(self._tok[row]))
         cos, sin = (t[0].contiguous() for t in lm.rotary_emb(x[None], positions[None]))
-        norms = [layer.input_layernorm for layer in lm.layers[1:]] + [lm.norm]
-        h = rmsnorm(x, lm.layers[0].input_layernorm.weight, lm.layers[0].input_layernorm.variance_epsilon)
-        for layer, nxt, kp, vp in zip(lm.layers, norms, self.k_pages, self.v_pages):
+        layers = lm.layers[:len(self.k_pages)]
+        norms = [layer.input_layernorm for layer in layers[1:]] + [lm.norm]
+        h = rmsnorm(x, layers[0].input_layernorm.weight, layers[0].input_layernorm.variance_epsilon)
+        for layer, nxt, kp, vp in zip(layers, norms, self.k_pages, self.v_pages):
             a, post = layer.self_attn, layer.post_attention_layernorm
             q, k, v = (p(h).view(R, -1, self.head_dim) for p in (a.q_proj, a.k_proj, a.v_proj))
             paged_write(k, v, slots, kp, vp, cos, sin)

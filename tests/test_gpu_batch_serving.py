@@ -401,3 +401,22 @@ def test_modules_that_return_another_type_are_refused(served, where):
     with pytest.raises(ValueError, match="return bfloat16"):
         dec.step()
     assert dec._graph is None and int(dec.lengths.sum()) == 0
+
+
+@pytest.mark.parametrize("configured, kept", [(1, 2), (2, 1)])
+def test_a_model_of_fewer_layers_than_it_has_or_says(configured, kept):
+    """transformers runs the first num_hidden_layers of a model's layers, and the final norm behind the last of those."""
+    model = _llama()
+    model.config.num_hidden_layers = configured
+    model.model.layers = model.model.layers[:kept]
+    g = torch.Generator().manual_seed(15)
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if "norm" in n:
+                p.copy_(1 + 0.5 * torch.randn(p.shape, generator=g))
+    model = model.to(DEV)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (6, 19)]
+    dec = BatchDecoder(model, 2, 48)
+    assert len(dec.k_pages) == 1
+    for tokens, logprobs in dec.generate(prompts, 9):
+        _check_answer(model, tokens, logprobs, tokens.numel() - 9)
