@@ -335,6 +335,9 @@ int ade_b200_attn_decode(const void* q, const void* k, const void* v, const void
  *   ade_b200_multi_delta   out[t] = y_dense[t] + U_d^ (V_d^^T x[t]) with d = ids[t], each row of x [T][N], y_dense and out [T][M]
  *                  (contiguous; out may be y_dense) with the delta of its own fine-tuned model; ids outside 0 .. deltas - 1: y_dense alone.
  *                  T <= ADE_B200_MAX_TOKENS, M and N <= 2^21, N % 128 == 0.  ids and the bank's start are read on the device.
+ *                  Two operands are rounded on the way, to fixed point of 16 bits: x vs of a row and rank group relative to the largest
+ *                  of each 128 columns, and h = V^^T x relative to the largest of each 128 ranks, off by half of 2^-14 of the power of
+ *                  two at or below that at most.  Products with the codes are exact, sums of them float32, the output is rounded once.
  *
  *   ade_b200_token_logprobs  from logits [rows][vocab] (rows row_stride apart; ADE_DTYPE_*): logprobs[r] = log softmax of token
  *                  tokens[r] (negative: none, 0; vocab or more: NaN; tokens and logprobs both NULL: left out), entropy[r] of the

@@ -401,6 +401,78 @@ def test_each_row_gets_its_own_delta(M, N, ranks, ids):
     _check_delta(M, N, ranks, ids, seed=M + N)
 
 
+def _grid(m):
+    """The step of the fixed point in which values of magnitude up to m are held: 2^-14 of the power of two at or below 1.004 m."""
+    return torch.exp2(torch.floor(torch.log2((1.004 * m).clamp(min=2.0 ** -100))) - 14)
+
+
+def _delta_spread(x, packed):
+    """(U^ V^^T x, covariance (rows, M, M) of what the two fixed-point roundings put a row's outputs off) in float64 for rows of one delta.
+
+    A value rounded to a grid of step s is off by s / sqrt(12), independently of the others.  x vs of each column, rank group and row is rounded on the
+    grid of its 128 columns, h of each rank and row on that of its 128 ranks; the codes carry both to the outputs: U V e and U f."""
+    p = {k: v.to(DEV).double() for k, v in packed.items()}
+    x, M = x.double(), p["U_codes"].shape[0]
+    out = torch.zeros(x.shape[0], M, dtype=torch.float64, device=DEV)
+    cov = torch.zeros(x.shape[0], M, M, dtype=torch.float64, device=DEV)
+    for g in range(p["Vt_scale"].shape[0]):
+        ranks = slice(128 * g, 128 * g + 128)
+        U = (p["U_codes"][:, ranks] - p["U_zero"][:, g:g + 1]) * p["U_scale"][:, g:g + 1]
+        V = p["Vt_codes"][ranks] - p["Vt_zero"][g]
+        xs = x * p["Vt_scale"][g]
+        h = xs @ V.t()
+        out += h @ U.t()
+        step = _grid(xs.abs().view(x.shape[0], -1, 128).amax(-1)).repeat_interleave(128, 1)
+        step_h = _grid(h.abs().amax(-1))
+        ranks_cov = torch.einsum("kn,tn,jn->tkj", V, step ** 2 / 12, V) + step_h[:, None, None] ** 2 / 12 * torch.eye(128, dtype=torch.float64, device=DEV)
+        cov += U @ ranks_cov @ U.t()
+    return out, cov
+
+
+@pytest.mark.parametrize("T", [3, 8, 40])
+@pytest.mark.parametrize("M, N, r, kind", [(512, 1024, 256, "normal"), (512, 1024, 256, "columns"), (300, 2176, 384, "one column"), (512, 1024, 256, "ranks"), (264, 4096, 128, "all"),
+                                           (128, 128, 128, "normal")])
+def test_deltas_are_as_exact_as_their_fixed_point(M, N, r, kind, T):
+    """The shared term takes away what the delta rounds to, so the output shows what is left of it some nine bits finer.
+
+    With columns of x that are a hundred to a thousand times larger than the others, and ranks of V^ whose h lies apart by more than two decades."""
+    packed = synth.random_packed(M, N, r, seed=M + N + r, device=DEV)
+    g = _gen(T + N)
+    x = torch.randn(T, N, generator=g, device=DEV)
+    if kind in ("columns", "all"):
+        x[:, 7::101] *= 100.0
+        x[:, 50::499] *= 1000.0
+    if kind == "one column":
+        x[:, 1000] = 1000.0
+    x = x.to(torch.bfloat16)
+    if kind in ("ranks", "all"):
+        # a third of the ranks hardly look at x and one looks just where that of the first row is: h from near nothing to as large as it can be
+        packed["Vt_zero"] = packed["Vt_zero"].clamp(max=14)
+        rank = torch.arange(r, device=DEV)[:, None]
+        little = packed["Vt_zero"].long().repeat_interleave(128, 0) + torch.randint(0, 2, (r, N), generator=g, device=DEV)
+        codes = torch.where(rank % 3 == 0, little, packed["Vt_codes"].long())
+        packed["Vt_codes"] = torch.where(rank % 128 == 5, torch.where(x[0] > 0, 15, 0), codes).to(torch.uint8)
+    want, cov = _delta_spread(x, packed)
+    y = (-want).to(torch.bfloat16)
+    left = want + y.double()
+    got = multi_delta_forward(x, y, bank_deltas([kernels.pack_int4(packed)]), _i32([0] * T)).double()
+    # What else is rounded: the output (a uniform error of a step of bfloat16 of what is left, with its error) and float32 sums of N / 128 and r / 128
+    # terms.  Codes less their zero-points do not average to zero, so the outputs of a row share most of their error: its root mean square is
+    # that of about one number a rank group.  So it is measured by its covariance C: off^T C^-1 off has the mean M and, for sums of many roundings, the
+    # deviation sqrt(2 M); over the rows, which err independently, six deviations are allowed.  x vs has 16 significant bits, so those in the grid's
+    # top binade can only be off by nothing or half a step, evenly: step^2 / 8 instead of step^2 / 12.  Of 128 normal values whose largest is 2.7
+    # deviations at most one in six lies there (above 1.35): 1 + 0.5 / 6 = 1.1 of the mean.  A float64 model of the two roundings gives 1.0 to 1.2; with
+    # one bit less in x vs or in h it gives 1.3 to 3.1, 1.6 to 1.9 and more for normal values, and 2.4 to 3.4 with one bit less in both.
+    variance = cov.diagonal(dim1=1, dim2=2)
+    ulp = torch.exp2(torch.floor(torch.log2(torch.maximum(left.abs(), variance.sqrt()))) - 7)
+    other = ulp ** 2 / 12 + ((N / 128 + r / 128 + 4) * 2.0 ** -24 * want.abs().amax(1, keepdim=True)) ** 2
+    off = got - left
+    solved = torch.linalg.solve_triangular(torch.linalg.cholesky(cov + torch.diag_embed(other)), off[..., None], upper=False)[..., 0]
+    size = float(solved.square().mean())
+    assert size <= 1.1 * (1 + 6 * math.sqrt(2 / (M * T))), size
+    assert bool((off.abs() <= 7 * (variance + other).sqrt()).all())
+
+
 def test_rows_of_one_delta_match_the_single_delta_path():
     """The factored kernel on the rows of each delta: both are within the factored path's tolerance of each other."""
     M, N, ranks, ids = 512, 1024, [256, 512], [0, 1, 1, 0, 1, 0, 0]
