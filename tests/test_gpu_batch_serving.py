@@ -420,3 +420,29 @@ def test_a_model_of_fewer_layers_than_it_has_or_says(configured, kept):
     assert len(dec.k_pages) == 1
     for tokens, logprobs in dec.generate(prompts, 9):
         _check_answer(model, tokens, logprobs, tokens.numel() - 9)
+
+
+def test_more_requests_than_one_launch_of_the_deltas_takes(served):
+    """A captured step of 150 rows: the deltas in two launches a module, pages and rows by one CTA of 512 threads; a few rest, a few have left."""
+    base, single, many = served
+    g = torch.Generator().manual_seed(16)
+    R = 150
+    dec = BatchDecoder(many, max_requests=R, max_len=32, page_size=4)
+    free = int(dec.free_count)
+    prompts = [torch.randint(0, VOCAB, (1 + i % 6,), generator=g) for i in range(R)]
+    models = [i % 4 - 1 for i in range(R)]
+    assert [dec.add(p, d) for p, d in zip(prompts, models)] == list(range(R))
+    for i in (0, 40, 127):
+        dec.finish(i)
+    dec.new_tokens[60:63] = 0
+    for _ in range(11):
+        dec.step()
+    dec.check_status()
+    gone, rest = {0, 40, 127}, {60, 61, 62}
+    assert dec.lengths.tolist() == [0 if i in gone else prompts[i].numel() + (0 if i in rest else 11) for i in range(R)]
+    for i in (1, 2, 3, 60, 126, 128, 129, 130, R - 1):
+        n, more = prompts[i].numel(), 0 if i in rest else 11
+        _check_answer(base if models[i] < 0 else single[models[i]], dec.tokens[i, :n + more + 1].clone(), dec.logprobs[i, n:n + more + 1].clone(), n)
+    for i in set(range(R)) - gone:
+        dec.finish(i)
+    assert int(dec.free_count) == free

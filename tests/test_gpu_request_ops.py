@@ -200,6 +200,23 @@ def test_write_puts_rows_into_their_slots(T, heads, dim, ps, layout, rope):
     assert bool(((kp.double() - want_k).abs() <= 2.0 ** -8 * want_k.abs() + 3 * 2.0 ** -24 * 2 * k.abs().max().double()).all())
 
 
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("slot", [0, 9, 34])
+def test_write_of_a_single_row(slot, odd):
+    g = _gen(slot)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)
+    k, v = (rnd(1, 3 * 64 + 2)[:, odd:odd + 192].view(1, 3, 64) for _ in range(2))
+    cos, sin = _angles(1, 64, g)
+    kp, vp = rnd(5, 3, 7, 64), rnd(5, 3, 7, 64)
+    want_k, want_v, before = kp.double(), vp.clone(), kp.clone()
+    want_k[slot // 7, :, slot % 7] = _rot64(k, cos, sin)[0]
+    want_v[slot // 7, :, slot % 7] = v[0]
+    paged_write(k, v, torch.tensor([slot], device=DEV), kp, vp, cos, sin)
+    assert torch.equal(vp, want_v) and int((kp != before).any(-1).sum()) == 3
+    # as above: one rounding of the result, three of products and their sum
+    assert bool(((kp.double() - want_k).abs() <= 2.0 ** -8 * want_k.abs() + 3 * 2.0 ** -24 * 2 * k.abs().max().double()).all())
+
+
 # ------------------------------------------------------------------------------------ paged_attn_decode
 def _attend64(q, table, requests, positions, kp, vp, scale, cos, sin):
     """Row by row in float64: (out, magnitude of the weighted sum, largest magnitude of a score) of every row and head."""
@@ -281,6 +298,31 @@ def test_attention_over_pages(hq, hk, dim, ps, lengths):
                                                       ([70] * 150, 8, 2, 64, 16), ([1] * 300, 4, 4, 32, 8), ([30000, 5], 16, 16, 128, 256)])
 def test_attention_split_over_long_caches_and_many_rows(lengths, hq, hk, dim, ps):
     _check_attn(_attn_case(len(lengths), hq, hk, dim, ps, lengths, seed=len(lengths)))
+
+
+@pytest.mark.parametrize("T", [1024, 1025, 2100])
+def test_attention_of_more_rows_than_one_launch_takes(T):
+    """Launches of up to 1024 rows share the workspace, one behind the other; rows at their ends with and without positions."""
+    lengths = [(t * 37) % 91 for t in range(T)]
+    lengths[1022:1026] = [300, 0, 300, 0][:T - 1022]
+    c = _attn_case(T, 2, 1, 32, 16, lengths, seed=T)
+    got = _check_attn(c)
+    for t in (0, 1, 1023, T - 1):                                     # by itself: the same but for the order of sums
+        one = {**c, **{n: c[n][t:t + 1].contiguous() for n in ("q", "requests", "positions", "cos", "sin")}}
+        assert float((got[t].double() - _check_attn(one)[0].double()).abs().max()) <= 2 * 2.0 ** -8 * float(got[t].double().abs().max())
+
+
+def test_attention_over_a_table_so_wide_that_a_launch_takes_fewer_rows():
+    """Places of 1024 rows as long as this table allows would not fit 31 bits: two launches for a thousand rows of two short requests."""
+    c = _attn_case(2, 8, 8, 64, 64, [150, 97], seed=12)
+    table = torch.full((2, 70000), -1, dtype=torch.int32, device=DEV)
+    table[:, :c["block_table"].shape[1]] = c["block_table"]
+    g = _gen(13)
+    T = 1000
+    c.update(q=torch.randn(T, 8, 64, generator=g, device=DEV).to(torch.bfloat16), block_table=table, requests=_i32([t % 2 for t in range(T)]),
+             positions=torch.tensor([t % (150 if t % 2 == 0 else 97) for t in range(T)], device=DEV))
+    c["cos"], c["sin"] = _angles(T, 64, g)
+    _check_attn(c)
 
 
 def test_attention_weights_that_one_position_takes():
@@ -399,6 +441,16 @@ def _check_delta(M, N, ranks, ids, seed):
     (400, 256, [128] * 40, list(range(40)) + [-1] * 3), (2048, 640, [512, 128, 1024], [(i * 7) % 4 - 1 for i in range(127)]), (16, 128, [128], [-1, -1])], ids=lambda v: str(v)[:40])
 def test_each_row_gets_its_own_delta(M, N, ranks, ids):
     _check_delta(M, N, ranks, ids, seed=M + N)
+
+
+@pytest.mark.parametrize("K", [127, 128, 130, 300])
+def test_banks_of_many_deltas(K):
+    """Up to 127 deltas their first rank groups are kept beside the rows, beyond that they are looked up."""
+    T = 128
+    ids = [(t * 7) % K for t in range(T)]
+    ids[5:9] = [K - 1, 0, K, -1]
+    ids[60:70] = [K - 1] * 10
+    _check_delta(24, 256, [128 * (1 + i % 2) for i in range(K)], ids, seed=K)
 
 
 def _grid(m):
