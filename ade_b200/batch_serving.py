@@ -123,7 +123,8 @@ class BatchDecoder:
 
     Linear modules may be MultiDeltaLinear (each request then has a model of its own), ADEKernelLinear or plain.  Device state of a
     request: its length, its row of the block table, its last token, and its history: `tokens` (max_requests, max_len) and `logprobs`, the
-    log probability each generated token had.  The step is captured at the first call of ``step``: the model's modules and weights stay as they are
+    log probability each generated token had.  Keys of a prompt are rotated by the model's forward (bfloat16, three roundings), those of
+    generated tokens by ``paged_write`` (float32, one rounding).  The step is captured at the first call of ``step``: the model's modules and weights stay as they are
     from then on.  A step calls the embedding, the rotary embedding, the linear modules and the head, whose hooks run when it is captured and
     not when it is replayed; it does the work of the other modules itself, so those have to be transformers' own and without hooks.
     """

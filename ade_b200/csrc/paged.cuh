@@ -21,8 +21,6 @@ __device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
 }
 
 // ------------------------------------------------------------------ page allocation, block tables, slot maps
-constexpr int PX_MAX_REQUESTS = 4096;
-
 struct ExtendParams {
     const int* lengths;          // [B] tokens each request has
     const int* fresh;            // [B] tokens to add; negative: the request ends and its pages go back

@@ -146,7 +146,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
 
     Returns:
         (logprobs (rows,) or empty without tokens, entropy (rows,), top_logprobs (rows, top), top_tokens (rows, top) int64); floats in
-        float32, natural logarithms.  Equal logits come in the order of their tokens.  There is no backward pass: logits that
+        float32, natural logarithms.  Equal logits come in the order of their tokens.  The four share one allocation: whoever keeps,
+        saves or resizes one of them by itself takes a clone.  There is no backward pass: logits that
         require a gradient are refused outside ``torch.no_grad()``.
     """
     return _call("token_logprobs", logits, tokens, top)

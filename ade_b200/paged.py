@@ -38,7 +38,9 @@ def paged_extend(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: t
         (slots, positions, requests, lengths, free_count, status): for each of the `total` rows the slot (page * page_size + offset, int64),
         the position in its request (int64) and the request (int32); rows behind the last token, and those of a request that
         could not grow, have slot -1, position 0, request -1.  status (B,) int32 is 0, or a key of ``_lib.PAGED_STATUS`` that says
-        why the request did not grow; its length then stays as it was.
+        why the request did not grow; its length then stays as it was.  Where `total` is too small, every request behind the first
+        that did not fit has ADE_PAGED_NO_ROW, one without new tokens too.  The returned tensors share one allocation: whoever
+        keeps, saves or resizes one of them by itself takes a clone.
     """
     out = _call("paged_extend", lengths, new_tokens, block_table, free_pages, free_count, total, page_size, in_place)
     return (*out[:3], lengths, free_count, out[5]) if in_place else out
@@ -49,8 +51,8 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     """Keys and values of new tokens into the pages of one layer.
 
     k and v are (rows, kv_heads, head_dim) bfloat16 views with a contiguous last dimension and any other strides; slots (rows,) int64 from
-    `paged_extend`.  With cos and sin, (rows, head_dim), keys are rotated as the model does it, in float32 and rounded once; without,
-    they are stored as they are.  Rows whose slot is no place of the cache are left out.  head_dim: a multiple of 32 up to 256.
+    `paged_extend`.  With cos and sin, (rows, head_dim), keys are rotated in float32 and rounded once (transformers rotates in bfloat16
+    and rounds three times, so last bits differ from its cache); without, they are stored as they are.  Rows whose slot is no place of the cache are left out.  head_dim: a multiple of 32 up to 256.
     """
     _call("paged_write", k, v, slots, k_pages, v_pages, cos, sin)
 

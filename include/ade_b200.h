@@ -317,7 +317,8 @@ int ade_b200_attn_decode(const void* q, const void* k, const void* v, const void
  *                  row of 0 .. total - 1: its slot, its position in the request, its request; rows behind the last one, and those
  *                  of a request that could not grow, get slot -1, position 0, request -1.  status[b]: ADE_PAGED_OK, or why
  *                  request b did not grow (its length then stays): ADE_PAGED_NO_PAGE (the stack does not reach to it),
- *                  ADE_PAGED_TABLE_FULL (width * page_size), ADE_PAGED_NO_ROW (its rows do not end within `total`),
+ *                  ADE_PAGED_TABLE_FULL (width * page_size), ADE_PAGED_NO_ROW (its rows do not end within `total`: that
+ *                  request and all behind it that do not end, those without new tokens, which have nothing to lose, included),
  *                  ADE_PAGED_BAD_LENGTH (negative, or beyond its row of the table; nothing is handed back either).  lengths_out
  *                  and free_count_out may be lengths and free_count; work: 16-byte aligned, ade_b200_paged_extend_workspace_bytes(B, total)
  *                  bytes, contents of no meaning before and after the call; it may be NULL where that function returns 0, which depends
