@@ -12,7 +12,7 @@ from ade_b200 import batch_serving, kernels, synth
 from ade_b200._lib import AdeKernelError
 from ade_b200.batch_serving import BatchDecoder, DeltaRoute, MultiDeltaLinear, attach_multi_deltas
 from ade_b200.decode_ops import enable_fused_decode_ops
-from ade_b200.serving import LINEAR_MODULE_NAMES, attach_kernel_linears
+from ade_b200.serving import LINEAR_MODULE_NAMES, attach_kernel_linears, fuse_kernel_linears
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -446,3 +446,15 @@ def test_more_requests_than_one_launch_of_the_deltas_takes(served):
     for i in set(range(R)) - gone:
         dec.finish(i)
     assert int(dec.free_count) == free
+
+
+def test_fused_groups_of_a_single_model_are_served_too(served):
+    """q/k/v and gate/up of a layer as one launch each, next to the other fused operations: prompts through their forwards, steps past them."""
+    _, single, _ = served
+    model = copy.deepcopy(single[1])
+    g = torch.Generator().manual_seed(17)
+    prompts = [torch.randint(0, VOCAB, (n,), generator=g) for n in (7, 40, 1)]
+    assert fuse_kernel_linears(model) > 0
+    enable_fused_decode_ops(model)
+    for tokens, logprobs in BatchDecoder(model, 4, 64, page_size=8).generate(prompts, 10):
+        _check_answer(single[1], tokens, logprobs, tokens.numel() - 10)
