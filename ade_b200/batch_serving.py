@@ -251,10 +251,15 @@ class BatchDecoder:
     @torch.no_grad()
     def step(self) -> None:
         """One token for every request whose `new_tokens` is 1; no host synchronisation once the first call has captured the step."""
+        self._check_route()
         with torch.cuda.device(self.device):
             if self._graph is None:
                 self._graph = self._capture()
             self._graph.replay()
+
+    def _check_route(self) -> None:
+        if getattr(self.model, "_ade_route", None) is not self._route:
+            raise ValueError("BatchDecoder: the model was given other deltas since; it needs a decoder of its own for them")
 
     def _capture(self):
         self._check_modules()
@@ -296,6 +301,7 @@ class BatchDecoder:
             raise ValueError(f"there is no fine-tuned model {model_id}")
         if not self._free_slots:
             raise ValueError(f"all {self.max_requests} requests are taken")
+        self._check_route()
         dev, route = self.device, self._route
         with torch.cuda.device(dev):
             ids = prompt.reshape(1, T).to(device=dev, dtype=torch.long)

@@ -458,3 +458,23 @@ def test_fused_groups_of_a_single_model_are_served_too(served):
     enable_fused_decode_ops(model)
     for tokens, logprobs in BatchDecoder(model, 4, 64, page_size=8).generate(prompts, 10):
         _check_answer(single[1], tokens, logprobs, tokens.numel() - 10)
+
+
+def test_a_decoder_serves_the_deltas_it_was_made_for(served):
+    """Deltas attached anew have a route of their own, which the decoder would not set: requests of fine-tuned models would get the base's answers."""
+    base, single, many = served
+    model = copy.deepcopy(many)
+    g = torch.Generator().manual_seed(18)
+    prompt = torch.randint(0, VOCAB, (9,), generator=g)
+    early, used, plain = BatchDecoder(model, 2, 48), BatchDecoder(model, 2, 48), BatchDecoder(copy.deepcopy(base), 2, 48)
+    a = used.add(prompt, 0)
+    used.step()
+    sd = {k: v.clone() for k, v in base.state_dict().items()}
+    attach_multi_deltas(model, sd, [_deltas(sd, 2), _deltas(sd, 1)], device=DEV)
+    attach_multi_deltas(plain.model, sd, [_deltas(sd, 2)], device=DEV)
+    for call in (lambda: early.add(prompt, 0), early.step, lambda: used.add(prompt, 0), used.step, lambda: plain.add(prompt), plain.step, lambda: early.generate([prompt], 3, [0])):
+        with pytest.raises(ValueError, match="other deltas"):
+            call()
+    used.finish(a)
+    (tokens, logprobs), = BatchDecoder(model, 2, 48).generate([prompt], 8, [1])
+    _check_answer(single[0], tokens, logprobs, 9)
