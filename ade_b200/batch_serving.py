@@ -302,6 +302,9 @@ class BatchDecoder:
         if not self._free_slots:
             raise ValueError(f"all {self.max_requests} requests are taken")
         self._check_route()
+        words = self.model.model.embed_tokens.weight.shape[0]
+        if int(prompt.min()) < 0 or int(prompt.max()) >= words:
+            raise ValueError(f"a prompt's token ids are 0 to {words - 1}")
         dev, route = self.device, self._route
         with torch.cuda.device(dev):
             ids = prompt.reshape(1, T).to(device=dev, dtype=torch.long)

@@ -478,3 +478,18 @@ def test_a_decoder_serves_the_deltas_it_was_made_for(served):
     used.finish(a)
     (tokens, logprobs), = BatchDecoder(model, 2, 48).generate([prompt], 8, [1])
     _check_answer(single[0], tokens, logprobs, 9)
+
+
+@pytest.mark.parametrize("where", ["cpu", DEV])
+def test_token_ids_that_the_embedding_does_not_have_are_refused(served, where):
+    """On the host: the embedding's own look-up would end the process's CUDA context."""
+    base, _, _ = served
+    dec = BatchDecoder(base, 2, 48)
+    free = int(dec.free_count)
+    for bad in ([0, VOCAB], [-1, 3], [2 ** 40], [5, -2 ** 31, 7]):
+        with pytest.raises(ValueError, match=f"0 to {VOCAB - 1}"):
+            dec.add(torch.tensor(bad, device=where))
+    assert int(dec.free_count) == free and dec._free_slots == [1, 0]
+    a = dec.add(torch.tensor([0, VOCAB - 1], device=where))
+    dec.step()
+    _check_answer(base, dec.tokens[a, :4].clone(), dec.logprobs[a, 2:4].clone(), 2)
