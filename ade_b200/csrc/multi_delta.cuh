@@ -72,7 +72,9 @@ struct MdEntries {
     int wsum[8], wcost[8];
 };
 
-// What a tile of the second launch costs with an entry of so many rank groups and rows, in about 25 cycles of a warp.
+// What a tile of the second launch costs with an entry of so many rank groups and rows, in about 25 cycles of a warp.  128 rows of 48 deltas of 256 to 768
+// ranks, 11008 x 4096, calls back to back in a graph: 47.7 us; 50.3 if entries of more than four rows cost the same as the others, 56.4 with one cost for all; 47.8 with 14 instead of 11.
+// 128 rows of 24 deltas, 4096 x 4096: 25.1, 25.4, 26.5, 25.3; 40 rows of 30, 4096 x 11008: 30.2, 30.8, 30.8, 30.1; 64 rows of 8, or all of one delta: the same.
 __device__ __forceinline__ int md_u_cost(int ng, int rows) { return ng == 0 ? 10 : rows <= 4 ? ng * 8 + 7 : ng * 11 + 6; }
 
 constexpr size_t md_v_smem() { return 8 * 2 * MD_THREADS * 16 + 8 * MD_ENTRY * MD_PART * sizeof(float) + 8 * 384; }

@@ -14,7 +14,8 @@
 // launch joins those parts in the order of the tiles.  A CTA whose tiles all belong to one pair joins its warps' parts itself.
 //
 // Long rows are bound by memory: 32 rows of 16 to 4000 positions, 32 heads of 128 (0.41 GB) take 81 us, 3 rows of up to 60 000 positions on 8 heads for 32
-// queries (0.47 GB) 87 us, 5.0 and 5.3 TB/s, of which 4 us are set-up and 3 the join.  Short ones are bound by two launches and what depends on
+// queries (0.47 GB) 87 us, 5.0 and 5.3 TB/s, of which 4 us are set-up and 3 the join.  At 256 dimensions four warps of a CTA have registers for the sums
+// and spill 232 bytes: the first case with 16 heads of 256, the same bytes, takes 131 us (3.4 TB/s).  Short rows are bound by two launches and what depends on
 // what in them: lengths, table, keys, parts.
 #pragma once
 #include "paged.cuh"
@@ -25,7 +26,11 @@ namespace ade {
 constexpr int PA_MAX_CTAS = 160;           // one CTA per SM; bounds the workspace
 constexpr int PA_MAX_ROWS = 1024;          // rows of one launch (their prefix sums lie in shared memory); the places of a launch fit 31 bits
 constexpr int PA_HEADS = 8;                // query heads that share one pass over the keys and values
-constexpr int PA_GAP = 3;                  // places of the line in front of a pair's tiles (0: 119 us, 2: 80.8, 3: 80.4, 5: 81.7 with 32 rows of 16 to 4000 positions)
+// Places of the line in front of a pair's tiles.  With 0, 2, 3, 5, 8 of them, us: 32 rows of 16 to 4000 positions, 32 heads of 128: 103, 81.5, 82.2, 81.6, 83.4;
+// 64 rows of 100 to 2000, 8 heads of 64: 27.0, 25.8, 26.1, 26.2, 27.0; 16 rows of 100 to 8000, 8 heads of 128 for 32 queries: 37.0, 37.2, 37.1, 36.9,
+// 36.6; 24 rows of 50 to 3000, 2 heads of 256 for 16: 34.2, 31.6, 31.1, 31.3, 30.8; 48 rows of 16 to 2000, 3 heads of 96 for 48: 27.7, 22.1, 22.2, 22.2, 22.5;
+// 8 rows of 20 to 200, 32 heads of 128: 14.7, 12.4, 12.8, 12.8, 13.6.
+constexpr int PA_GAP = 3;
 
 struct PagedAttnParams {
     const __nv_bfloat16 *q, *cs, *sn;          // q [T][q_heads][dim] by strides; cs, sn [T][dim] or nullptr: q is used as it is
